@@ -509,6 +509,96 @@ MCA_API int mca_decode_attention_static(const float* q, const float* k_new, cons
                                         int seq_len, int max_len, const float* freq_real, const float* freq_imag,
                                         float* out, void* stream);
 
+/* ---- 2b. paged key/value cache ---------------------------------------------------------------- */
+/* New tokens of many sequences over a cache made of pages: prompts, chunks of prompts and single tokens in one call.  No
+ * counterpart in the reference, whose llama2 route takes one token of one sequence over a contiguous cache
+ * (CudaExtension.llm32.llama2/Files/llama2_gpu.cpp:32-111); the arithmetic is that of its attention and rope
+ * (llama2_cpu.cpp:239-342).  Nothing here allocates, synchronises or copies; every call may be captured into a CUDA graph.
+ *
+ * A page holds page_size consecutive positions of one sequence: k_pages and v_pages are (n_pages, page_size, n_kv_heads,
+ * head_size), contiguous within a page, page_stride elements from one page to the next (of one layer's slice of a larger
+ * pool, for instance).  page_size: a power of two, 16 to 65536.  head_size: 32, 48, 64, 96 or 128.  Query head h reads
+ * key/value head h / (n_heads / n_kv_heads).  Pages are 16-byte aligned, page_stride a multiple of 16 bytes.
+ * page_table (n_seqs, table_stride): the page of positions [i page_size, (i + 1) page_size) of each sequence; the tables of two
+ * sequences may name the same page (a shared prefix), as long as neither appends to it.  -1: the page is not held any more
+ * (evicted): its keys are left out.  Any other id outside [0, n_pages) is left out too, and mca_paged_status reports it. */
+typedef struct McaPagedCache {
+  void* k_pages;
+  void* v_pages;
+  int64_t page_stride;
+  int n_pages, page_size, n_heads, n_kv_heads, head_size;
+  int dtype;               /* of the pages: MCA_DTYPE_F32 or MCA_DTYPE_BF16 */
+} McaPagedCache;
+/* The new tokens of a step: those of sequence b are rows [starts[b], starts[b+1]) of the token tensors, the last of its
+ * lengths[b] positions (so lengths counts them: token i of the sequence has position lengths[b] - (starts[b+1] - starts[b]) + i).
+ * starts rises from 0 on; a sequence may have none.  Rows behind starts[n_seqs], up to n_tokens, are not read and not written.
+ * starts, lengths and page_table are device memory; what the host knows of them is an upper bound: no sequence has more than max_new
+ * new tokens or max_len positions (max_len <= table_stride * page_size).  A sequence outside these bounds, or with fewer positions
+ * than new tokens, is refused on the device: nothing of it is read or stored, those of its rows that lie below n_tokens are zero, and
+ * mca_paged_status reports it. */
+typedef struct McaPagedBatch {
+  const int* starts;       /* (n_seqs + 1) */
+  const int* lengths;      /* (n_seqs) */
+  const int* page_table;
+  int table_stride, n_seqs, n_tokens, max_new, max_len;
+} McaPagedBatch;
+/* Norm of each head and rotation by position, y = R(position) (w o x / sqrt(mean(x^2) + eps)).  MCA_QK_NORM: with the norm; the
+ * weights are (head_size) floats shared by the heads, or null: ones.  Tables (table_len, head_size / 2) as mca_rope_tables_host
+ * builds them, or both null: no rotation.  MCA_ROPE_HALVES: pair p is (x[p], x[p + head_size / 2]); else the reference's (x[2p],
+ * x[2p+1]) (rope.cu:724-864). */
+#define MCA_QK_NORM 1
+#define MCA_ROPE_HALVES 2
+typedef struct McaQkRotation {
+  const float* q_weight;
+  const float* k_weight;
+  const float* cos_table;
+  const float* sin_table;
+  int table_len;
+  int flags;
+  float eps;
+} McaQkRotation;
+/* A (B, T, heads, head_size) view: head_size contiguous, the other strides in elements.  Base 16-byte aligned, strides multiples of
+ * 16 bytes.  Where there are token rows instead of (B, T), stride_b is not used. */
+typedef struct McaHeads {
+  void* data;
+  int64_t stride_b, stride_t, stride_h;
+} McaHeads;
+
+/* The norm and rotation for training.  q (B,T,n_heads,D) and k (B,T,n_kv_heads,D) -> q_out, k_out, fp32 or bf16 (dtype), arithmetic
+ * in fp32 with one rounding at the end.  positions: (B,T) device ints, or null: 0 .. T-1 of every batch item (then T <= table_len); a
+ * position outside the tables gives a zero row, which mca_paged_status reports.  An output may be its own input (same data and
+ * strides); other overlaps are not allowed.  D: a multiple of 16 up to 256.  k (and k_out, dk_out, dk) may be null with n_kv_heads 0. */
+MCA_API int mca_qk_norm_rope_forward(const McaQkRotation* rotation, const McaHeads* q, const McaHeads* k, const int* positions, int dtype,
+                                     int B, int T, int n_heads, int n_kv_heads, int D, const McaHeads* q_out, const McaHeads* k_out,
+                                     void* stream);
+/* Its backward from the forward's inputs and the gradients of its outputs: g = R^T dy, dw = sum over all rows of g o xhat,
+ * dx = inv (g o w - xhat mean(g o w o xhat)) with xhat = x inv, inv = 1 / sqrt(mean(x^2) + eps).  dq_weight, dk_weight: (D) floats
+ * each or null (null without MCA_QK_NORM).  scratch: mca_qk_norm_rope_backward_scratch_floats(D) floats where a weight gradient is
+ * asked for.  Sums run in a fixed order.  dq may be dq_out, dk dk_out (same data and strides). */
+MCA_API int64_t mca_qk_norm_rope_backward_scratch_floats(int D);
+MCA_API int mca_qk_norm_rope_backward(const McaQkRotation* rotation, const McaHeads* q, const McaHeads* k, const int* positions,
+                                      const McaHeads* dq_out, const McaHeads* dk_out, int dtype, int B, int T, int n_heads,
+                                      int n_kv_heads, int D, const McaHeads* dq, const McaHeads* dk, float* dq_weight, float* dk_weight,
+                                      float* scratch, int64_t scratch_floats, void* stream);
+/* The norm and rotation of the new tokens' queries into q_out, of their keys into their pages, and their values into theirs, in one
+ * launch.  q, q_out (n_tokens, n_heads, D), k, v (n_tokens, n_kv_heads, D) in dtype; a bf16 dtype needs a bf16 cache.  A position
+ * outside the tables, or a token whose page is not held, is not stored (a zero query in the first case) and reported.  q_out may be q. */
+MCA_API int mca_paged_append(const McaPagedCache* cache, const McaPagedBatch* batch, const McaQkRotation* rotation, int dtype,
+                             const McaHeads* q, const McaHeads* k, const McaHeads* v, const McaHeads* q_out, void* stream);
+/* Attention of the new tokens over their sequences' pages, the new tokens' own keys among them (append first):
+ * out_t = sum over j <= position(t) of softmax_j(scale q_t . k_j) v_j; scale 0: 1 / sqrt(head_size).  A token with no key left has a
+ * zero row.  q, out (n_tokens, n_heads, D) in dtype: fp32 activations over an fp32 or a bf16 cache (fp32 accuracy), or bf16 over
+ * bf16.  out must not overlap q or the pages.  workspace: mca_paged_attention_workspace_bytes bytes, 16-byte aligned (0: none is
+ * needed; -1: arguments that mca_paged_attention refuses); two calls that may overlap, two captured graphs among them, need one each. */
+MCA_API int64_t mca_paged_attention_workspace_bytes(const McaPagedCache* cache, const McaPagedBatch* batch, int dtype);
+MCA_API int mca_paged_attention(const McaPagedCache* cache, const McaPagedBatch* batch, int dtype, const McaHeads* q, float scale,
+                                const McaHeads* out, void* workspace, int64_t workspace_bytes, void* stream);
+/* Reads and clears the status words of the calls above on the current device (blocking; call after the stream has been
+ * synchronised): status4[0] = 0, or what was refused first: 1 a sequence's lengths (status4[1] = the sequence, [2] = its length), 2 a
+ * page id ([1] = the sequence, [2] = the id), 3 a position outside the tables ([1] = the token row, [2] = the position), 4 a bounded
+ * wait of the attention kernel gave up ([1] = the stage, [2] = the block): its output is not complete; status4[3] = how many. */
+MCA_API int mca_paged_status(int* status4);
+
 /* TFT interpretable attention forward.  Replaces the attention block of
  * MultiHeadAttentionInterpLayer<T>.forward, MyCaffe.layers.tft/layers.tft/
  * MultiHeadAttentionInterpLayer.cs:728-759.  q (B,H,Nq,d), k (B,H,Nk,d), v (B,Nk,d) shared by the

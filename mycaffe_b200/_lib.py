@@ -92,6 +92,13 @@ SIGNATURES = {
     "mca_llama_forward": (_i, [_vp, _vp, _vp, _vp, _vp, _i, _i, _vp, _vp]),
     "mca_decode_static_scratch_floats": (_i64, []),
     "mca_decode_attention_static": (_i, [_vp, _vp, _vp, _vp, _vp, _i, _i64, _vp, _i, _i, _i, _i, _i, _i, _vp, _vp, _vp, _vp]),
+    "mca_qk_norm_rope_forward": (_i, [_vp, _vp, _vp, _vp, _i, _i, _i, _i, _i, _i, _vp, _vp, _vp]),
+    "mca_qk_norm_rope_backward_scratch_floats": (_i64, [_i]),
+    "mca_qk_norm_rope_backward": (_i, [_vp, _vp, _vp, _vp, _vp, _vp, _i, _i, _i, _i, _i, _i, _vp, _vp, _vp, _vp, _vp, _i64, _vp]),
+    "mca_paged_append": (_i, [_vp, _vp, _vp, _i, _vp, _vp, _vp, _vp, _vp]),
+    "mca_paged_attention_workspace_bytes": (_i64, [_vp, _vp, _i]),
+    "mca_paged_attention": (_i, [_vp, _vp, _i, _vp, C.c_float, _vp, _vp, _i64, _vp]),
+    "mca_paged_status": (_i, [C.POINTER(_i)]),
     "mca_tft_attention_forward_f32": (_i, [_vp, _vp, _vp, _vp, _i, _i, _i, _i, _i, _vp, _vp, _vp]),
     "mca_tft_attention_backward_f32": (_i, [_vp, _vp, _vp, _vp, _vp, _vp, _i, _i, _i, _i, _i, _vp, _vp, _vp, _vp]),
     "mca_layernorm_forward_f32": (_i, [_vp, _vp, _vp, _i64, _i, C.c_float, _vp]),

@@ -7,7 +7,7 @@
 // the array it reads is its own device's.
 #pragma once
 
-enum McaFailWord : int { MCA_FAIL_TC = 0, MCA_FAIL_DECODE = 1, MCA_FAIL_PROJ = 2, MCA_FAIL_WORDS = 4 };
+enum McaFailWord : int { MCA_FAIL_TC = 0, MCA_FAIL_DECODE = 1, MCA_FAIL_PROJ = 2, MCA_FAIL_PAGED = 3, MCA_FAIL_WORDS = 4 };
 constexpr int MCA_FAIL_DEVICES = 64;
 
 struct McaFailTable {

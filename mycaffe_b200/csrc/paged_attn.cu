@@ -1,0 +1,938 @@
+// Attention of new tokens -- prompts, chunks, single tokens, any mix of them -- over a cache made of pages.
+//
+//   out_t = sum_j p_tj v_j / sum_j p_tj,  p_tj = exp(scale q_t . k_j - m_t),  j = 0 .. position(t)
+//
+// in one pass over the keys with the running maximum and sum.  The query heads that share a key/value head are rows of one
+// tile (row = token x group + head), so that a page is read once for all of them.  Three kernels:
+//
+//   paged_tc_kernel      bf16 pages: S = Q K^T and O += P V on the tensor cores (tcgen05, TMEM), pages by TMA.
+//   paged_simt_kernel    fp32 activations: exact fp32 products, a lane group per cache row.
+//   paged_join_kernel    where few rows meet a long cache the keys are cut into splits, joined here by their maxima and sums.
+#include <algorithm>
+#include <mutex>
+
+#define MCA_TU_FAIL_FAMILY MCA_FAIL_PAGED
+#include "paged_common.cuh"
+#include "tc_common.cuh"
+
+namespace {
+
+using paged::Batch;
+using paged::Sequence;
+
+constexpr float LOG2E = 1.4426950408889634f;
+
+__device__ int g_wait_status[4];   // what a bounded wait of the tensor-core kernel leaves (see tc_common.cuh)
+
+struct AttnArgs {
+  Batch batch;
+  const char* q;            // (token, head) rows
+  char* out;
+  int64_t q_st, q_sh, out_st, out_sh;   // bytes
+  const char *k_pages, *v_pages;
+  int64_t page_bytes, row_bytes;
+  int n_heads, n_kv, group, hs;
+  int split_len, nsplit, tiles;
+  float scale_log2;         // scale x log2(e): the softmax runs on powers of two
+  float* part_acc;          // (n_tokens, n_heads, nsplit, hs)
+  float* part_ml;           // (n_tokens, n_heads, nsplit, 2): reference point (log2), sum
+};
+
+// Tile -> sequence and its first row; every lane of the warp takes part.  Tiles of a sequence: its rows (new tokens x group) in
+// steps of R; a sequence that is refused has none.
+__device__ __forceinline__ bool find_tile(const Batch& t, int group, int R, int tile, int* seq, int* row0, Sequence* out) {
+  const int lane = threadIdx.x & 31;
+  int before = 0;
+  for (int s0 = 0; s0 < t.n_seqs; s0 += 32) {
+    const int b = s0 + lane;
+    Sequence s{0, 0, 0, false};
+    if (b < t.n_seqs) s = paged::sequence(t, b);
+    const int n = s.good ? (s.count * group + R - 1) / R : 0;
+    int incl = n;
+#pragma unroll
+    for (int o = 1; o < 32; o <<= 1) {
+      const int up = __shfl_up_sync(0xffffffffu, incl, o);
+      if (lane >= o) incl += up;
+    }
+    const unsigned past = __ballot_sync(0xffffffffu, before + incl > tile);
+    if (past != 0) {
+      const int src = __ffs(past) - 1;
+      *seq = s0 + src;
+      *row0 = (tile - before - __shfl_sync(0xffffffffu, incl - n, src)) * R;
+      out->start = __shfl_sync(0xffffffffu, s.start, src);
+      out->count = __shfl_sync(0xffffffffu, s.count, src);
+      out->length = __shfl_sync(0xffffffffu, s.length, src);
+      out->good = true;
+      return true;
+    }
+    before += __shfl_sync(0xffffffffu, incl, 31);
+  }
+  return false;
+}
+
+// What one CTA more than the tiles does: reports the sequences that are refused and writes zeros over their rows.
+template <typename T> __device__ void look_over(const AttnArgs& p) {
+  for (int b = 0; b < p.batch.n_seqs; ++b) {
+    const Sequence s = paged::sequence(p.batch, b);
+    if (s.good) continue;
+    if (threadIdx.x == 0) paged::refuse(paged::REFUSED_LENGTHS, b, s.length);
+    const int lo = max(s.start, 0), hi = min(p.batch.starts[b + 1], p.batch.n_tokens);
+    const int64_t n = (int64_t)max(hi - lo, 0) * p.n_heads * p.hs;
+    for (int64_t i = threadIdx.x; i < n; i += blockDim.x) {
+      const int e = (int)(i % p.hs), h = (int)(i / p.hs % p.n_heads), t = lo + (int)(i / p.hs / p.n_heads);
+      reinterpret_cast<T*>(p.out + t * p.out_st + h * p.out_sh)[e] = T(0.f);
+    }
+  }
+}
+
+// Page of a position, or -1 where it is not held (or no page of the pool: `tell` says who reports that).
+__device__ __forceinline__ int page_of(const Batch& t, int seq, int pos, bool tell) {
+  const int id = t.table[(int64_t)seq * t.table_stride + (pos >> t.page_shift)];
+  if (id >= 0 && id < t.n_pages) return id;
+  if (tell && id != -1) paged::refuse(paged::REFUSED_PAGE, seq, id);
+  return -1;
+}
+
+// ---------------------------------------------------------------------------------------------------------------------
+// fp32 activations: exact fp32 products
+// ---------------------------------------------------------------------------------------------------------------------
+constexpr int SIMT_THREADS = 256, SIMT_WARPS = SIMT_THREADS / 32;
+
+// Elements of a row one lane holds: a group of HS / EPL lanes (a power of two) covers a row with 16-byte pieces.
+template <typename CT, int HS> struct Lanes {
+  static constexpr int VEC = 16 / (int)sizeof(CT);
+  static constexpr int EPL = HS % 48 == 0 ? (VEC == 4 ? 12 : 24) : 16;
+  static constexpr int G = HS / EPL;
+  static constexpr int NV = EPL / VEC;
+  static constexpr int STAGES = NV <= 2 ? 6 : (NV == 3 ? 4 : 3);   // row steps in flight: 96 KB a CTA
+  static constexpr size_t RING = (size_t)SIMT_WARPS * STAGES * 2 * NV * 32 * 16;
+};
+template <typename CT> __device__ __forceinline__ void unpack16(const uint4& t, float* x) {
+  const uint32_t w[4] = {t.x, t.y, t.z, t.w};
+#pragma unroll
+  for (int i = 0; i < 4; ++i) {
+    if constexpr (sizeof(CT) == 4) {
+      x[i] = __uint_as_float(w[i]);
+    } else {
+      x[2 * i] = __uint_as_float(w[i] << 16);
+      x[2 * i + 1] = __uint_as_float(w[i] & 0xffff0000u);
+    }
+  }
+}
+
+template <typename CT, int HS, int R>
+__global__ void __launch_bounds__(SIMT_THREADS, R <= 2 ? 2 : 1) paged_simt_kernel(const AttnArgs p) {
+  using L = Lanes<CT, HS>;
+  constexpr int G = L::G, EPL = L::EPL, NV = L::NV, VEC = L::VEC, STAGES = L::STAGES, RPW = 32 / G;
+  __shared__ float s_acc[SIMT_WARPS][R][HS];
+  __shared__ float s_ml[SIMT_WARPS][R][2];
+  extern __shared__ __align__(16) uint4 ring[];
+  mca_pdl_launch_dependents();
+  mca_pdl_wait();
+  if ((int)blockIdx.x == p.tiles) {
+    if (blockIdx.y == 0 && blockIdx.z == 0) look_over<float>(p);
+    return;
+  }
+  int seq, row0;
+  Sequence sq;
+  if (!find_tile(p.batch, p.group, R, blockIdx.x, &seq, &row0, &sq)) return;
+  const int kvh = blockIdx.y, split = blockIdx.z;
+  const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
+  const int gl = lane % G, g = lane / G;
+  const int rows = min(R, sq.count * p.group - row0);
+  const int pos0 = sq.length - sq.count;               // position of the sequence's first new token
+  const int r_begin = split * p.split_len;
+  const int last = pos0 + (row0 + rows - 1) / p.group;  // the last key any row sees
+  if (r_begin > last) return;
+  const int r_end = min(last + 1, r_begin + p.split_len);
+
+  float q[R][EPL], m[R], l[R], acc[R][EPL];
+  int lim[R];
+#pragma unroll
+  for (int x = 0; x < R; ++x) {
+    const int row = row0 + min(x, rows - 1), t = row / p.group, h = kvh * p.group + row - t * p.group;
+    lim[x] = x < rows ? pos0 + t : -1;
+    const float* src = reinterpret_cast<const float*>(p.q + (int64_t)(sq.start + t) * p.q_st + h * p.q_sh);
+    m[x] = -INFINITY; l[x] = 0.f;
+#pragma unroll
+    for (int c = 0; c < NV; ++c)
+#pragma unroll
+      for (int i = 0; i < VEC; i += 4) {
+        const float4 v = mca_ld_f4(src + (c * G + gl) * VEC + i);
+        q[x][c * VEC + i] = v.x * p.scale_log2; q[x][c * VEC + i + 1] = v.y * p.scale_log2;
+        q[x][c * VEC + i + 2] = v.z * p.scale_log2; q[x][c * VEC + i + 3] = v.w * p.scale_log2;
+      }
+#pragma unroll
+    for (int i = 0; i < EPL; ++i) acc[x][i] = 0.f;
+  }
+
+  // Each lane copies exactly the 16-byte pieces that it consumes itself, so its own wait_group is all the synchronisation.
+  uint4* my = ring + (size_t)warp * STAGES * 2 * NV * 32 + lane;
+  const uint32_t my_s = (uint32_t)__cvta_generic_to_shared(my);
+  const int first = r_begin + warp * RPW + g;
+  constexpr int STRIDE = SIMT_WARPS * RPW;
+  const int n_steps = (r_end - r_begin - warp * RPW + STRIDE - 1) / STRIDE;   // of the warp; not positive: none
+  const int64_t head_off = (int64_t)kvh * HS * sizeof(CT);
+  const int in_page = (1 << p.batch.page_shift) - 1;
+  unsigned held = 0;   // of the steps in flight, whether this lane's row is there (a shift register, the newest at bit 0)
+  auto issue = [&](int t) {
+    const int row = first + t * STRIDE;
+    int page = -1;
+    if (t < n_steps && row < r_end) page = page_of(p.batch, seq, row, gl == 0 && kvh == 0);
+    held = held << 1 | (page >= 0 ? 1u : 0u);
+    if (page >= 0) {
+      const uint32_t dst = my_s + (uint32_t)((t % STAGES) * 2 * NV * 32 * 16);
+      const int64_t off = page * p.page_bytes + (int64_t)(row & in_page) * p.row_bytes + head_off + gl * 16;
+#pragma unroll
+      for (int c = 0; c < NV; ++c) {
+        mca_cp_async16(dst + (uint32_t)(c * 32 * 16), p.k_pages + off + c * G * 16);
+        mca_cp_async16(dst + (uint32_t)((NV + c) * 32 * 16), p.v_pages + off + c * G * 16);
+      }
+    }
+    mca_cp_async_commit();
+  };
+#pragma unroll
+  for (int t = 0; t < STAGES - 1; ++t) issue(t);
+  for (int t = 0; t < n_steps; ++t) {
+    issue(t + STAGES - 1);
+    mca_cp_async_wait<STAGES - 1>();
+    const int row = first + t * STRIDE;
+    const bool valid = (held >> (STAGES - 1)) & 1u;
+    float kx[EPL], vx[EPL];
+    if (valid) {
+      const uint4* src = my + (size_t)(t % STAGES) * 2 * NV * 32;
+#pragma unroll
+      for (int c = 0; c < NV; ++c) {
+        unpack16<CT>(src[c * 32], kx + VEC * c);
+        unpack16<CT>(src[(NV + c) * 32], vx + VEC * c);
+      }
+    } else {
+#pragma unroll
+      for (int i = 0; i < EPL; ++i) kx[i] = vx[i] = 0.f;
+    }
+#pragma unroll
+    for (int x = 0; x < R; ++x) {
+      float s = 0.f;
+#pragma unroll
+      for (int i = 0; i < EPL; ++i) s = fmaf(q[x][i], kx[i], s);
+#pragma unroll
+      for (int o = G / 2; o > 0; o >>= 1) s += __shfl_xor_sync(0xffffffffu, s, o);
+      if (valid && row <= lim[x]) {
+        if (s > m[x]) {   // the running maximum moves (rare once it has settled): rescale what was accumulated
+          const float f = tc::fast_exp2(m[x] - s);
+          l[x] *= f;
+#pragma unroll
+          for (int i = 0; i < EPL; ++i) acc[x][i] *= f;
+          m[x] = s;
+        }
+        const float w = tc::fast_exp2(s - m[x]);
+        l[x] += w;
+#pragma unroll
+        for (int i = 0; i < EPL; ++i) acc[x][i] = fmaf(w, vx[i], acc[x][i]);
+      }
+    }
+  }
+  mca_cp_async_wait<0>();
+
+  // join the lane groups of a warp, then the warps of the CTA
+#pragma unroll
+  for (int x = 0; x < R; ++x) {
+    float mx = m[x];
+#pragma unroll
+    for (int o = G; o < 32; o <<= 1) mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, o));
+    const float f = m[x] == -INFINITY ? (l[x] == 0.f ? 0.f : 1.f) : tc::fast_exp2(m[x] - mx);
+    float sum = l[x] * f;
+#pragma unroll
+    for (int o = G; o < 32; o <<= 1) sum += __shfl_xor_sync(0xffffffffu, sum, o);
+#pragma unroll
+    for (int i = 0; i < EPL; ++i) {
+      float a = f == 0.f ? 0.f : acc[x][i] * f;
+#pragma unroll
+      for (int o = G; o < 32; o <<= 1) a += __shfl_xor_sync(0xffffffffu, a, o);
+      if (g == 0) s_acc[warp][x][((i / VEC) * G + gl) * VEC + i % VEC] = a;
+    }
+    if (lane == 0) { s_ml[warp][x][0] = mx; s_ml[warp][x][1] = sum; }
+  }
+  __syncthreads();
+  for (int i = threadIdx.x; i < rows * HS; i += SIMT_THREADS) {
+    const int x = i / HS, e = i % HS;
+    float M = -INFINITY;
+#pragma unroll
+    for (int w = 0; w < SIMT_WARPS; ++w) M = fmaxf(M, s_ml[w][x][0]);
+    float sum = 0.f, a = 0.f;
+#pragma unroll
+    for (int w = 0; w < SIMT_WARPS; ++w) {
+      const float mw = s_ml[w][x][0];
+      const float f = mw == -INFINITY ? (s_ml[w][x][1] == 0.f ? 0.f : 1.f) : tc::fast_exp2(mw - M);
+      sum += f == 0.f ? 0.f : s_ml[w][x][1] * f;
+      a += f == 0.f ? 0.f : s_acc[w][x][e] * f;
+    }
+    const int row = row0 + x, t = row / p.group, h = kvh * p.group + row - t * p.group;
+    if (p.nsplit == 1) {
+      reinterpret_cast<float*>(p.out + (int64_t)(sq.start + t) * p.out_st + h * p.out_sh)[e] = sum == 0.f ? 0.f : a / sum;
+    } else {
+      const int64_t slot = ((int64_t)(sq.start + t) * p.n_heads + h) * p.nsplit + split;
+      p.part_acc[slot * HS + e] = a;
+      if (e == 0) { p.part_ml[slot * 2] = M; p.part_ml[slot * 2 + 1] = sum; }
+    }
+  }
+}
+
+// ---------------------------------------------------------------------------------------------------------------------
+// Join of the splits: out = sum_s 2^(m_s - M) acc_s / sum_s 2^(m_s - M) l_s.  A warp per (token, head), a lane four elements.
+// ---------------------------------------------------------------------------------------------------------------------
+template <typename T>
+__global__ void __launch_bounds__(128) paged_join_kernel(const AttnArgs p) {
+  mca_pdl_launch_dependents();
+  mca_pdl_wait();
+  const int lane = threadIdx.x & 31;
+  const int64_t item = (int64_t)blockIdx.x * 4 + (threadIdx.x >> 5);
+  const int t = (int)(item / p.n_heads), h = (int)(item - (int64_t)t * p.n_heads);
+  if (t >= p.batch.n_tokens) return;
+  const int b = paged::sequence_of(p.batch, t);
+  if (b < 0) return;
+  const Sequence s = paged::sequence(p.batch, b);
+  if (!s.good) return;
+  const int pos = s.length - s.count + t - s.start;
+  const int n = pos / p.split_len + 1;   // splits that have keys of this row
+  const int64_t slot = item * p.nsplit;
+  const float2* ml = reinterpret_cast<const float2*>(p.part_ml) + slot;
+  float M = -INFINITY;
+  for (int i = lane; i < n; i += 32) M = fmaxf(M, ml[i].x);
+#pragma unroll
+  for (int o = 16; o > 0; o >>= 1) M = fmaxf(M, __shfl_xor_sync(0xffffffffu, M, o));
+  float sum = 0.f;
+  float4 a = make_float4(0.f, 0.f, 0.f, 0.f);
+  const float4* acc = reinterpret_cast<const float4*>(p.part_acc + slot * p.hs) + lane;
+  const int step = p.hs / 4;
+#pragma unroll 4
+  for (int i = 0; i < n; ++i) {
+    const float2 v = ml[i];
+    const float f = v.y == 0.f ? 0.f : (v.x == -INFINITY ? 1.f : tc::fast_exp2(v.x - M));
+    if (f == 0.f) continue;   // a split with nothing of this row: its sums need not be there
+    sum = fmaf(v.y, f, sum);
+    if (lane < step) {
+      const float4 w = acc[(int64_t)i * step];
+      a.x = fmaf(w.x, f, a.x); a.y = fmaf(w.y, f, a.y); a.z = fmaf(w.z, f, a.z); a.w = fmaf(w.w, f, a.w);
+    }
+  }
+  if (lane < step) {
+    const float inv = sum == 0.f ? 0.f : 1.f / sum;
+    char* dst = p.out + t * p.out_st + h * p.out_sh;
+    if constexpr (sizeof(T) == 4) {
+      reinterpret_cast<float4*>(dst)[lane] = make_float4(a.x * inv, a.y * inv, a.z * inv, a.w * inv);
+    } else {
+      reinterpret_cast<uint2*>(dst)[lane] = make_uint2(tc::pack_bf16(a.x * inv, a.y * inv), tc::pack_bf16(a.z * inv, a.w * inv));
+    }
+  }
+}
+
+// ---------------------------------------------------------------------------------------------------------------------
+// bf16 pages: the tensor-core kernel
+// ---------------------------------------------------------------------------------------------------------------------
+// One CTA owns a tile of query rows of one (sequence, key/value head) and walks the keys of its split 128 at a time; two CTAs
+// share an SM, so that one's softmax runs under the other's products.
+//   warps 0-7   write the query tile, then softmax: a warp reads 16 rows x 128 keys of S in the 16-lane quad layout.  Warps
+//               whose rows lie behind the tile's last take no part in the loop: a single token has one warp at work.
+//   warp 8      TMA producer: lane i fetches the i-th page of a key tile.  Columns behind the head size, and pages that are not
+//               held, lie outside the tensor map and arrive as zeros.
+//   warp 9      MMA issuer (an elected lane), owner of the TMEM allocation.
+// fp32 activations (ACT32) over bf16 pages: a query row q is two bf16 rows of the tile, hi = bf16(q) and lo = bf16(q - hi), 16
+// lanes apart, so that one product S = [hi; lo] K^T forms both and the softmax warp adds them (the pages are bf16 as they are: q
+// to 2^-18 is all that is rounded); the probabilities go back the same way, [p_hi; p_lo], and the two halves of O are added at the
+// end.  64 query rows fill a tile then.
+using namespace tc;
+
+constexpr int KEYS = 128;   // of a key tile
+
+template <int HDP> struct TcPlan {   // HDP: 64 or 128, the head size padded
+  static constexpr int SUB = HDP / 64;
+  static constexpr uint32_t SUB_BYTES = KEYS * 128, TILE_BYTES = SUB * SUB_BYTES;
+  static constexpr int STG = HDP == 64 ? 2 : 1;
+  static constexpr uint32_t OFF_Q = 0, OFF_K = TILE_BYTES, OFF_V = OFF_K + STG * TILE_BYTES, OFF_BAR = OFF_V + STG * TILE_BYTES;
+  static constexpr uint32_t OFF_RED = OFF_BAR + 256;
+  static constexpr uint32_t BYTES = OFF_RED + 2 * 128 * 4 + 1024;   // + alignment slack
+  static_assert(2 * (BYTES + 1024) <= 227 * 1024, "two CTAs share an SM");
+};
+constexpr int TC_THREADS = 320, TC_WARP_TMA = 8, TC_WARP_MMA = 9;
+constexpr uint32_t TC_TMEM = 256;    // S in columns [0, 128), O behind it
+constexpr float TC_RESCALE = 8.0f;   // the softmax's reference point moves when a row's maximum outgrows it by 2^8
+
+enum TcBar : int { TB_Q = 0, TB_KF = 1, TB_KE = 3, TB_VF = 5, TB_VE = 7, TB_S = 9, TB_P1 = 10, TB_P2 = 11, TB_P3 = 12, TB_O = 13, TB_DRAIN = 14, TB_RED = 15, TB_COUNT = 16 };
+
+template <int HDP, bool ACT32>
+__global__ void __launch_bounds__(TC_THREADS, 2) paged_tc_kernel(const __grid_constant__ CUtensorMap map_k, const __grid_constant__ CUtensorMap map_v,
+                                                                 const AttnArgs p) {
+  using PL = TcPlan<HDP>;
+  constexpr int STG = PL::STG;
+  constexpr int R = ACT32 ? 64 : 128;   // query rows of a tile
+  extern __shared__ uint8_t smem_raw[];
+  const uint32_t smem_base = (smem_u32(smem_raw) + 1023u) & ~1023u;
+  uint8_t* smem = smem_raw + (smem_base - smem_u32(smem_raw));
+  volatile uint32_t* tmem_slot = reinterpret_cast<volatile uint32_t*>(smem + PL::OFF_BAR + TB_COUNT * 8);
+  auto bar = [&](int i) { return smem_base + PL::OFF_BAR + 8u * (uint32_t)i; };
+  const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
+  int* const status = g_wait_status;
+
+  mca_pdl_launch_dependents();
+  if (warp == TC_WARP_MMA) {
+    tmem_alloc(smem_u32(const_cast<uint32_t*>(tmem_slot)), TC_TMEM);
+    tmem_relinquish();
+  }
+  if (warp == TC_WARP_TMA && lane == 0) {
+    prefetch_tensormap(&map_k);
+    prefetch_tensormap(&map_v);
+  }
+  mca_pdl_wait();   // from here on the results of the kernels before this one are complete and visible
+  const int kvh = blockIdx.y, split = blockIdx.z;
+  int seq = 0, row0 = 0;
+  Sequence sq{0, 0, 0, false};
+  // tiles are handed out from the last: those of a chunk see the most keys
+  const bool work = (int)blockIdx.x < p.tiles && find_tile(p.batch, p.group, R, p.tiles - 1 - (int)blockIdx.x, &seq, &row0, &sq);
+  if ((int)blockIdx.x == p.tiles && blockIdx.y == 0 && blockIdx.z == 0) {
+    if constexpr (ACT32) look_over<float>(p);
+    else look_over<__nv_bfloat16>(p);
+  }
+  const int rows = min(R, sq.count * p.group - row0);     // of this tile
+  const int pos0 = sq.length - sq.count;
+  const int last = pos0 + (row0 + rows - 1) / p.group;    // the last key that any row of the tile sees
+  const int k_begin = split * p.split_len;
+  const int k_end = min(last + 1, k_begin + p.split_len);
+  const int n = work && k_end > k_begin ? (k_end - k_begin + KEYS - 1) / KEYS : 0;
+  const int n_act = (rows + 15) / 16;                     // softmax warps at work
+  if (tid == 0 && n > 0) {
+    for (int i = 0; i < TB_COUNT; ++i) {
+      const bool by_softmax = (i >= TB_P1 && i <= TB_P3) || i == TB_RED;
+      mbar_init(bar(i), i == TB_Q ? 8u : (by_softmax ? (uint32_t)n_act : 1u));
+    }
+    asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
+  }
+  // does the split meet a page that is not held?
+  bool hole = false;
+  if (n > 0) {
+    const int shift = p.batch.page_shift;
+    for (int i = (k_begin >> shift) + tid; i <= (k_end - 1) >> shift; i += TC_THREADS) {
+      const int id = p.batch.table[(int64_t)seq * p.batch.table_stride + i];
+      if (id < 0 || id >= p.batch.n_pages) {
+        hole = true;
+        if (id != -1 && kvh == 0) paged::refuse(paged::REFUSED_PAGE, seq, id);
+      }
+    }
+  }
+  __shared__ int s_abort;
+  if (tid == 32) s_abort = *reinterpret_cast<volatile int*>(status);
+  tc_fence_before();
+  const bool holes = __syncthreads_or(hole) != 0;
+  tc_fence_after();
+  const uint32_t tmem_base = *tmem_slot;
+  if (n == 0 || s_abort != 0) {   // nothing to do, or an earlier CTA gave up (a uniform decision, before any copy or product)
+    if (warp == TC_WARP_MMA) tmem_dealloc(tmem_base, TC_TMEM);
+    return;
+  }
+  bool ok = true;
+
+  if (warp == TC_WARP_TMA) {
+    // ------------------------------------------------------------------ producer
+    const int shift = p.batch.page_shift;
+    const int box_rows = shift >= 7 ? KEYS : 1 << shift;
+    const int boxes = KEYS / box_rows;
+    auto page_at = [&](int j) {   // this lane's page of key tile j; n_pages: none, zeros arrive
+      const int pos = k_begin + j * KEYS + lane * box_rows;
+      if (lane >= boxes || pos >= k_end || j >= n) return p.batch.n_pages;
+      const int id = p.batch.table[(int64_t)seq * p.batch.table_stride + (pos >> shift)];
+      return id >= 0 && id < p.batch.n_pages ? id : p.batch.n_pages;
+    };
+    int page = page_at(0);
+    int issued_k = 0, issued_v = 0;
+    for (int j = 0; j < n && ok; ++j) {
+      const int st = j % STG;
+      const uint32_t ph = (uint32_t)((j / STG) & 1);
+      const int next = page_at(j + 1);
+      const int slot = (k_begin + j * KEYS + lane * box_rows) & ((1 << shift) - 1);
+      ok = __all_sync(0xffffffffu, mbar_wait(bar(TB_KE + st), ph ^ 1u, status, 10, j));
+      if (!ok) break;
+      if (lane == 0) mbar_expect_tx(bar(TB_KF + st), PL::TILE_BYTES);
+      __syncwarp();
+      if (lane < boxes)
+#pragma unroll
+        for (int s = 0; s < PL::SUB; ++s)
+          tma_load_4d(smem_base + PL::OFF_K + st * PL::TILE_BYTES + s * PL::SUB_BYTES + lane * box_rows * 128, &map_k, bar(TB_KF + st), s * 64, kvh, slot, page);
+      issued_k = j + 1;
+      ok = __all_sync(0xffffffffu, mbar_wait(bar(TB_VE + st), ph ^ 1u, status, 11, j));
+      if (!ok) break;
+      if (lane == 0) mbar_expect_tx(bar(TB_VF + st), PL::TILE_BYTES);
+      __syncwarp();
+      if (lane < boxes)
+#pragma unroll
+        for (int s = 0; s < PL::SUB; ++s)
+          tma_load_4d(smem_base + PL::OFF_V + st * PL::TILE_BYTES + s * PL::SUB_BYTES + lane * box_rows * 128, &map_v, bar(TB_VF + st), s * 64, kvh, slot, page);
+      issued_v = j + 1;
+      page = next;
+    }
+    if (!ok) {   // copies in flight get a bounded time to land before the CTA's memory is released
+      for (int j = max(0, issued_k - STG); j < issued_k; ++j) mbar_wait(bar(TB_KF + (j % STG)), (uint32_t)((j / STG) & 1), status, 13, j);
+      for (int j = max(0, issued_v - STG); j < issued_v; ++j) mbar_wait(bar(TB_VF + (j % STG)), (uint32_t)((j / STG) & 1), status, 14, j);
+    }
+  } else if (warp == TC_WARP_MMA) {
+    // ------------------------------------------------------------------ MMA issuer, in lock step; one elected lane issues
+    const uint32_t leader = elect_one() ? 1u : 0u;
+    const uint32_t tm = __shfl_sync(0xffffffffu, tmem_base, 0);
+    constexpr uint32_t IDESC_QK = make_idesc_fmt(128, KEYS, 0, 0, 1), IDESC_PV = make_idesc_fmt(128, HDP, 0, 1, 1);
+    const uint64_t dq = make_desc(smem_base + PL::OFF_Q, 16, 1024);
+    const uint64_t dk0 = make_desc(smem_base + PL::OFF_K, 16, 1024), dv0 = make_desc(smem_base + PL::OFF_V, PL::SUB_BYTES, 1024);
+    auto issue_qk = [&](int st) {
+      const uint64_t dk = dk0 + (uint64_t)((st * PL::TILE_BYTES) >> 4);
+#pragma unroll
+      for (int kk = 0; kk < HDP / 16; ++kk) {
+        const uint32_t off = ((uint32_t)(kk >> 2) * PL::SUB_BYTES + (uint32_t)(kk & 3) * 32u) >> 4;
+        umma_ss_if<false>(leader, tm, dq + off, dk + off, IDESC_QK, kk > 0 ? 1u : 0u);
+      }
+    };
+    auto issue_pv = [&](int st, bool first, int lo, int hi) {   // 16 keys a step
+      const uint64_t dv = dv0 + (uint64_t)((st * PL::TILE_BYTES) >> 4);
+#pragma unroll
+      for (int kk = lo; kk < hi; ++kk)
+        umma_ts_if<false>(leader, tm + 128, tm + (uint32_t)(kk * 8), dv + (uint64_t)((uint32_t)kk * (2048u >> 4)), IDESC_PV, (first && kk == 0) ? 0u : 1u);
+    };
+    auto wait = [&](int b, uint32_t ph, int stage, int j) { return __all_sync(0xffffffffu, mbar_wait(bar(b), ph, status, stage, j)); };
+    ok = wait(TB_Q, 0, 20, 0) && wait(TB_KF, 0, 21, 0);
+    if (ok) {
+      tc_fence_after();
+      issue_qk(0);
+      umma_commit_if(leader, bar(TB_S));
+      umma_commit_if(leader, bar(TB_KE));
+    }
+    for (int j = 0; j < n && ok; ++j) {
+      const int st = j % STG, stn = (j + 1) % STG;
+      const uint32_t ph = (uint32_t)((j / STG) & 1), phn = (uint32_t)(((j + 1) / STG) & 1), pj = (uint32_t)(j & 1);
+      if (!(ok = wait(TB_VF + st, ph, 22, j))) break;
+      if (!(ok = wait(TB_P1, pj, 28, j))) break;
+      tc_fence_after();
+      issue_pv(st, j == 0, 0, 4);
+      if (j + 1 < n && !(ok = wait(TB_KF + stn, phn, 25, j))) break;
+      if (!(ok = wait(TB_P2, pj, 40, j))) break;
+      tc_fence_after();
+      issue_pv(st, j == 0, 4, 6);
+      if (!(ok = wait(TB_P3, pj, 23, j))) break;
+      tc_fence_after();
+      issue_pv(st, j == 0, 6, 8);
+      umma_commit_if(leader, bar(TB_VE + st));
+      if (j + 1 < n) {
+        issue_qk(stn);
+        umma_commit_if(leader, bar(TB_S));   // covers every product before it, P V(j) among them
+        umma_commit_if(leader, bar(TB_KE + stn));
+      } else {
+        umma_commit_if(leader, bar(TB_O));
+      }
+    }
+    umma_commit_if(leader, bar(TB_DRAIN));   // the tensor pipe is idle (bounded) before TMEM is freed
+    mbar_wait(bar(TB_DRAIN), 0, status, 27, 0);
+    __syncwarp();
+  } else {
+    // ------------------------------------------------------------------ the query tile, 16-byte pieces in the swizzled layout
+    constexpr int CH = HDP / 8;
+    for (int i = tid; i < rows * CH; i += 256) {
+      const int r = i / CH, c = i - r * CH;
+      const int row = row0 + r, t = row / p.group, h = kvh * p.group + row - t * p.group;
+      const char* src = p.q + (int64_t)(sq.start + t) * p.q_st + h * p.q_sh;
+      const bool in = c * 8 < p.hs;
+      const uint32_t sub = PL::OFF_Q + (uint32_t)(c >> 3) * PL::SUB_BYTES;
+      if constexpr (ACT32) {
+        float x[8];
+#pragma unroll
+        for (int k = 0; k < 8; ++k) x[k] = 0.f;
+        if (in) {
+          const float4 a = mca_ld_f4(reinterpret_cast<const float*>(src) + c * 8), b = mca_ld_f4(reinterpret_cast<const float*>(src) + c * 8 + 4);
+          x[0] = a.x; x[1] = a.y; x[2] = a.z; x[3] = a.w; x[4] = b.x; x[5] = b.y; x[6] = b.z; x[7] = b.w;
+        }
+        uint32_t hi[4], lo[4];
+#pragma unroll
+        for (int k = 0; k < 4; ++k) {
+          hi[k] = pack_bf16(x[2 * k], x[2 * k + 1]);
+          lo[k] = pack_bf16(x[2 * k] - __uint_as_float(hi[k] << 16), x[2 * k + 1] - __uint_as_float(hi[k] & 0xffff0000u));
+        }
+        const int r_hi = (r >> 4) * 32 + (r & 15);
+        const uint32_t at = sub + (uint32_t)(r_hi * 128 + (((c & 7) ^ (r_hi & 7)) << 4));
+        *reinterpret_cast<uint4*>(smem + at) = make_uint4(hi[0], hi[1], hi[2], hi[3]);
+        *reinterpret_cast<uint4*>(smem + at + 16 * 128) = make_uint4(lo[0], lo[1], lo[2], lo[3]);   // 16 rows on: the same swizzle
+      } else {
+        uint4 v = make_uint4(0, 0, 0, 0);
+        if (in) v = *(reinterpret_cast<const uint4*>(src) + c);
+        *reinterpret_cast<uint4*>(smem + sub + (uint32_t)(r * 128 + (((c & 7) ^ (r & 7)) << 4))) = v;
+      }
+    }
+    asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
+    __syncwarp();
+    if (lane == 0) mbar_arrive(bar(TB_Q));
+
+    // ------------------------------------------------------------------ softmax
+    const int rank = ACT32 ? warp : (warp & 3) * 2 + (warp >> 2);   // the 16 rows of the tile that are this warp's
+    const int lane_base = ACT32 ? warp * 32 : rank * 16;
+    const int quad = lane & 3;
+    const int r0 = rank * 16 + (lane >> 2);
+    float* red_l = reinterpret_cast<float*>(smem + PL::OFF_RED);
+    float* red_m = red_l + 128;
+    if (rank < n_act) {
+      const uint32_t t_s = tmem_base + ((uint32_t)lane_base << 16), t_o = t_s + 128;
+      constexpr uint32_t LO = 16u << 16;   // ACT32: the low halves' lanes
+      int lim[2];   // the last key that rows r0 and r0 + 8 see
+#pragma unroll
+      for (int h = 0; h < 2; ++h) lim[h] = r0 + 8 * h < rows ? pos0 + (row0 + r0 + 8 * h) / p.group : -1;
+      const int lim_min = pos0 + row0 / p.group;   // of the tile's first row
+      const float scale = p.scale_log2;
+      const float2 scale2 = make_float2(scale, scale);
+      float m_used[2] = {-INFINITY, -INFINITY}, l[2] = {0.f, 0.f};
+      for (int j = 0; j < n && ok; ++j) {
+        ok = __all_sync(0xffffffffu, mbar_wait(bar(TB_S), (uint32_t)(j & 1), status, 30, j));
+        if (!ok) break;
+        tc_fence_after();
+        // s[4g + 2h + e] = logit of row r0 + 8h, key 8g + 2 quad + e
+        uint32_t s[64];
+        if constexpr (ACT32) {
+#pragma unroll
+          for (int c = 0; c < 4; ++c) {
+            uint32_t lo[16];
+            tmem_ldq256_x2(t_s + 32 * c, s + 16 * c);
+            tmem_ldq256_x2(t_s + 32 * c + 16, s + 16 * c + 8);
+            tmem_ldq256_x2(t_s + LO + 32 * c, lo);
+            tmem_ldq256_x2(t_s + LO + 32 * c + 16, lo + 8);
+            tmem_wait_ld();
+#pragma unroll
+            for (int i = 0; i < 16; ++i) s[16 * c + i] = __float_as_uint(__uint_as_float(s[16 * c + i]) + __uint_as_float(lo[i]));
+          }
+        } else {
+          tmem_ldq256_x8(t_s, s);
+          tmem_ldq256_x8(t_s + 64, s + 32);
+          tmem_wait_ld();
+        }
+        const int key0 = k_begin + j * KEYS;
+        if (key0 + KEYS - 1 > lim_min) {
+#pragma unroll
+          for (int i = 0; i < 64; ++i)
+            if (key0 + 8 * (i >> 2) + 2 * quad + (i & 1) > lim[(i >> 1) & 1]) s[i] = 0xff800000u;
+          if (key0 + KEYS > last + 1 && j == n - 1) {
+            // what lies behind the last key is nobody's: its values become zeros, since 0 x infinity is not
+            ok = __all_sync(0xffffffffu, mbar_wait(bar(TB_VF + (j % STG)), (uint32_t)((j / STG) & 1), status, 31, j));
+            if (!ok) break;
+            uint8_t* v = smem + PL::OFF_V + (j % STG) * PL::TILE_BYTES;
+            const int z0 = last + 1 - key0;
+            for (int i = rank * 32 + lane; i < (KEYS - z0) * CH; i += n_act * 32) {
+              const int r = z0 + i / CH, c = i % CH;
+              *reinterpret_cast<uint4*>(v + (c >> 3) * PL::SUB_BYTES + r * 128 + (c & 7) * 16) = make_uint4(0, 0, 0, 0);
+            }
+            asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
+          }
+        }
+        if (holes) {
+#pragma unroll 1
+          for (int c = 0; c < 8; ++c) {   // 16 keys: within one page
+            const int pos = key0 + 16 * c;
+            if (pos >= k_end || page_of(p.batch, seq, pos, false) >= 0) continue;
+#pragma unroll
+            for (int i = 0; i < 64; ++i)
+              if ((i >> 3) == c) s[i] = 0xff800000u;
+          }
+        }
+        float mx[2];
+#pragma unroll
+        for (int h = 0; h < 2; ++h) {
+          float ma = -INFINITY, mb = -INFINITY;
+#pragma unroll
+          for (int g = 0; g < 16; g += 2) {
+            ma = max3(ma, __uint_as_float(s[4 * g + 2 * h]), __uint_as_float(s[4 * g + 2 * h + 1]));
+            mb = max3(mb, __uint_as_float(s[4 * g + 4 + 2 * h]), __uint_as_float(s[4 * g + 4 + 2 * h + 1]));
+          }
+          mx[h] = fmaxf(ma, mb) * scale;
+        }
+        const bool grown = mx[0] > m_used[0] + TC_RESCALE || mx[1] > m_used[1] + TC_RESCALE;
+        if (j == 0 || __any_sync(0xffffffffu, grown)) {
+          float f[2];
+#pragma unroll
+          for (int h = 0; h < 2; ++h) {
+            mx[h] = fmaxf(mx[h], __shfl_xor_sync(0xffffffffu, mx[h], 1));
+            mx[h] = fmaxf(mx[h], __shfl_xor_sync(0xffffffffu, mx[h], 2));
+            float m_new = mx[h] > m_used[h] + TC_RESCALE ? mx[h] : m_used[h];
+            if (m_new == -INFINITY) m_new = 0.f;   // no key seen yet
+            f[h] = m_new != m_used[h] ? fast_exp2(m_used[h] - m_new) : 1.0f;
+            l[h] *= f[h];
+            m_used[h] = m_new;
+          }
+          if (j > 0) {   // P V(j - 1) finished before S(j) did
+#pragma unroll
+            for (int c = 0; c < (ACT32 ? 2 : 1) * (HDP / 16); ++c) {
+              const uint32_t at = t_o + (c % (HDP / 16)) * 16 + (c >= HDP / 16 ? LO : 0u);
+              uint32_t o[8];
+              tmem_ldq256_x2(at, o);
+              tmem_wait_ld();
+#pragma unroll
+              for (int i = 0; i < 8; ++i) o[i] = __float_as_uint(__uint_as_float(o[i]) * f[(i >> 1) & 1]);
+              tmem_stq256_x2(at, o);
+            }
+          }
+        }
+        // p = 2^(s scale - m), handed over in three pieces (64, 32, 32 keys); the sum is of the unrounded ones
+        const float2 nm2[2] = {make_float2(-m_used[0], -m_used[0]), make_float2(-m_used[1], -m_used[1])};
+        float2 rs[2] = {make_float2(0.f, 0.f), make_float2(0.f, 0.f)};
+        auto quarter = [&](const int i) {
+          uint32_t pk[8], pl[ACT32 ? 8 : 1];
+#pragma unroll
+          for (int g = 4 * i; g < 4 * i + 4; ++g)
+#pragma unroll
+            for (int h = 0; h < 2; ++h) {
+              const float2 xx = ffma2(make_float2(__uint_as_float(s[4 * g + 2 * h]), __uint_as_float(s[4 * g + 2 * h + 1])), scale2, nm2[h]);
+              const float p0 = fast_exp2(xx.x), p1 = fast_exp2(xx.y);
+              const uint32_t w = pack_bf16(p0, p1);
+              pk[2 * (g & 3) + h] = w;
+              if constexpr (ACT32) pl[2 * (g & 3) + h] = pack_bf16(p0 - __uint_as_float(w << 16), p1 - __uint_as_float(w & 0xffff0000u));
+              rs[h] = fadd2(rs[h], make_float2(p0, p1));
+            }
+          tmem_stq128_x4(t_s + 16 * i, pk);
+          if constexpr (ACT32) tmem_stq128_x4(t_s + LO + 16 * i, pl);
+        };
+        auto hand_over = [&](int b) {
+          tmem_wait_st();
+          tc_fence_before();
+          __syncwarp();
+          if (lane == 0) mbar_arrive(bar(b));
+        };
+        quarter(0);
+        quarter(1);
+        hand_over(TB_P1);
+        quarter(2);
+        hand_over(TB_P2);
+        quarter(3);
+        hand_over(TB_P3);
+        l[0] += rs[0].x + rs[0].y;
+        l[1] += rs[1].x + rs[1].y;
+      }
+      if (ok) {
+#pragma unroll
+        for (int h = 0; h < 2; ++h) {
+          l[h] += __shfl_xor_sync(0xffffffffu, l[h], 1);
+          l[h] += __shfl_xor_sync(0xffffffffu, l[h], 2);
+        }
+        if (quad == 0) {
+          red_l[r0] = l[0]; red_l[r0 + 8] = l[1];
+          red_m[r0] = m_used[0]; red_m[r0 + 8] = m_used[1];
+        }
+        __syncwarp();
+        if (lane == 0) mbar_arrive(bar(TB_RED));
+      }
+    }
+    // ------------------------------------------------------------------ epilogue: a lane a row, warps w and w + 4 half the columns each
+    const int first_row = ACT32 ? (warp & 3) * 16 : (warp & 3) * 32;
+    if (ok && first_row < rows) {
+      ok = __all_sync(0xffffffffu, mbar_wait(bar(TB_RED), 0, status, 36, n));
+      if (ok) ok = __all_sync(0xffffffffu, mbar_wait(bar(TB_O), 0, status, 34, n));
+      if (ok) {
+        tc_fence_after();
+        constexpr int OC = HDP / 2;
+        const int col0 = (warp >> 2) * OC;
+        const int r = ACT32 ? first_row + (lane & 15) : first_row + lane;
+        const uint32_t t_o = tmem_base + ((uint32_t)((warp & 3) * 32) << 16) + 128 + col0;
+        const bool mine = r < rows && (!ACT32 || lane < 16);
+        const int rr = min(r, rows - 1);
+        const int row = row0 + rr, t = row / p.group, h = kvh * p.group + row - t * p.group;
+        const float sum = red_l[rr];
+        const int64_t slot = ((int64_t)(sq.start + t) * p.n_heads + h) * p.nsplit + split;
+        const float inv = p.nsplit > 1 ? 1.f : (sum == 0.f ? 0.f : 1.f / sum);
+        char* dst = p.out + (int64_t)(sq.start + t) * p.out_st + h * p.out_sh;
+        float* part = p.part_acc + slot * p.hs;
+        if (p.nsplit > 1 && mine && col0 == 0) {
+          p.part_ml[slot * 2] = red_m[rr];
+          p.part_ml[slot * 2 + 1] = sum;
+        }
+#pragma unroll
+        for (int c = 0; c < OC / 16; ++c) {
+          uint32_t o[16];
+          tmem_ld16(t_o + c * 16, o);
+          tmem_wait_ld();
+          if constexpr (ACT32)
+#pragma unroll
+            for (int i = 0; i < 16; ++i)
+              o[i] = __float_as_uint(__uint_as_float(o[i]) + __uint_as_float(__shfl_xor_sync(0xffffffffu, o[i], 16)));
+          const int col = col0 + c * 16;
+          if (!mine || col >= p.hs) continue;
+          if (ACT32 || p.nsplit > 1) {
+            float* f = p.nsplit > 1 ? part : reinterpret_cast<float*>(dst);
+#pragma unroll
+            for (int i = 0; i < 16; i += 4)
+              *reinterpret_cast<float4*>(f + col + i) = make_float4(__uint_as_float(o[i]) * inv, __uint_as_float(o[i + 1]) * inv,
+                                                                    __uint_as_float(o[i + 2]) * inv, __uint_as_float(o[i + 3]) * inv);
+          } else {
+#pragma unroll
+            for (int i = 0; i < 16; i += 8)
+              *reinterpret_cast<uint4*>(reinterpret_cast<__nv_bfloat16*>(dst) + col + i) =
+                  make_uint4(pack_bf16(__uint_as_float(o[i]) * inv, __uint_as_float(o[i + 1]) * inv), pack_bf16(__uint_as_float(o[i + 2]) * inv, __uint_as_float(o[i + 3]) * inv),
+                             pack_bf16(__uint_as_float(o[i + 4]) * inv, __uint_as_float(o[i + 5]) * inv), pack_bf16(__uint_as_float(o[i + 6]) * inv, __uint_as_float(o[i + 7]) * inv));
+          }
+        }
+      }
+    }
+  }
+  tc_fence_before();
+  __syncthreads();
+  if (warp == TC_WARP_MMA) {
+    tc_fence_after();
+    tmem_dealloc(tmem_base, TC_TMEM);
+  }
+}
+
+// ---------------------------------------------------------------------------------------------------------------------
+// Host
+// ---------------------------------------------------------------------------------------------------------------------
+struct Plan {
+  bool tc;
+  int rows;       // query rows of a tile
+  int tiles, split_len, nsplit;
+  int64_t bytes;  // of workspace
+};
+
+// Which kernel, and how the keys are split.
+int make_plan(const McaPagedCache* c, const McaPagedBatch* b, int dtype, Plan* out) {
+  const int group = c->n_heads / c->n_kv_heads;
+  const int64_t most_rows = (int64_t)b->max_new * group;   // of one sequence and key/value head
+  const bool act32 = dtype == MCA_DTYPE_F32;
+  out->tc = !act32 || (c->dtype == MCA_DTYPE_BF16 && most_rows > 4);
+  out->rows = out->tc ? (act32 ? 64 : 128) : (most_rows >= 4 ? 4 : (most_rows >= 2 ? 2 : 1));
+  const int64_t tiles = most_rows <= out->rows ? b->n_seqs : (int64_t)b->n_tokens * group / out->rows + b->n_seqs;
+  if (tiles >= (1ll << 30)) return ERROR_PARAM_OUT_OF_RANGE;
+  out->tiles = (int)tiles;
+  const int64_t ctas = tiles * c->n_kv_heads;
+  const int slots = !out->tc && out->rows == 4 ? 148 : 296;
+  const int step = out->tc ? KEYS : 16, least = out->tc ? 2 * KEYS : 128;
+  // time in keys of one CTA: whole waves of (set-up + the keys of a split); more than one split also writes and joins partial results
+  const double setup = out->tc ? 512 : 64;
+  const double part_keys = (double)b->n_tokens * c->n_heads * c->head_size * 8.0 / 5e6 * 128.0;   // 5 TB/s; 128 keys are about a microsecond
+  double best = 1e300;
+  int64_t len = 0;
+  for (int n = 1; n <= std::max(1, std::min(64, b->max_len / least)); ++n) {
+    const int64_t l = ((b->max_len + n - 1) / n + step - 1) / step * step;
+    const double cost = (double)((ctas * n + slots - 1) / slots) * (setup + (double)l) + (n > 1 ? 512 + n * part_keys : 0);
+    if (cost < best) { best = cost; len = l; }
+  }
+  out->split_len = (int)len;
+  out->nsplit = (int)((b->max_len + len - 1) / len);
+  out->bytes = out->nsplit > 1 ? (int64_t)b->n_tokens * c->n_heads * out->nsplit * (c->head_size + 2) * 4 : 0;
+  return 0;
+}
+
+int page_map(CUtensorMap* map, const void* base, const McaPagedCache* c) {
+  EncodeTiledFn fn = get_encode_fn();
+  if (!fn) return ERROR_NOT_IMPLEMENTED;
+  const cuuint64_t dims[4] = {(cuuint64_t)c->head_size, (cuuint64_t)c->n_kv_heads, (cuuint64_t)c->page_size, (cuuint64_t)c->n_pages};
+  const cuuint64_t strides[3] = {(cuuint64_t)c->head_size * 2, (cuuint64_t)c->n_kv_heads * c->head_size * 2, (cuuint64_t)c->page_stride * 2};
+  const cuuint32_t box[4] = {64, 1, (cuuint32_t)std::min(c->page_size, KEYS), 1}, ones[4] = {1, 1, 1, 1};
+  const CUresult r = fn(map, CU_TENSOR_MAP_DATA_TYPE_BFLOAT16, 4, const_cast<void*>(base), dims, strides, box, ones, CU_TENSOR_MAP_INTERLEAVE_NONE,
+                        CU_TENSOR_MAP_SWIZZLE_128B, CU_TENSOR_MAP_L2_PROMOTION_L2_256B, CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE);
+  return r == CUDA_SUCCESS ? 0 : ERROR_PARAM_OUT_OF_RANGE;
+}
+
+template <int HDP, bool ACT32>
+int launch_tc(const McaPagedCache* c, const AttnArgs& a, cudaStream_t st) {
+  CUtensorMap mk, mv;
+  int e;
+  if ((e = page_map(&mk, c->k_pages, c)) || (e = page_map(&mv, c->v_pages, c))) return e;
+  static std::atomic<uint64_t> done{0};
+  if ((e = mca_smem_once(done, paged_tc_kernel<HDP, ACT32>, TcPlan<HDP>::BYTES))) return e;
+  return mca_launch_pdl(paged_tc_kernel<HDP, ACT32>, dim3(a.tiles + 1, a.n_kv, a.nsplit), dim3(TC_THREADS), TcPlan<HDP>::BYTES, st, mk, mv, a);
+}
+template <typename CT, int HS>
+int launch_simt(int rows, const AttnArgs& a, cudaStream_t st) {
+  constexpr size_t smem = Lanes<CT, HS>::RING;
+  static std::atomic<uint64_t> done1{0}, done2{0}, done4{0};
+  const dim3 grid(a.tiles + 1, a.n_kv, a.nsplit);
+  int e;
+  switch (rows) {
+    case 1:
+      if ((e = mca_smem_once(done1, paged_simt_kernel<CT, HS, 1>, smem))) return e;
+      return mca_launch_pdl(paged_simt_kernel<CT, HS, 1>, grid, dim3(SIMT_THREADS), smem, st, a);
+    case 2:
+      if ((e = mca_smem_once(done2, paged_simt_kernel<CT, HS, 2>, smem))) return e;
+      return mca_launch_pdl(paged_simt_kernel<CT, HS, 2>, grid, dim3(SIMT_THREADS), smem, st, a);
+    default:
+      if ((e = mca_smem_once(done4, paged_simt_kernel<CT, HS, 4>, smem))) return e;
+      return mca_launch_pdl(paged_simt_kernel<CT, HS, 4>, grid, dim3(SIMT_THREADS), smem, st, a);
+  }
+}
+
+int check_types(const McaPagedCache* c, int dtype) {
+  if (dtype != MCA_DTYPE_F32 && dtype != MCA_DTYPE_BF16) return ERROR_ATTN_UNSUPPORTED_SHAPE;
+  if (dtype == MCA_DTYPE_BF16 && c->dtype != MCA_DTYPE_BF16) return ERROR_ATTN_UNSUPPORTED_SHAPE;
+  return c->n_kv_heads > 65535 ? ERROR_PARAM_OUT_OF_RANGE : 0;
+}
+
+}  // namespace
+
+int64_t mca_paged_attention_workspace_bytes(const McaPagedCache* cache, const McaPagedBatch* batch, int dtype) {
+  Batch view;
+  Plan plan;
+  if (paged::check(cache, batch, &view) || check_types(cache, dtype) || make_plan(cache, batch, dtype, &plan)) return -1;
+  return plan.bytes;
+}
+
+int mca_paged_attention(const McaPagedCache* cache, const McaPagedBatch* batch, int dtype, const McaHeads* q, float scale, const McaHeads* out,
+                        void* workspace, int64_t workspace_bytes, void* stream) {
+  AttnArgs a;
+  int e = paged::check(cache, batch, &a.batch);
+  if (e || (e = check_types(cache, dtype))) return e;
+  if (!(scale >= 0.f) || scale > 3.0e38f) return ERROR_PARAM_OUT_OF_RANGE;
+  if (batch->n_tokens == 0) return 0;
+  if ((e = paged::check_heads(q, dtype, false)) || (e = paged::check_heads(out, dtype, false))) return e;
+  Plan plan;
+  if ((e = make_plan(cache, batch, dtype, &plan))) return e;
+  if (plan.bytes > 0) {
+    if (!workspace || workspace_bytes < plan.bytes) return ERROR_ATTN_SCRATCH_TOO_SMALL;
+    if ((uintptr_t)workspace & 15) return ERROR_PARAM_OUT_OF_RANGE;
+  }
+  const int D = cache->head_size, size = dtype == MCA_DTYPE_BF16 ? 2 : 4, csize = cache->dtype == MCA_DTYPE_BF16 ? 2 : 4;
+  a.q = static_cast<const char*>(q->data); a.out = static_cast<char*>(out->data);
+  a.q_st = q->stride_t * size; a.q_sh = q->stride_h * size; a.out_st = out->stride_t * size; a.out_sh = out->stride_h * size;
+  a.k_pages = static_cast<const char*>(cache->k_pages); a.v_pages = static_cast<const char*>(cache->v_pages);
+  a.page_bytes = cache->page_stride * csize; a.row_bytes = (int64_t)cache->n_kv_heads * D * csize;
+  a.n_heads = cache->n_heads; a.n_kv = cache->n_kv_heads; a.group = cache->n_heads / cache->n_kv_heads; a.hs = D;
+  a.split_len = plan.split_len; a.nsplit = plan.nsplit; a.tiles = plan.tiles;
+  a.scale_log2 = (scale == 0.f ? 1.0f / sqrtf((float)D) : scale) * LOG2E;
+  a.part_acc = static_cast<float*>(workspace);
+  a.part_ml = plan.nsplit > 1 ? a.part_acc + (int64_t)batch->n_tokens * cache->n_heads * plan.nsplit * D : nullptr;
+  cudaStream_t st = (cudaStream_t)stream;
+  if (plan.tc) {
+    if (dtype == MCA_DTYPE_F32) e = D <= 64 ? launch_tc<64, true>(cache, a, st) : launch_tc<128, true>(cache, a, st);
+    else e = D <= 64 ? launch_tc<64, false>(cache, a, st) : launch_tc<128, false>(cache, a, st);
+  } else {
+    switch (D) {
+#define MCA_PAGED_CASE(HS_) \
+      case HS_: e = csize == 2 ? launch_simt<__nv_bfloat16, HS_>(plan.rows, a, st) : launch_simt<float, HS_>(plan.rows, a, st); break;
+      MCA_PAGED_CASE(32) MCA_PAGED_CASE(48) MCA_PAGED_CASE(64) MCA_PAGED_CASE(96) MCA_PAGED_CASE(128)
+#undef MCA_PAGED_CASE
+      default: return ERROR_ATTN_UNSUPPORTED_SHAPE;
+    }
+  }
+  if (e || plan.nsplit == 1) return e;
+  const int64_t items = (int64_t)batch->n_tokens * cache->n_heads;
+  const dim3 grid((unsigned)((items + 3) / 4));
+  return dtype == MCA_DTYPE_F32 ? mca_launch_pdl(paged_join_kernel<float>, grid, dim3(128), 0, st, a)
+                                : mca_launch_pdl(paged_join_kernel<__nv_bfloat16>, grid, dim3(128), 0, st, a);
+}
+
+int mca_paged_status(int* status4) {
+  if (!status4) return ERROR_PARAM_NULL;
+  int own[4] = {0, 0, 0, 0}, norm[4] = {0, 0, 0, 0}, wait[4] = {0, 0, 0, 0};
+  int e = paged::read_status(own);
+  if (e || (e = mca_qk_norm_read_status(norm))) return e;
+  MCA_CUDA_TRY(cudaMemcpyFromSymbol(wait, g_wait_status, sizeof(wait)));
+  if (wait[0] != 0) {
+    const int zero[4] = {0, 0, 0, 0};
+    MCA_CUDA_TRY(cudaMemcpyToSymbol(g_wait_status, zero, sizeof(zero)));
+    status4[0] = paged::REFUSED_WAIT; status4[1] = wait[1]; status4[2] = wait[2]; status4[3] = 1;
+    return 0;
+  }
+  const int* s = norm[3] != 0 ? norm : own;
+  status4[0] = s[0]; status4[1] = s[1]; status4[2] = s[2]; status4[3] = own[3] + norm[3];
+  return 0;
+}
+
+int mca_set_fail_words_paged(int* words) {
+  MCA_CUDA_TRY(cudaMemcpyToSymbol(paged::g_fail_words, &words, sizeof(words)));
+  return (int)cudaMemcpyToSymbol(tc::g_fail_words, &words, sizeof(words));
+}

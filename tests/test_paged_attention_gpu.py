@@ -1,0 +1,178 @@
+"""Attention of new tokens over a paged cache against its formula in 64 bits.  What no sequence owns of the pool is NaN, so that a
+read behind a length, or of a page that is not held, shows."""
+import math
+
+import pytest
+
+pytestmark = pytest.mark.gpu
+torch = pytest.importorskip("torch")
+
+TYPES = [("f32", "f32"), ("f32", "bf16"), ("bf16", "bf16")]
+
+
+def setup(*a, **k):
+    from paged_util import Setup
+    return Setup(*a, **k)
+
+
+@pytest.mark.parametrize("act,cache", TYPES)
+@pytest.mark.parametrize("hs", [32, 48, 64, 96, 128])
+def test_single_tokens(act, cache, hs):
+    s = setup([(1, n) for n in (1, 2, 15, 16, 17, 127, 128, 129, 300)], 4, 2, hs, 16, act, cache)
+    s.cache.attend(s.batch, s.q, s.out)
+    s.check()
+    assert s.cache.status() == (0, 0, 0, 0)
+
+
+@pytest.mark.parametrize("act,cache", TYPES)
+@pytest.mark.parametrize("heads,kv", [(1, 1), (3, 1), (4, 1), (6, 2), (8, 8), (16, 1)])
+def test_chunks(act, cache, heads, kv):
+    s = setup([(1, 1), (2, 2), (33, 33), (130, 131), (5, 200), (64, 128), (1, 77)], heads, kv, 64, 32, act, cache, seed=1)
+    s.cache.attend(s.batch, s.q, s.out)
+    s.check()
+
+
+@pytest.mark.parametrize("act,cache", TYPES)
+@pytest.mark.parametrize("page", [16, 64, 128, 256, 1024])
+def test_pages(act, cache, page):
+    s = setup([(40, 300), (1, 1030), (7, 7)], 8, 2, 128, page, act, cache, seed=2)
+    s.cache.attend(s.batch, s.q, s.out)
+    s.check()
+
+
+@pytest.mark.parametrize("act,cache", TYPES)
+def test_long_single_tokens_are_split(act, cache):
+    s = setup([(1, 5003), (1, 129), (1, 2500)], 4, 1, 128, 64, act, cache, seed=3)
+    s.cache.attend(s.batch, s.q, s.out)
+    s.check()
+
+
+@pytest.mark.parametrize("act,cache", TYPES)
+def test_chunk_over_a_long_cache_is_split(act, cache):
+    s = setup([(37, 4001), (1, 9)], 4, 4, 64, 32, act, cache, seed=4)
+    s.cache.attend(s.batch, s.q, s.out)
+    s.check()
+
+
+@pytest.mark.parametrize("act,cache", TYPES)
+def test_pages_not_held(act, cache):
+    """The middle, the first, the last and all pages of a sequence are gone; a token with no key left gives zeros."""
+    s = setup([(3, 100), (40, 90), (1, 64), (20, 20), (1, 1500)], 4, 2, 64, 16, act, cache, seed=5,
+              drop=[(0, 0), (0, 3), (1, 0), (1, 1), (1, 2), (1, 3), (2, 3), (3, 0), (3, 1)] + [(4, i) for i in range(3, 60)])
+    s.cache.attend(s.batch, s.q, s.out)
+    s.check()
+    assert not s.out[s.starts[3]:s.starts[4]].any()
+    assert s.cache.status() == (0, 0, 0, 0)
+
+
+@pytest.mark.parametrize("act,cache", TYPES)
+def test_padding_and_sequences_without_tokens(act, cache):
+    s = setup([(0, 50), (3, 10), (0, 0), (1, 40), (0, 17)], 4, 4, 64, 16, act, cache, seed=6, pad=9, max_new=50, max_len=64)
+    s.cache.attend(s.batch, s.q, s.out)
+    s.check()                                   # rows behind the last sequence: still 7
+    assert s.cache.status() == (0, 0, 0, 0)
+
+
+@pytest.mark.parametrize("act,cache", TYPES)
+def test_strides_and_scale(act, cache):
+    """q and out as parts of wider rows, pages apart from one another, a scale of the caller's."""
+    s = setup([(20, 150), (1, 33)], 4, 2, 64, 16, act, cache, seed=7, stride_pages=64)
+    wide = torch.zeros(s.n_tokens, 10, 80, device="cuda", dtype=s.act)
+    wide[:, 2:6, :64] = s.q
+    out = torch.full_like(wide, 7.0)
+    s.cache.attend(s.batch, wide[:, 2:6, :64], out[:, 5:9, :64], scale=0.21)
+    s.out = out[:, 5:9, :64].contiguous()
+    s.check(scale=0.21)
+    out[:, 5:9, :64] = 7.0
+    assert (out == 7.0).all()
+
+
+@pytest.mark.parametrize("act,cache", TYPES)
+def test_more_sequences_than_a_warp_looks_at_once(act, cache):
+    s = setup([(1 + b % 3, 3 + b) for b in range(70)], 2, 1, 32, 16, act, cache, seed=8)
+    s.cache.attend(s.batch, s.q, s.out)
+    s.check()
+
+
+@pytest.mark.parametrize("act,cache", TYPES)
+def test_large_logits(act, cache):
+    """One key far above the others, and the maximum moving late: the sums are rescaled."""
+    s = setup([(5, 400), (1, 700)], 2, 2, 64, 32, act, cache, seed=9)
+    s.q *= 6.0
+    s.cache.attend(s.batch, s.q, s.out)
+    s.check()
+
+
+@pytest.mark.parametrize("act,cache", TYPES)
+def test_captured_and_on_another_stream(act, cache):
+    """A captured call follows new lengths and queries; two graphs in flight at once do not share a workspace."""
+    a, b = (setup([(1, 2000), (3, 300)], 4, 1, 64, 16, act, cache, seed=10 + i) for i in range(2))
+    side = [torch.cuda.Stream() for _ in range(2)]
+    graphs = []
+    torch.cuda.synchronize()
+    for s, st in zip((a, b), side):
+        with torch.cuda.stream(st):
+            s.cache.attend(s.batch, s.q, s.out)
+            st.synchronize()
+            g = torch.cuda.CUDAGraph()
+            g.capture_begin()
+            s.cache.attend(s.batch, s.q, s.out)
+            g.capture_end()
+            graphs.append(g)
+    for s in (a, b):
+        s.q.copy_(torch.randn_like(s.q.float()).to(s.q.dtype))
+        s.lengths.copy_(torch.tensor([1990, 299], device="cuda", dtype=torch.int32))
+        s.seqs = [(1, 1990), (3, 299)]
+        s.k, s.v = [k[:n] for k, (_, n) in zip(s.k, s.seqs)], [v[:n] for v, (_, n) in zip(s.v, s.seqs)]
+        s.held = [h[:n] for h, (_, n) in zip(s.held, s.seqs)]
+    torch.cuda.synchronize()
+    for _ in range(20):
+        for g, st in zip(graphs, side):
+            with torch.cuda.stream(st):
+                g.replay()
+    torch.cuda.synchronize()
+    for s in (a, b):
+        s.check()
+    del graphs
+
+
+@pytest.mark.parametrize("act,cache", TYPES)
+def test_refused_sequences_give_zeros_and_a_status(act, cache):
+    s = setup([(2, 40), (3, 50), (4, 60)], 4, 2, 64, 16, act, cache, seed=12)
+    ref, tol = s.exact()
+    bad = torch.tensor([40, 2, 60], device="cuda", dtype=torch.int32)       # fewer positions than new tokens
+    batch = s.cache.batch(s.starts, bad, s.table, s.n_tokens, s.max_new, s.max_len)
+    s.cache.attend(batch, s.q, s.out)
+    assert s.cache.status() == (1, 1, 2, 1)
+    assert not s.out[2:5].any()
+    keep = [0, 1, 5, 6, 7, 8]
+    assert ((s.out.double() - ref).abs()[keep] <= tol[keep]).all()
+    assert s.cache.status() == (0, 0, 0, 0)
+    long = torch.tensor([40, 50, 61], device="cuda", dtype=torch.int32)      # longer than the bound
+    s.cache.attend(s.cache.batch(s.starts, long, s.table, s.n_tokens, s.max_new, 60), s.q, s.out)
+    assert s.cache.status() == (1, 2, 61, 1) and not s.out[5:].any()
+
+
+@pytest.mark.parametrize("act,cache", TYPES)
+def test_page_ids_outside_the_pool_are_left_out(act, cache):
+    s = setup([(2, 40), (1, 50)], 4, 2, 64, 16, act, cache, seed=13, drop=[(1, 1)])
+    s.table[1, 1] = s.k_pages.shape[0]
+    s.cache.attend(s.batch, s.q, s.out)
+    s.check()
+    st = s.cache.status()
+    assert st[:3] == (2, 1, s.k_pages.shape[0]) and st[3] >= 1
+    s.table[1, 1] = -2
+    s.cache.attend(s.batch, s.q, s.out)
+    s.check()
+    assert s.cache.status()[:3] == (2, 1, -2)
+
+
+def test_runs_alike():
+    """The same call gives the same bits."""
+    s = setup([(1, 3000), (50, 700)], 8, 2, 128, 64, "bf16", "bf16", seed=14)
+    s.cache.attend(s.batch, s.q, s.out)
+    first = s.out.clone()
+    for _ in range(3):
+        s.out.zero_()
+        s.cache.attend(s.batch, s.q, s.out)
+        assert torch.equal(first, s.out)
