@@ -9,7 +9,7 @@
 //   paged_simt_kernel    fp32 activations: exact fp32 products, a lane group per cache row.
 //   paged_join_kernel    where few rows meet a long cache the keys are cut into splits, joined here by their maxima and sums.
 #include <algorithm>
-#include <mutex>
+#include <cmath>
 
 #define MCA_TU_FAIL_FAMILY MCA_FAIL_PAGED
 #include "paged_common.cuh"
@@ -34,8 +34,12 @@ struct AttnArgs {
   int n_heads, n_kv, group, hs;
   int split_len, nsplit, tiles;
   float scale_log2;         // scale x log2(e): the softmax runs on powers of two
-  float* part_acc;          // (n_tokens, n_heads, nsplit, hs)
-  float* part_ml;           // (n_tokens, n_heads, nsplit, 2): reference point (log2), sum
+  float* part_acc;          // partial results: fp32 kernel (n_tokens, n_heads, nsplit, hs), tensor-core kernel (ctas, 2, rows_max, hs)
+  float* part_ml;           // the same with 2 in place of hs: reference point (log2), sum
+  // tensor-core kernel
+  int tile_shift, parts, items;    // log2 of the tokens of a tile; tiles that share a token's group of heads; parts x key/value heads
+  int ctas, least_units, warps, rows_max;
+  int4* meta;               // (ctas, 2): the item that ends in a CTA and began in another: {that CTA or -1, token row, head, rows}, {heads}
 };
 
 // Tile -> sequence and its first row; every lane of the warp takes part.  Tiles of a sequence: its rows (new tokens x group) in
@@ -281,8 +285,7 @@ __global__ void __launch_bounds__(SIMT_THREADS, R <= 2 ? 2 : 1) paged_simt_kerne
 // ---------------------------------------------------------------------------------------------------------------------
 // Join of the splits: out = sum_s 2^(m_s - M) acc_s / sum_s 2^(m_s - M) l_s.  A warp per (token, head), a lane four elements.
 // ---------------------------------------------------------------------------------------------------------------------
-template <typename T>
-__global__ void __launch_bounds__(128) paged_join_kernel(const AttnArgs p) {
+__global__ void __launch_bounds__(128) paged_simt_join_kernel(const AttnArgs p) {
   mca_pdl_launch_dependents();
   mca_pdl_wait();
   const int lane = threadIdx.x & 31;
@@ -318,52 +321,208 @@ __global__ void __launch_bounds__(128) paged_join_kernel(const AttnArgs p) {
   }
   if (lane < step) {
     const float inv = sum == 0.f ? 0.f : 1.f / sum;
-    char* dst = p.out + t * p.out_st + h * p.out_sh;
-    if constexpr (sizeof(T) == 4) {
-      reinterpret_cast<float4*>(dst)[lane] = make_float4(a.x * inv, a.y * inv, a.z * inv, a.w * inv);
-    } else {
-      reinterpret_cast<uint2*>(dst)[lane] = make_uint2(tc::pack_bf16(a.x * inv, a.y * inv), tc::pack_bf16(a.z * inv, a.w * inv));
-    }
+    reinterpret_cast<float4*>(p.out + t * p.out_st + h * p.out_sh)[lane] = make_float4(a.x * inv, a.y * inv, a.z * inv, a.w * inv);
   }
 }
 
 // ---------------------------------------------------------------------------------------------------------------------
 // bf16 pages: the tensor-core kernel
 // ---------------------------------------------------------------------------------------------------------------------
-// One CTA owns a tile of query rows of one (sequence, key/value head) and walks the keys of its split 128 at a time; two CTAs
-// share an SM, so that one's softmax runs under the other's products.
-//   warps 0-7   write the query tile, then softmax: a warp reads 16 rows x 128 keys of S in the 16-lane quad layout.  Warps
-//               whose rows lie behind the tile's last take no part in the loop: a single token has one warp at work.
+// Work is counted in units: an item is a tile of query rows of one (sequence, key/value head), its units are the tiles of 128 keys
+// that the rows see (and ITEM_UNITS more, for its set-up and end).  The launch's CTAs, as many as the machine holds at once, take
+// equal contiguous shares of all units, whatever the lengths are: a CTA ends the item its neighbour began, works whole ones, and
+// begins one more.  An item within one CTA is written out; the parts of the others go to the workspace (at most two a CTA) and
+// are joined by paged_join_kernel in the order of the CTAs.
+//   warps 0-7   write the query tile, then softmax: a warp reads 16 rows x 128 keys of S in the 16-lane quad layout.  Where no
+//               sequence has that many rows the warps behind the last take no part in the key loop.
 //   warp 8      TMA producer: lane i fetches the i-th page of a key tile.  Columns behind the head size, and pages that are not
 //               held, lie outside the tensor map and arrive as zeros.
 //   warp 9      MMA issuer (an elected lane), owner of the TMEM allocation.
+// FEW: no sequence has more rows than a tile, so pages are read once: bound by memory.  One CTA per SM with all its shared
+//   memory in K and V stages (192 KB on their way), two S tiles, so that the next product runs under this one's softmax.
+// else: tiles share their keys through L2, and the products bound: two CTAs per SM, one's softmax under the other's products.
 // fp32 activations (ACT32) over bf16 pages: a query row q is two bf16 rows of the tile, hi = bf16(q) and lo = bf16(q - hi), 16
 // lanes apart, so that one product S = [hi; lo] K^T forms both and the softmax warp adds them (the pages are bf16 as they are: q
-// to 2^-18 is all that is rounded); the probabilities go back the same way, [p_hi; p_lo], and the two halves of O are added at the
+// to 2^-16 is all that is rounded); the probabilities go back the same way, [p_hi; p_lo], and the two halves of O are added at the
 // end.  64 query rows fill a tile then.
 using namespace tc;
 
 constexpr int KEYS = 128;   // of a key tile
+constexpr int ITEM_UNITS = 1;
 
-template <int HDP> struct TcPlan {   // HDP: 64 or 128, the head size padded
+template <int HDP, bool FEW> struct TcPlan {   // HDP: 64 or 128, the head size padded
   static constexpr int SUB = HDP / 64;
   static constexpr uint32_t SUB_BYTES = KEYS * 128, TILE_BYTES = SUB * SUB_BYTES;
-  static constexpr int STG = HDP == 64 ? 2 : 1;
+  static constexpr int STG = FEW ? (HDP == 64 ? 6 : 3) : (HDP == 64 ? 2 : 1);
   static constexpr uint32_t OFF_Q = 0, OFF_K = TILE_BYTES, OFF_V = OFF_K + STG * TILE_BYTES, OFF_BAR = OFF_V + STG * TILE_BYTES;
-  static constexpr uint32_t OFF_RED = OFF_BAR + 256;
+  static constexpr uint32_t OFF_SEG = OFF_BAR + 384, OFF_RED = OFF_SEG + 256;
   static constexpr uint32_t BYTES = OFF_RED + 2 * 128 * 4 + 1024;   // + alignment slack
-  static_assert(2 * (BYTES + 1024) <= 227 * 1024, "two CTAs share an SM");
+  static constexpr int CTAS = FEW ? 1 : 2;                          // per SM
+  static constexpr uint32_t TMEM = FEW ? 512 : 256;                 // S tiles, then O
+  static constexpr uint32_t O_COL = FEW ? 256 : 128;
+  static_assert(FEW ? BYTES + 64 <= 227 * 1024 : 2 * (BYTES + 1024) <= 227 * 1024, "shared memory of an SM");
 };
+constexpr int SEGMENTS = 4;   // parts of items that the producer is ahead of the others
 constexpr int TC_THREADS = 320, TC_WARP_TMA = 8, TC_WARP_MMA = 9;
-constexpr uint32_t TC_TMEM = 256;    // S in columns [0, 128), O behind it
 constexpr float TC_RESCALE = 8.0f;   // the softmax's reference point moves when a row's maximum outgrows it by 2^8
 
-enum TcBar : int { TB_Q = 0, TB_KF = 1, TB_KE = 3, TB_VF = 5, TB_VE = 7, TB_S = 9, TB_P1 = 10, TB_P2 = 11, TB_P3 = 12, TB_O = 13, TB_DRAIN = 14, TB_RED = 15, TB_COUNT = 16 };
+enum TcBar : int {
+  TB_Q = 0,      // query tile written
+  TB_S = 1,      // [2] S written by the MMA (FEW: two tiles in turn)
+  TB_P1 = 3,     // [2] first 64 keys of P written by the softmax warps, then 32, then 32 (FEW: in turn, as the softmax may be one
+  TB_P2 = 5,     //     key tile ahead of the products)
+  TB_P3 = 7,
+  TB_O = 9,      // FEW: P V of a key tile finished
+  TB_DONE = 10,  // the item's last product finished
+  TB_RED = 11,   // row sums in shared memory
+  TB_DRAIN = 12,
+  TB_KF = 13,    // [6] each: K, V stages full, empty
+  TB_KE = 19,
+  TB_VF = 25,
+  TB_VE = 31,
+  TB_GF = 37,    // [SEGMENTS] each: entries of the segment ring full, empty
+  TB_GE = 41,
+  TB_COUNT = 45
+};
 
-template <int HDP, bool ACT32>
-__global__ void __launch_bounds__(TC_THREADS, 2) paged_tc_kernel(const __grid_constant__ CUtensorMap map_k, const __grid_constant__ CUtensorMap map_v,
-                                                                 const AttnArgs p) {
-  using PL = TcPlan<HDP>;
+// Sum over the first n tiles of c = 2^shift tokens, from position `pos` on, of the key tiles that each sees: ceil((pos + (i + 1) c) / 128).
+// With k = 128 / c tiles to a key tile that is floor((i + d) / k), d = floor((pos + c + 127) / c), whose sums have a closed form.
+__device__ __forceinline__ int64_t key_tiles_of(int pos, int shift, int n) {
+  const int k = 7 - shift;
+  auto below = [&](int64_t x) {   // sum of floor(i / 2^k) over i < x
+    const int64_t q = x >> k;
+    return (q * (q - 1) << k) / 2 + q * (x - (q << k));
+  };
+  const int64_t d = ((int64_t)pos + (1 << shift) + KEYS - 1) >> shift;
+  return below(d + n) - below(d);
+}
+
+// The items in their order (sequences, their tiles of 2^tile_shift tokens, heads) and a CTA's share of their units.  Every warp
+// walks by itself; all lanes hold the same.
+struct Walk {
+  int64_t share, left;      // units of a CTA; of this one's, those still to come
+  int64_t item_unit;        // first unit of the current item
+  int from;                 // units of the current item that belong to the CTAs before
+  int seq, tile, head;      // current item; head: key/value head x parts of its group
+  int start, count, pos0;   // of its sequence
+
+  __device__ __forceinline__ int tiles(const AttnArgs& p) const { return (count + (1 << p.tile_shift) - 1) >> p.tile_shift; }
+  __device__ __forceinline__ int last(const AttnArgs& p) const { return pos0 + min((tile + 1) << p.tile_shift, count) - 1; }   // key any row of the item sees
+  __device__ __forceinline__ int key_tiles(const AttnArgs& p) const { return last(p) / KEYS + 1; }
+  // units of a sequence's first n tiles, all of them full, for one head
+  static __device__ __forceinline__ int64_t units_of(const AttnArgs& p, int pos0, int n) {
+    return n <= 0 ? 0 : key_tiles_of(pos0, p.tile_shift, n) + (int64_t)n * ITEM_UNITS;
+  }
+  static __device__ __forceinline__ int64_t units_of(const AttnArgs& p, const Sequence& s) {
+    if (!s.good || s.count == 0) return 0;
+    const int full = (s.count - 1) >> p.tile_shift;
+    return units_of(p, s.length - s.count, full) + (s.length + KEYS - 1) / KEYS + ITEM_UNITS;
+  }
+  __device__ __forceinline__ void enter(const AttnArgs& p, int b) {
+    const Sequence s = paged::sequence(p.batch, b);
+    seq = b; start = s.start; count = s.good ? s.count : 0; pos0 = s.length - s.count;
+  }
+
+  __device__ __forceinline__ void begin(const AttnArgs& p, int cta) {
+    const int lane = threadIdx.x & 31, n = p.batch.n_seqs;
+    int64_t total = 0;
+    for (int b = lane; b < n; b += 32) total += units_of(p, paged::sequence(p.batch, b));
+#pragma unroll
+    for (int o = 16; o > 0; o >>= 1) total += __shfl_xor_sync(0xffffffffu, total, o);
+    total *= p.items;
+    share = max((total + p.ctas - 1) / p.ctas, (int64_t)p.least_units);
+    const int64_t lo = (int64_t)cta * share;
+    left = min(total - lo, share);
+    item_unit = 0; from = seq = tile = head = start = count = pos0 = 0;
+    if (left <= 0) return;
+    int64_t before = 0;
+    for (int s0 = 0; s0 < n; s0 += 32) {
+      const int64_t mine = s0 + lane < n ? units_of(p, paged::sequence(p.batch, s0 + lane)) * p.items : 0;
+      int64_t incl = mine;
+#pragma unroll
+      for (int o = 1; o < 32; o <<= 1) {
+        const int64_t up = __shfl_up_sync(0xffffffffu, incl, o);
+        if (lane >= o) incl += up;
+      }
+      const unsigned past = __ballot_sync(0xffffffffu, before + incl > lo);
+      if (past != 0) {
+        const int src = __ffs(past) - 1;
+        before += __shfl_sync(0xffffffffu, incl - mine, src);
+        enter(p, s0 + src);
+        break;
+      }
+      before += __shfl_sync(0xffffffffu, incl, 31);
+    }
+    // the last tile that begins at or before the share, 32 candidates at a time
+    const int64_t rel = lo - before;
+    int a = 0, b = tiles(p);
+    while (b - a > 1) {
+      const int step = (b - a + 31) / 32, t = a + lane * step;
+      const unsigned fits = __ballot_sync(0xffffffffu, t < b && units_of(p, pos0, t) * p.items <= rel);
+      a += (__popc(fits) - 1) * step;
+      b = min(b, a + step);
+    }
+    tile = a;
+    const int64_t in = rel - units_of(p, pos0, tile) * p.items;
+    const int units = key_tiles(p) + ITEM_UNITS;
+    head = (int)(in / units);
+    from = (int)(in - (int64_t)head * units);
+    item_unit = lo - from;
+  }
+  // Key tiles [kt0, kt1) of the current item are this CTA's (there may be none).
+  __device__ __forceinline__ void take(const AttnArgs& p, int* kt0, int* kt1) {
+    const int units = key_tiles(p) + ITEM_UNITS;
+    const int to = (int)min((int64_t)units, from + left);
+    *kt0 = max(from - ITEM_UNITS, 0);
+    *kt1 = max(to - ITEM_UNITS, 0);
+    left -= to - from;
+  }
+  __device__ __forceinline__ void advance(const AttnArgs& p) {
+    item_unit += key_tiles(p) + ITEM_UNITS;
+    from = 0;
+    if (++head < p.items) return;
+    head = 0;
+    if (++tile < tiles(p)) return;
+    tile = 0;
+    do {
+      if (seq + 1 >= p.batch.n_seqs) { left = 0; return; }   // cannot happen: the shares end with the last item
+      enter(p, seq + 1);
+    } while (count == 0);
+  }
+};
+
+// One part of an item.  The producer's warp walks and puts the parts into a ring in shared memory, where the other roles read them
+// (the softmax has no registers to hold them: with a walk of its own in each warp a key tile took a quarter longer).
+struct __align__(16) Segment {
+  int n, k_begin, k_end, last;    // key tiles (0: no more work); keys [k_begin, k_end); the last key any row sees
+  int token0, rows, heads, pos;   // first token row; rows; query heads of the part; position of the first token
+  int head0, kvh, seq;            // first query head; key/value head; sequence
+  int slot;                       // workspace slot of a part; -1: all keys of the item, written out
+};
+static_assert(sizeof(Segment) * SEGMENTS <= 256, "segment ring");
+template <int R> __device__ __forceinline__ Segment segment(const AttnArgs& p, const Walk& w, int kt0, int kt1) {
+  Segment g;
+  const int part = p.parts > 1 ? w.head % p.parts : 0;
+  g.kvh = p.parts > 1 ? w.head / p.parts : w.head;
+  g.head0 = g.kvh * p.group + part * R;
+  g.heads = min(R, p.group - part * R);
+  const int t0 = w.tile << p.tile_shift;
+  g.token0 = w.start + t0;
+  g.rows = min(1 << p.tile_shift, w.count - t0) * g.heads;
+  g.pos = w.pos0 + t0;
+  g.seq = w.seq;
+  g.last = w.last(p);
+  g.n = kt1 - kt0;
+  g.k_begin = kt0 * KEYS;
+  g.k_end = min(g.last + 1, kt1 * KEYS);
+  g.slot = kt0 == 0 && kt1 == w.key_tiles(p) ? -1 : 2 * (int)blockIdx.x + (kt0 == 0 ? 1 : 0);
+  return g;
+}
+
+template <int HDP, bool ACT32, bool FEW>
+__global__ void __launch_bounds__(TC_THREADS, (TcPlan<HDP, FEW>::CTAS)) paged_tc_kernel(const __grid_constant__ CUtensorMap map_k,
+                                                                                       const __grid_constant__ CUtensorMap map_v, const AttnArgs p) {
+  using PL = TcPlan<HDP, FEW>;
   constexpr int STG = PL::STG;
   constexpr int R = ACT32 ? 64 : 128;   // query rows of a tile
   extern __shared__ uint8_t smem_raw[];
@@ -373,101 +532,121 @@ __global__ void __launch_bounds__(TC_THREADS, 2) paged_tc_kernel(const __grid_co
   auto bar = [&](int i) { return smem_base + PL::OFF_BAR + 8u * (uint32_t)i; };
   const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
   int* const status = g_wait_status;
+  __shared__ int s_abort;
 
   mca_pdl_launch_dependents();
+  if ((int)blockIdx.x == p.ctas) {   // one more CTA looks the sequences over
+    mca_pdl_wait();
+    if constexpr (ACT32) look_over<float>(p);
+    else look_over<__nv_bfloat16>(p);
+    return;
+  }
   if (warp == TC_WARP_MMA) {
-    tmem_alloc(smem_u32(const_cast<uint32_t*>(tmem_slot)), TC_TMEM);
+    tmem_alloc(smem_u32(const_cast<uint32_t*>(tmem_slot)), PL::TMEM);
     tmem_relinquish();
   }
   if (warp == TC_WARP_TMA && lane == 0) {
     prefetch_tensormap(&map_k);
     prefetch_tensormap(&map_v);
   }
-  mca_pdl_wait();   // from here on the results of the kernels before this one are complete and visible
-  const int kvh = blockIdx.y, split = blockIdx.z;
-  int seq = 0, row0 = 0;
-  Sequence sq{0, 0, 0, false};
-  // tiles are handed out from the last: those of a chunk see the most keys
-  const bool work = (int)blockIdx.x < p.tiles && find_tile(p.batch, p.group, R, p.tiles - 1 - (int)blockIdx.x, &seq, &row0, &sq);
-  if ((int)blockIdx.x == p.tiles && blockIdx.y == 0 && blockIdx.z == 0) {
-    if constexpr (ACT32) look_over<float>(p);
-    else look_over<__nv_bfloat16>(p);
-  }
-  const int rows = min(R, sq.count * p.group - row0);     // of this tile
-  const int pos0 = sq.length - sq.count;
-  const int last = pos0 + (row0 + rows - 1) / p.group;    // the last key that any row of the tile sees
-  const int k_begin = split * p.split_len;
-  const int k_end = min(last + 1, k_begin + p.split_len);
-  const int n = work && k_end > k_begin ? (k_end - k_begin + KEYS - 1) / KEYS : 0;
-  const int n_act = (rows + 15) / 16;                     // softmax warps at work
-  if (tid == 0 && n > 0) {
+  if (tid == 0) {
     for (int i = 0; i < TB_COUNT; ++i) {
-      const bool by_softmax = (i >= TB_P1 && i <= TB_P3) || i == TB_RED;
-      mbar_init(bar(i), i == TB_Q ? 8u : (by_softmax ? (uint32_t)n_act : 1u));
+      const bool by_softmax = (i >= TB_P1 && i < TB_O) || i == TB_RED;
+      mbar_init(bar(i), i == TB_Q ? 8u : (by_softmax ? (uint32_t)p.warps : (i >= TB_GE ? 9u : 1u)));
     }
     asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
   }
-  // does the split meet a page that is not held?
-  bool hole = false;
-  if (n > 0) {
-    const int shift = p.batch.page_shift;
-    for (int i = (k_begin >> shift) + tid; i <= (k_end - 1) >> shift; i += TC_THREADS) {
-      const int id = p.batch.table[(int64_t)seq * p.batch.table_stride + i];
-      if (id < 0 || id >= p.batch.n_pages) {
-        hole = true;
-        if (id != -1 && kvh == 0) paged::refuse(paged::REFUSED_PAGE, seq, id);
-      }
-    }
-  }
-  __shared__ int s_abort;
+  mca_pdl_wait();   // from here on the results of the kernels before this one are complete and visible
   if (tid == 32) s_abort = *reinterpret_cast<volatile int*>(status);
   tc_fence_before();
-  const bool holes = __syncthreads_or(hole) != 0;
+  __syncthreads();
   tc_fence_after();
   const uint32_t tmem_base = *tmem_slot;
-  if (n == 0 || s_abort != 0) {   // nothing to do, or an earlier CTA gave up (a uniform decision, before any copy or product)
-    if (warp == TC_WARP_MMA) tmem_dealloc(tmem_base, TC_TMEM);
+  if (s_abort != 0) {   // an earlier CTA gave up (a uniform decision, before any copy or product)
+    if (warp == TC_WARP_MMA) tmem_dealloc(tmem_base, PL::TMEM);
     return;
   }
   bool ok = true;
+  int c = 0;      // key tiles so far: stages and phases go by it
+  int item = 0;   // parts of items so far
+  Segment* const ring = reinterpret_cast<Segment*>(smem + PL::OFF_SEG);
+  auto next_segment = [&](int stage) -> const Segment* {   // for the roles but the producer; null: no more
+    ok = __all_sync(0xffffffffu, mbar_wait(bar(TB_GF + item % SEGMENTS), (uint32_t)((item / SEGMENTS) & 1), status, stage, item));
+    return ok && ring[item % SEGMENTS].n > 0 ? ring + item % SEGMENTS : nullptr;
+  };
+  auto release_segment = [&]() {
+    __syncwarp();
+    if (lane == 0) mbar_arrive(bar(TB_GE + item % SEGMENTS));
+    ++item;
+  };
 
   if (warp == TC_WARP_TMA) {
     // ------------------------------------------------------------------ producer
     const int shift = p.batch.page_shift;
     const int box_rows = shift >= 7 ? KEYS : 1 << shift;
     const int boxes = KEYS / box_rows;
-    auto page_at = [&](int j) {   // this lane's page of key tile j; n_pages: none, zeros arrive
-      const int pos = k_begin + j * KEYS + lane * box_rows;
-      if (lane >= boxes || pos >= k_end || j >= n) return p.batch.n_pages;
-      const int id = p.batch.table[(int64_t)seq * p.batch.table_stride + (pos >> shift)];
-      return id >= 0 && id < p.batch.n_pages ? id : p.batch.n_pages;
-    };
-    int page = page_at(0);
     int issued_k = 0, issued_v = 0;
-    for (int j = 0; j < n && ok; ++j) {
-      const int st = j % STG;
-      const uint32_t ph = (uint32_t)((j / STG) & 1);
-      const int next = page_at(j + 1);
-      const int slot = (k_begin + j * KEYS + lane * box_rows) & ((1 << shift) - 1);
-      ok = __all_sync(0xffffffffu, mbar_wait(bar(TB_KE + st), ph ^ 1u, status, 10, j));
-      if (!ok) break;
-      if (lane == 0) mbar_expect_tx(bar(TB_KF + st), PL::TILE_BYTES);
-      __syncwarp();
-      if (lane < boxes)
+    Walk w;
+    w.begin(p, blockIdx.x);
+    if (p.meta != nullptr && lane == 0) p.meta[2 * blockIdx.x].x = -1;   // no item ends here that another CTA began, unless found below
+    bool more = w.left > 0, first = true;
+    while (ok) {
+      int kt0 = 0, kt1 = 0;
+      Segment g;
+      g.n = 0;
+      if (more) {
+        w.take(p, &kt0, &kt1);
+        g = segment<R>(p, w, kt0, kt1);
+        if (first && p.meta != nullptr && lane == 0 && g.n > 0 && kt0 > 0 && kt1 == w.key_tiles(p)) {   // what the join needs
+          p.meta[2 * blockIdx.x] = make_int4((int)((w.item_unit + ITEM_UNITS) / w.share), g.token0, g.head0, g.rows);
+          p.meta[2 * blockIdx.x + 1] = make_int4(g.heads, 0, 0, 0);
+        }
+        first = false;
+      }
+      if (!more || g.n > 0) {
+        ok = __all_sync(0xffffffffu, mbar_wait(bar(TB_GE + item % SEGMENTS), (uint32_t)((item / SEGMENTS) & 1) ^ 1u, status, 9, item));
+        if (!ok) break;
+        if (lane == 0) {
+          ring[item % SEGMENTS] = g;
+          mbar_arrive(bar(TB_GF + item % SEGMENTS));
+        }
+        ++item;
+      }
+      if (!more) break;
+      auto page_at = [&](int j) {   // this lane's page of key tile j; n_pages: none, zeros arrive
+        const int pos = g.k_begin + j * KEYS + lane * box_rows;
+        if (lane >= boxes || pos >= g.k_end || j >= g.n) return p.batch.n_pages;
+        const int id = p.batch.table[(int64_t)g.seq * p.batch.table_stride + (pos >> shift)];
+        return id >= 0 && id < p.batch.n_pages ? id : p.batch.n_pages;
+      };
+      int page = page_at(0);
+      for (int j = 0; j < g.n; ++j, ++c) {
+        const int st = c % STG;
+        const uint32_t ph = (uint32_t)((c / STG) & 1);
+        const int next = page_at(j + 1);
+        const int slot = (g.k_begin + j * KEYS + lane * box_rows) & ((1 << shift) - 1);
+        ok = __all_sync(0xffffffffu, mbar_wait(bar(TB_KE + st), ph ^ 1u, status, 10, c));
+        if (!ok) break;
+        if (lane == 0) mbar_expect_tx(bar(TB_KF + st), PL::TILE_BYTES);
+        __syncwarp();
+        if (lane < boxes)
 #pragma unroll
-        for (int s = 0; s < PL::SUB; ++s)
-          tma_load_4d(smem_base + PL::OFF_K + st * PL::TILE_BYTES + s * PL::SUB_BYTES + lane * box_rows * 128, &map_k, bar(TB_KF + st), s * 64, kvh, slot, page);
-      issued_k = j + 1;
-      ok = __all_sync(0xffffffffu, mbar_wait(bar(TB_VE + st), ph ^ 1u, status, 11, j));
-      if (!ok) break;
-      if (lane == 0) mbar_expect_tx(bar(TB_VF + st), PL::TILE_BYTES);
-      __syncwarp();
-      if (lane < boxes)
+          for (int s = 0; s < PL::SUB; ++s)
+            tma_load_4d(smem_base + PL::OFF_K + st * PL::TILE_BYTES + s * PL::SUB_BYTES + lane * box_rows * 128, &map_k, bar(TB_KF + st), s * 64, g.kvh, slot, page);
+        issued_k = c + 1;
+        ok = __all_sync(0xffffffffu, mbar_wait(bar(TB_VE + st), ph ^ 1u, status, 11, c));
+        if (!ok) break;
+        if (lane == 0) mbar_expect_tx(bar(TB_VF + st), PL::TILE_BYTES);
+        __syncwarp();
+        if (lane < boxes)
 #pragma unroll
-        for (int s = 0; s < PL::SUB; ++s)
-          tma_load_4d(smem_base + PL::OFF_V + st * PL::TILE_BYTES + s * PL::SUB_BYTES + lane * box_rows * 128, &map_v, bar(TB_VF + st), s * 64, kvh, slot, page);
-      issued_v = j + 1;
-      page = next;
+          for (int s = 0; s < PL::SUB; ++s)
+            tma_load_4d(smem_base + PL::OFF_V + st * PL::TILE_BYTES + s * PL::SUB_BYTES + lane * box_rows * 128, &map_v, bar(TB_VF + st), s * 64, g.kvh, slot, page);
+        issued_v = c + 1;
+        page = next;
+      }
+      more = w.left > 0;
+      if (more) w.advance(p);
     }
     if (!ok) {   // copies in flight get a bounded time to land before the CTA's memory is released
       for (int j = max(0, issued_k - STG); j < issued_k; ++j) mbar_wait(bar(TB_KF + (j % STG)), (uint32_t)((j / STG) & 1), status, 13, j);
@@ -480,301 +659,371 @@ __global__ void __launch_bounds__(TC_THREADS, 2) paged_tc_kernel(const __grid_co
     constexpr uint32_t IDESC_QK = make_idesc_fmt(128, KEYS, 0, 0, 1), IDESC_PV = make_idesc_fmt(128, HDP, 0, 1, 1);
     const uint64_t dq = make_desc(smem_base + PL::OFF_Q, 16, 1024);
     const uint64_t dk0 = make_desc(smem_base + PL::OFF_K, 16, 1024), dv0 = make_desc(smem_base + PL::OFF_V, PL::SUB_BYTES, 1024);
-    auto issue_qk = [&](int st) {
-      const uint64_t dk = dk0 + (uint64_t)((st * PL::TILE_BYTES) >> 4);
+    auto issue_qk = [&](int t) {   // of key tile t (of the CTA's)
+      const uint64_t dk = dk0 + (uint64_t)(((t % STG) * PL::TILE_BYTES) >> 4);
+      const uint32_t d = tm + (FEW ? (uint32_t)(t & 1) * 128u : 0u);
 #pragma unroll
       for (int kk = 0; kk < HDP / 16; ++kk) {
         const uint32_t off = ((uint32_t)(kk >> 2) * PL::SUB_BYTES + (uint32_t)(kk & 3) * 32u) >> 4;
-        umma_ss_if<false>(leader, tm, dq + off, dk + off, IDESC_QK, kk > 0 ? 1u : 0u);
+        umma_ss_if<false>(leader, d, dq + off, dk + off, IDESC_QK, kk > 0 ? 1u : 0u);
       }
+      umma_commit_if(leader, bar(TB_S + (FEW ? t & 1 : 0)));   // covers every product before it
+      umma_commit_if(leader, bar(TB_KE + t % STG));
     };
-    auto issue_pv = [&](int st, bool first, int lo, int hi) {   // 16 keys a step
-      const uint64_t dv = dv0 + (uint64_t)((st * PL::TILE_BYTES) >> 4);
+    auto issue_pv = [&](int t, bool first, int lo, int hi) {   // 16 keys a step
+      const uint64_t dv = dv0 + (uint64_t)(((t % STG) * PL::TILE_BYTES) >> 4);
+      const uint32_t a = tm + (FEW ? (uint32_t)(t & 1) * 128u : 0u);
 #pragma unroll
       for (int kk = lo; kk < hi; ++kk)
-        umma_ts_if<false>(leader, tm + 128, tm + (uint32_t)(kk * 8), dv + (uint64_t)((uint32_t)kk * (2048u >> 4)), IDESC_PV, (first && kk == 0) ? 0u : 1u);
+        umma_ts_if<false>(leader, tm + PL::O_COL, a + (uint32_t)(kk * 8), dv + (uint64_t)((uint32_t)kk * (2048u >> 4)), IDESC_PV, (first && kk == 0) ? 0u : 1u);
     };
-    auto wait = [&](int b, uint32_t ph, int stage, int j) { return __all_sync(0xffffffffu, mbar_wait(bar(b), ph, status, stage, j)); };
-    ok = wait(TB_Q, 0, 20, 0) && wait(TB_KF, 0, 21, 0);
-    if (ok) {
-      tc_fence_after();
-      issue_qk(0);
-      umma_commit_if(leader, bar(TB_S));
-      umma_commit_if(leader, bar(TB_KE));
-    }
-    for (int j = 0; j < n && ok; ++j) {
-      const int st = j % STG, stn = (j + 1) % STG;
-      const uint32_t ph = (uint32_t)((j / STG) & 1), phn = (uint32_t)(((j + 1) / STG) & 1), pj = (uint32_t)(j & 1);
-      if (!(ok = wait(TB_VF + st, ph, 22, j))) break;
-      if (!(ok = wait(TB_P1, pj, 28, j))) break;
-      tc_fence_after();
-      issue_pv(st, j == 0, 0, 4);
-      if (j + 1 < n && !(ok = wait(TB_KF + stn, phn, 25, j))) break;
-      if (!(ok = wait(TB_P2, pj, 40, j))) break;
-      tc_fence_after();
-      issue_pv(st, j == 0, 4, 6);
-      if (!(ok = wait(TB_P3, pj, 23, j))) break;
-      tc_fence_after();
-      issue_pv(st, j == 0, 6, 8);
-      umma_commit_if(leader, bar(TB_VE + st));
-      if (j + 1 < n) {
-        issue_qk(stn);
-        umma_commit_if(leader, bar(TB_S));   // covers every product before it, P V(j) among them
-        umma_commit_if(leader, bar(TB_KE + stn));
-      } else {
-        umma_commit_if(leader, bar(TB_O));
+    auto wait = [&](int b, uint32_t ph, int stage) { return __all_sync(0xffffffffu, mbar_wait(bar(b), ph & 1u, status, stage, c)); };
+    while (const Segment* g = next_segment(19)) {
+      const int n = g->n;
+      {
+        ok = wait(TB_Q, item, 20) && wait(TB_KF + c % STG, c / STG, 21);
+        if (!ok) break;
+        tc_fence_after();
+        issue_qk(c);
+        for (int j = 0; j < n; ++j, ++c) {
+          if (FEW && j + 1 < n) {
+            if (!(ok = wait(TB_KF + (c + 1) % STG, (c + 1) / STG, 25))) break;
+            tc_fence_after();
+            issue_qk(c + 1);
+          }
+          if (!(ok = wait(TB_VF + c % STG, c / STG, 22))) break;
+          if (!(ok = wait(TB_P1 + (FEW ? c & 1 : 0), FEW ? c >> 1 : c, 28))) break;
+          tc_fence_after();
+          issue_pv(c, j == 0, 0, 4);
+          if (!FEW && j + 1 < n && !(ok = wait(TB_KF + (c + 1) % STG, (c + 1) / STG, 25))) break;
+          if (!(ok = wait(TB_P2 + (FEW ? c & 1 : 0), FEW ? c >> 1 : c, 40))) break;
+          tc_fence_after();
+          issue_pv(c, j == 0, 4, 6);
+          if (!(ok = wait(TB_P3 + (FEW ? c & 1 : 0), FEW ? c >> 1 : c, 23))) break;
+          tc_fence_after();
+          issue_pv(c, j == 0, 6, 8);
+          umma_commit_if(leader, bar(TB_VE + c % STG));
+          if (FEW) umma_commit_if(leader, bar(TB_O));
+          if (j + 1 == n) umma_commit_if(leader, bar(TB_DONE));
+          else if (!FEW) issue_qk(c + 1);
+        }
       }
+      if (!ok) break;
+      release_segment();
     }
     umma_commit_if(leader, bar(TB_DRAIN));   // the tensor pipe is idle (bounded) before TMEM is freed
     mbar_wait(bar(TB_DRAIN), 0, status, 27, 0);
     __syncwarp();
   } else {
-    // ------------------------------------------------------------------ the query tile, 16-byte pieces in the swizzled layout
-    constexpr int CH = HDP / 8;
-    for (int i = tid; i < rows * CH; i += 256) {
-      const int r = i / CH, c = i - r * CH;
-      const int row = row0 + r, t = row / p.group, h = kvh * p.group + row - t * p.group;
-      const char* src = p.q + (int64_t)(sq.start + t) * p.q_st + h * p.q_sh;
-      const bool in = c * 8 < p.hs;
-      const uint32_t sub = PL::OFF_Q + (uint32_t)(c >> 3) * PL::SUB_BYTES;
-      if constexpr (ACT32) {
-        float x[8];
-#pragma unroll
-        for (int k = 0; k < 8; ++k) x[k] = 0.f;
-        if (in) {
-          const float4 a = mca_ld_f4(reinterpret_cast<const float*>(src) + c * 8), b = mca_ld_f4(reinterpret_cast<const float*>(src) + c * 8 + 4);
-          x[0] = a.x; x[1] = a.y; x[2] = a.z; x[3] = a.w; x[4] = b.x; x[5] = b.y; x[6] = b.z; x[7] = b.w;
-        }
-        uint32_t hi[4], lo[4];
-#pragma unroll
-        for (int k = 0; k < 4; ++k) {
-          hi[k] = pack_bf16(x[2 * k], x[2 * k + 1]);
-          lo[k] = pack_bf16(x[2 * k] - __uint_as_float(hi[k] << 16), x[2 * k + 1] - __uint_as_float(hi[k] & 0xffff0000u));
-        }
-        const int r_hi = (r >> 4) * 32 + (r & 15);
-        const uint32_t at = sub + (uint32_t)(r_hi * 128 + (((c & 7) ^ (r_hi & 7)) << 4));
-        *reinterpret_cast<uint4*>(smem + at) = make_uint4(hi[0], hi[1], hi[2], hi[3]);
-        *reinterpret_cast<uint4*>(smem + at + 16 * 128) = make_uint4(lo[0], lo[1], lo[2], lo[3]);   // 16 rows on: the same swizzle
-      } else {
-        uint4 v = make_uint4(0, 0, 0, 0);
-        if (in) v = *(reinterpret_cast<const uint4*>(src) + c);
-        *reinterpret_cast<uint4*>(smem + sub + (uint32_t)(r * 128 + (((c & 7) ^ (r & 7)) << 4))) = v;
-      }
-    }
-    asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
-    __syncwarp();
-    if (lane == 0) mbar_arrive(bar(TB_Q));
-
-    // ------------------------------------------------------------------ softmax
+    constexpr int CH = HDP / 8;   // 16-byte pieces of a row
     const int rank = ACT32 ? warp : (warp & 3) * 2 + (warp >> 2);   // the 16 rows of the tile that are this warp's
     const int lane_base = ACT32 ? warp * 32 : rank * 16;
     const int quad = lane & 3;
     const int r0 = rank * 16 + (lane >> 2);
     float* red_l = reinterpret_cast<float*>(smem + PL::OFF_RED);
     float* red_m = red_l + 128;
-    if (rank < n_act) {
-      const uint32_t t_s = tmem_base + ((uint32_t)lane_base << 16), t_o = t_s + 128;
-      constexpr uint32_t LO = 16u << 16;   // ACT32: the low halves' lanes
-      int lim[2];   // the last key that rows r0 and r0 + 8 see
+    const float scale = p.scale_log2;
+    const float2 scale2 = make_float2(scale, scale);
+    while (const Segment* gp = next_segment(18)) {
+      const Segment& g = *gp;
+      {
+        // ---------------------------------------------------------------- the query tile, 16-byte pieces in the swizzled layout
+        for (int i = tid; i < g.rows * CH; i += 256) {
+          const int r = i / CH, ch = i - r * CH;
+          const int t = r / g.heads;
+          const char* src = p.q + (int64_t)(g.token0 + t) * p.q_st + (g.head0 + r - t * g.heads) * p.q_sh;
+          const bool in = ch * 8 < p.hs;
+          const uint32_t sub = PL::OFF_Q + (uint32_t)(ch >> 3) * PL::SUB_BYTES;
+          if constexpr (ACT32) {
+            float x[8];
 #pragma unroll
-      for (int h = 0; h < 2; ++h) lim[h] = r0 + 8 * h < rows ? pos0 + (row0 + r0 + 8 * h) / p.group : -1;
-      const int lim_min = pos0 + row0 / p.group;   // of the tile's first row
-      const float scale = p.scale_log2;
-      const float2 scale2 = make_float2(scale, scale);
-      float m_used[2] = {-INFINITY, -INFINITY}, l[2] = {0.f, 0.f};
-      for (int j = 0; j < n && ok; ++j) {
-        ok = __all_sync(0xffffffffu, mbar_wait(bar(TB_S), (uint32_t)(j & 1), status, 30, j));
-        if (!ok) break;
-        tc_fence_after();
-        // s[4g + 2h + e] = logit of row r0 + 8h, key 8g + 2 quad + e
-        uint32_t s[64];
-        if constexpr (ACT32) {
+            for (int k = 0; k < 8; ++k) x[k] = 0.f;
+            if (in) {
+              const float4 a = mca_ld_f4(reinterpret_cast<const float*>(src) + ch * 8), b = mca_ld_f4(reinterpret_cast<const float*>(src) + ch * 8 + 4);
+              x[0] = a.x; x[1] = a.y; x[2] = a.z; x[3] = a.w; x[4] = b.x; x[5] = b.y; x[6] = b.z; x[7] = b.w;
+            }
+            uint32_t hi[4], lo[4];
 #pragma unroll
-          for (int c = 0; c < 4; ++c) {
-            uint32_t lo[16];
-            tmem_ldq256_x2(t_s + 32 * c, s + 16 * c);
-            tmem_ldq256_x2(t_s + 32 * c + 16, s + 16 * c + 8);
-            tmem_ldq256_x2(t_s + LO + 32 * c, lo);
-            tmem_ldq256_x2(t_s + LO + 32 * c + 16, lo + 8);
-            tmem_wait_ld();
-#pragma unroll
-            for (int i = 0; i < 16; ++i) s[16 * c + i] = __float_as_uint(__uint_as_float(s[16 * c + i]) + __uint_as_float(lo[i]));
+            for (int k = 0; k < 4; ++k) {
+              hi[k] = pack_bf16(x[2 * k], x[2 * k + 1]);
+              lo[k] = pack_bf16(x[2 * k] - __uint_as_float(hi[k] << 16), x[2 * k + 1] - __uint_as_float(hi[k] & 0xffff0000u));
+            }
+            const int r_hi = (r >> 4) * 32 + (r & 15);
+            const uint32_t at = sub + (uint32_t)(r_hi * 128 + (((ch & 7) ^ (r_hi & 7)) << 4));
+            *reinterpret_cast<uint4*>(smem + at) = make_uint4(hi[0], hi[1], hi[2], hi[3]);
+            *reinterpret_cast<uint4*>(smem + at + 16 * 128) = make_uint4(lo[0], lo[1], lo[2], lo[3]);   // 16 rows on: the same swizzle
+          } else {
+            uint4 v = make_uint4(0, 0, 0, 0);
+            if (in) v = *(reinterpret_cast<const uint4*>(src) + ch);
+            *reinterpret_cast<uint4*>(smem + sub + (uint32_t)(r * 128 + (((ch & 7) ^ (r & 7)) << 4))) = v;
           }
-        } else {
-          tmem_ldq256_x8(t_s, s);
-          tmem_ldq256_x8(t_s + 64, s + 32);
-          tmem_wait_ld();
         }
-        const int key0 = k_begin + j * KEYS;
-        if (key0 + KEYS - 1 > lim_min) {
+        asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
+        __syncwarp();
+        if (lane == 0) mbar_arrive(bar(TB_Q));
+
+        // ---------------------------------------------------------------- softmax
+        if (rank < p.warps) {
+          bool hole = false;   // does the part meet a page that is not held?
+          for (int i = (g.k_begin >> p.batch.page_shift) + lane; i <= (g.k_end - 1) >> p.batch.page_shift; i += 32) {
+            const int id = p.batch.table[(int64_t)g.seq * p.batch.table_stride + i];
+            if (id < 0 || id >= p.batch.n_pages) {
+              hole = true;
+              if (id != -1 && rank == 0 && g.head0 == 0) paged::refuse(paged::REFUSED_PAGE, g.seq, id);
+            }
+          }
+          const bool holes = __any_sync(0xffffffffu, hole);
+          constexpr uint32_t LO = 16u << 16;   // ACT32: the low halves' lanes
+          const uint32_t t_row = tmem_base + ((uint32_t)lane_base << 16), t_o = t_row + PL::O_COL;
+          int lim[2];   // the last key that rows r0 and r0 + 8 see
 #pragma unroll
-          for (int i = 0; i < 64; ++i)
-            if (key0 + 8 * (i >> 2) + 2 * quad + (i & 1) > lim[(i >> 1) & 1]) s[i] = 0xff800000u;
-          if (key0 + KEYS > last + 1 && j == n - 1) {
-            // what lies behind the last key is nobody's: its values become zeros, since 0 x infinity is not
-            ok = __all_sync(0xffffffffu, mbar_wait(bar(TB_VF + (j % STG)), (uint32_t)((j / STG) & 1), status, 31, j));
+          for (int h = 0; h < 2; ++h) lim[h] = r0 + 8 * h < g.rows ? g.pos + (r0 + 8 * h) / g.heads : -1;
+          float m_used[2] = {-INFINITY, -INFINITY}, l[2] = {0.f, 0.f};
+          for (int j = 0; j < g.n; ++j, ++c) {
+            const uint32_t t_s = t_row + (FEW ? (uint32_t)(c & 1) * 128u : 0u);
+            ok = __all_sync(0xffffffffu, mbar_wait(bar(TB_S + (FEW ? c & 1 : 0)), (uint32_t)((FEW ? c >> 1 : c) & 1), status, 30, c));
             if (!ok) break;
-            uint8_t* v = smem + PL::OFF_V + (j % STG) * PL::TILE_BYTES;
-            const int z0 = last + 1 - key0;
-            for (int i = rank * 32 + lane; i < (KEYS - z0) * CH; i += n_act * 32) {
-              const int r = z0 + i / CH, c = i % CH;
-              *reinterpret_cast<uint4*>(v + (c >> 3) * PL::SUB_BYTES + r * 128 + (c & 7) * 16) = make_uint4(0, 0, 0, 0);
-            }
-            asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
-          }
-        }
-        if (holes) {
-#pragma unroll 1
-          for (int c = 0; c < 8; ++c) {   // 16 keys: within one page
-            const int pos = key0 + 16 * c;
-            if (pos >= k_end || page_of(p.batch, seq, pos, false) >= 0) continue;
+            tc_fence_after();
+            // s[4g + 2h + e] = logit of row r0 + 8h, key 8g + 2 quad + e
+            uint32_t s[64];
+            if constexpr (ACT32) {
 #pragma unroll
-            for (int i = 0; i < 64; ++i)
-              if ((i >> 3) == c) s[i] = 0xff800000u;
-          }
-        }
-        float mx[2];
+              for (int k = 0; k < 4; ++k) {
+                uint32_t lo[16];
+                tmem_ldq256_x2(t_s + 32 * k, s + 16 * k);
+                tmem_ldq256_x2(t_s + 32 * k + 16, s + 16 * k + 8);
+                tmem_ldq256_x2(t_s + LO + 32 * k, lo);
+                tmem_ldq256_x2(t_s + LO + 32 * k + 16, lo + 8);
+                tmem_wait_ld();
 #pragma unroll
-        for (int h = 0; h < 2; ++h) {
-          float ma = -INFINITY, mb = -INFINITY;
-#pragma unroll
-          for (int g = 0; g < 16; g += 2) {
-            ma = max3(ma, __uint_as_float(s[4 * g + 2 * h]), __uint_as_float(s[4 * g + 2 * h + 1]));
-            mb = max3(mb, __uint_as_float(s[4 * g + 4 + 2 * h]), __uint_as_float(s[4 * g + 4 + 2 * h + 1]));
-          }
-          mx[h] = fmaxf(ma, mb) * scale;
-        }
-        const bool grown = mx[0] > m_used[0] + TC_RESCALE || mx[1] > m_used[1] + TC_RESCALE;
-        if (j == 0 || __any_sync(0xffffffffu, grown)) {
-          float f[2];
-#pragma unroll
-          for (int h = 0; h < 2; ++h) {
-            mx[h] = fmaxf(mx[h], __shfl_xor_sync(0xffffffffu, mx[h], 1));
-            mx[h] = fmaxf(mx[h], __shfl_xor_sync(0xffffffffu, mx[h], 2));
-            float m_new = mx[h] > m_used[h] + TC_RESCALE ? mx[h] : m_used[h];
-            if (m_new == -INFINITY) m_new = 0.f;   // no key seen yet
-            f[h] = m_new != m_used[h] ? fast_exp2(m_used[h] - m_new) : 1.0f;
-            l[h] *= f[h];
-            m_used[h] = m_new;
-          }
-          if (j > 0) {   // P V(j - 1) finished before S(j) did
-#pragma unroll
-            for (int c = 0; c < (ACT32 ? 2 : 1) * (HDP / 16); ++c) {
-              const uint32_t at = t_o + (c % (HDP / 16)) * 16 + (c >= HDP / 16 ? LO : 0u);
-              uint32_t o[8];
-              tmem_ldq256_x2(at, o);
+                for (int i = 0; i < 16; ++i) s[16 * k + i] = __float_as_uint(__uint_as_float(s[16 * k + i]) + __uint_as_float(lo[i]));
+              }
+            } else {
+              tmem_ldq256_x8(t_s, s);
+              tmem_ldq256_x8(t_s + 64, s + 32);
               tmem_wait_ld();
-#pragma unroll
-              for (int i = 0; i < 8; ++i) o[i] = __float_as_uint(__uint_as_float(o[i]) * f[(i >> 1) & 1]);
-              tmem_stq256_x2(at, o);
             }
-          }
-        }
-        // p = 2^(s scale - m), handed over in three pieces (64, 32, 32 keys); the sum is of the unrounded ones
-        const float2 nm2[2] = {make_float2(-m_used[0], -m_used[0]), make_float2(-m_used[1], -m_used[1])};
-        float2 rs[2] = {make_float2(0.f, 0.f), make_float2(0.f, 0.f)};
-        auto quarter = [&](const int i) {
-          uint32_t pk[8], pl[ACT32 ? 8 : 1];
+            const int key0 = g.k_begin + j * KEYS;
+            if (key0 + KEYS - 1 > g.pos) {   // g.pos: the last key the tile's first row sees
 #pragma unroll
-          for (int g = 4 * i; g < 4 * i + 4; ++g)
+              for (int i = 0; i < 64; ++i)
+                if (key0 + 8 * (i >> 2) + 2 * quad + (i & 1) > lim[(i >> 1) & 1]) s[i] = 0xff800000u;
+              if (key0 + KEYS > g.last + 1) {
+                // what lies behind the last key is nobody's: its values become zeros, since 0 x infinity is not
+                ok = __all_sync(0xffffffffu, mbar_wait(bar(TB_VF + c % STG), (uint32_t)((c / STG) & 1), status, 31, c));
+                if (!ok) break;
+                uint8_t* v = smem + PL::OFF_V + (c % STG) * PL::TILE_BYTES;
+                const int z0 = g.last + 1 - key0;
+                for (int i = rank * 32 + lane; i < (KEYS - z0) * CH; i += p.warps * 32) {
+                  const int r = z0 + i / CH, ch = i % CH;
+                  *reinterpret_cast<uint4*>(v + (ch >> 3) * PL::SUB_BYTES + r * 128 + (ch & 7) * 16) = make_uint4(0, 0, 0, 0);
+                }
+                asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
+              }
+            }
+            if (holes) {
+#pragma unroll 1
+              for (int k = 0; k < 8; ++k) {   // 16 keys: within one page
+                const int pos = key0 + 16 * k;
+                if (pos >= g.k_end || page_of(p.batch, g.seq, pos, false) >= 0) continue;
+#pragma unroll
+                for (int i = 0; i < 64; ++i)
+                  if ((i >> 3) == k) s[i] = 0xff800000u;
+              }
+            }
+            float mx[2];
 #pragma unroll
             for (int h = 0; h < 2; ++h) {
-              const float2 xx = ffma2(make_float2(__uint_as_float(s[4 * g + 2 * h]), __uint_as_float(s[4 * g + 2 * h + 1])), scale2, nm2[h]);
-              const float p0 = fast_exp2(xx.x), p1 = fast_exp2(xx.y);
-              const uint32_t w = pack_bf16(p0, p1);
-              pk[2 * (g & 3) + h] = w;
-              if constexpr (ACT32) pl[2 * (g & 3) + h] = pack_bf16(p0 - __uint_as_float(w << 16), p1 - __uint_as_float(w & 0xffff0000u));
-              rs[h] = fadd2(rs[h], make_float2(p0, p1));
+              float ma = -INFINITY, mb = -INFINITY;
+#pragma unroll
+              for (int k = 0; k < 16; k += 2) {
+                ma = max3(ma, __uint_as_float(s[4 * k + 2 * h]), __uint_as_float(s[4 * k + 2 * h + 1]));
+                mb = max3(mb, __uint_as_float(s[4 * k + 4 + 2 * h]), __uint_as_float(s[4 * k + 4 + 2 * h + 1]));
+              }
+              mx[h] = fmaxf(ma, mb) * scale;
             }
-          tmem_stq128_x4(t_s + 16 * i, pk);
-          if constexpr (ACT32) tmem_stq128_x4(t_s + LO + 16 * i, pl);
-        };
-        auto hand_over = [&](int b) {
-          tmem_wait_st();
-          tc_fence_before();
-          __syncwarp();
-          if (lane == 0) mbar_arrive(bar(b));
-        };
-        quarter(0);
-        quarter(1);
-        hand_over(TB_P1);
-        quarter(2);
-        hand_over(TB_P2);
-        quarter(3);
-        hand_over(TB_P3);
-        l[0] += rs[0].x + rs[0].y;
-        l[1] += rs[1].x + rs[1].y;
-      }
-      if (ok) {
+            const bool grown = mx[0] > m_used[0] + TC_RESCALE || mx[1] > m_used[1] + TC_RESCALE;
+            if (j == 0 || __any_sync(0xffffffffu, grown)) {
+              float f[2];
 #pragma unroll
-        for (int h = 0; h < 2; ++h) {
-          l[h] += __shfl_xor_sync(0xffffffffu, l[h], 1);
-          l[h] += __shfl_xor_sync(0xffffffffu, l[h], 2);
-        }
-        if (quad == 0) {
-          red_l[r0] = l[0]; red_l[r0 + 8] = l[1];
-          red_m[r0] = m_used[0]; red_m[r0 + 8] = m_used[1];
-        }
-        __syncwarp();
-        if (lane == 0) mbar_arrive(bar(TB_RED));
-      }
-    }
-    // ------------------------------------------------------------------ epilogue: a lane a row, warps w and w + 4 half the columns each
-    const int first_row = ACT32 ? (warp & 3) * 16 : (warp & 3) * 32;
-    if (ok && first_row < rows) {
-      ok = __all_sync(0xffffffffu, mbar_wait(bar(TB_RED), 0, status, 36, n));
-      if (ok) ok = __all_sync(0xffffffffu, mbar_wait(bar(TB_O), 0, status, 34, n));
-      if (ok) {
-        tc_fence_after();
-        constexpr int OC = HDP / 2;
-        const int col0 = (warp >> 2) * OC;
-        const int r = ACT32 ? first_row + (lane & 15) : first_row + lane;
-        const uint32_t t_o = tmem_base + ((uint32_t)((warp & 3) * 32) << 16) + 128 + col0;
-        const bool mine = r < rows && (!ACT32 || lane < 16);
-        const int rr = min(r, rows - 1);
-        const int row = row0 + rr, t = row / p.group, h = kvh * p.group + row - t * p.group;
-        const float sum = red_l[rr];
-        const int64_t slot = ((int64_t)(sq.start + t) * p.n_heads + h) * p.nsplit + split;
-        const float inv = p.nsplit > 1 ? 1.f : (sum == 0.f ? 0.f : 1.f / sum);
-        char* dst = p.out + (int64_t)(sq.start + t) * p.out_st + h * p.out_sh;
-        float* part = p.part_acc + slot * p.hs;
-        if (p.nsplit > 1 && mine && col0 == 0) {
-          p.part_ml[slot * 2] = red_m[rr];
-          p.part_ml[slot * 2 + 1] = sum;
-        }
+              for (int h = 0; h < 2; ++h) {
+                mx[h] = fmaxf(mx[h], __shfl_xor_sync(0xffffffffu, mx[h], 1));
+                mx[h] = fmaxf(mx[h], __shfl_xor_sync(0xffffffffu, mx[h], 2));
+                float m_new = mx[h] > m_used[h] + TC_RESCALE ? mx[h] : m_used[h];
+                if (m_new == -INFINITY) m_new = 0.f;   // no key seen yet
+                f[h] = m_new != m_used[h] ? fast_exp2(m_used[h] - m_new) : 1.0f;
+                l[h] *= f[h];
+                m_used[h] = m_new;
+              }
+              if (j > 0) {
+                if constexpr (FEW) {   // P V(c - 1) may still be running; with one S tile it finished before S(c) did
+                  ok = __all_sync(0xffffffffu, mbar_wait(bar(TB_O), (uint32_t)((c - 1) & 1), status, 32, c));
+                  if (!ok) break;
+                  tc_fence_after();
+                }
 #pragma unroll
-        for (int c = 0; c < OC / 16; ++c) {
-          uint32_t o[16];
-          tmem_ld16(t_o + c * 16, o);
-          tmem_wait_ld();
-          if constexpr (ACT32)
+                for (int k = 0; k < (ACT32 ? 2 : 1) * (HDP / 16); ++k) {
+                  const uint32_t at = t_o + (k % (HDP / 16)) * 16 + (k >= HDP / 16 ? LO : 0u);
+                  uint32_t o[8];
+                  tmem_ldq256_x2(at, o);
+                  tmem_wait_ld();
 #pragma unroll
-            for (int i = 0; i < 16; ++i)
-              o[i] = __float_as_uint(__uint_as_float(o[i]) + __uint_as_float(__shfl_xor_sync(0xffffffffu, o[i], 16)));
-          const int col = col0 + c * 16;
-          if (!mine || col >= p.hs) continue;
-          if (ACT32 || p.nsplit > 1) {
-            float* f = p.nsplit > 1 ? part : reinterpret_cast<float*>(dst);
+                  for (int i = 0; i < 8; ++i) o[i] = __float_as_uint(__uint_as_float(o[i]) * f[(i >> 1) & 1]);
+                  tmem_stq256_x2(at, o);
+                }
+              }
+            }
+            // p = 2^(s scale - m), handed over in three pieces (64, 32, 32 keys); the sum is of the unrounded ones
+            const float2 nm2[2] = {make_float2(-m_used[0], -m_used[0]), make_float2(-m_used[1], -m_used[1])};
+            float2 rs[2] = {make_float2(0.f, 0.f), make_float2(0.f, 0.f)};
+            auto quarter = [&](const int q) {
+              uint32_t pk[8], pl[ACT32 ? 8 : 1];
 #pragma unroll
-            for (int i = 0; i < 16; i += 4)
-              *reinterpret_cast<float4*>(f + col + i) = make_float4(__uint_as_float(o[i]) * inv, __uint_as_float(o[i + 1]) * inv,
-                                                                    __uint_as_float(o[i + 2]) * inv, __uint_as_float(o[i + 3]) * inv);
-          } else {
+              for (int k = 4 * q; k < 4 * q + 4; ++k)
 #pragma unroll
-            for (int i = 0; i < 16; i += 8)
-              *reinterpret_cast<uint4*>(reinterpret_cast<__nv_bfloat16*>(dst) + col + i) =
-                  make_uint4(pack_bf16(__uint_as_float(o[i]) * inv, __uint_as_float(o[i + 1]) * inv), pack_bf16(__uint_as_float(o[i + 2]) * inv, __uint_as_float(o[i + 3]) * inv),
-                             pack_bf16(__uint_as_float(o[i + 4]) * inv, __uint_as_float(o[i + 5]) * inv), pack_bf16(__uint_as_float(o[i + 6]) * inv, __uint_as_float(o[i + 7]) * inv));
+                for (int h = 0; h < 2; ++h) {
+                  const float2 xx = ffma2(make_float2(__uint_as_float(s[4 * k + 2 * h]), __uint_as_float(s[4 * k + 2 * h + 1])), scale2, nm2[h]);
+                  const float p0 = fast_exp2(xx.x), p1 = fast_exp2(xx.y);
+                  const uint32_t pw = pack_bf16(p0, p1);
+                  pk[2 * (k & 3) + h] = pw;
+                  if constexpr (ACT32) pl[2 * (k & 3) + h] = pack_bf16(p0 - __uint_as_float(pw << 16), p1 - __uint_as_float(pw & 0xffff0000u));
+                  rs[h] = fadd2(rs[h], make_float2(p0, p1));
+                }
+              tmem_stq128_x4(t_s + 16 * q, pk);
+              if constexpr (ACT32) tmem_stq128_x4(t_s + LO + 16 * q, pl);
+            };
+            auto hand_over = [&](int b) {
+              tmem_wait_st();
+              tc_fence_before();
+              __syncwarp();
+              if (lane == 0) mbar_arrive(bar(b));
+            };
+            quarter(0);
+            quarter(1);
+            hand_over(TB_P1 + (FEW ? c & 1 : 0));
+            quarter(2);
+            hand_over(TB_P2 + (FEW ? c & 1 : 0));
+            quarter(3);
+            hand_over(TB_P3 + (FEW ? c & 1 : 0));
+            l[0] += rs[0].x + rs[0].y;
+            l[1] += rs[1].x + rs[1].y;
           }
+          if (ok) {
+#pragma unroll
+            for (int h = 0; h < 2; ++h) {
+              l[h] += __shfl_xor_sync(0xffffffffu, l[h], 1);
+              l[h] += __shfl_xor_sync(0xffffffffu, l[h], 2);
+            }
+            if (quad == 0) {
+              red_l[r0] = l[0]; red_l[r0 + 8] = l[1];
+              red_m[r0] = m_used[0]; red_m[r0 + 8] = m_used[1];
+            }
+            __syncwarp();
+            if (lane == 0) mbar_arrive(bar(TB_RED));
+          }
+        } else {
+          c += g.n;
+        }
+        // ---------------------------------------------------------------- epilogue: a lane a row, warps w and w + 4 half the columns each.  All eight wait for the
+        // item's last product: it has read the query tile and left O, which the next item's overwrite
+        if (ok) ok = __all_sync(0xffffffffu, mbar_wait(bar(TB_DONE), (uint32_t)(item & 1), status, 34, c));
+        if (ok) ok = __all_sync(0xffffffffu, mbar_wait(bar(TB_RED), (uint32_t)(item & 1), status, 36, c));
+        const int first_row = ACT32 ? (warp & 3) * 16 : (warp & 3) * 32;
+        if (ok && first_row < g.rows) {
+          tc_fence_after();
+          constexpr int OC = HDP / 2;
+          const int col0 = (warp >> 2) * OC;
+          const int r = ACT32 ? first_row + (lane & 15) : first_row + lane;
+          const uint32_t t_o = tmem_base + ((uint32_t)((warp & 3) * 32) << 16) + PL::O_COL + col0;
+          const bool mine = r < g.rows && (!ACT32 || lane < 16);
+          const int rr = min(r, g.rows - 1), t = rr / g.heads;
+          const float sum = red_l[rr];
+          const float inv = g.slot >= 0 ? 1.f : (sum == 0.f ? 0.f : 1.f / sum);
+          char* dst = p.out + (int64_t)(g.token0 + t) * p.out_st + (g.head0 + rr - t * g.heads) * p.out_sh;
+          const int64_t slot = (int64_t)g.slot * p.rows_max + rr;
+          if (g.slot >= 0 && mine && col0 == 0) {
+            p.part_ml[slot * 2] = red_m[rr];
+            p.part_ml[slot * 2 + 1] = sum;
+          }
+#pragma unroll
+          for (int k = 0; k < OC / 16; ++k) {
+            uint32_t o[16];
+            tmem_ld16(t_o + k * 16, o);
+            tmem_wait_ld();
+            if constexpr (ACT32)
+#pragma unroll
+              for (int i = 0; i < 16; ++i) o[i] = __float_as_uint(__uint_as_float(o[i]) + __uint_as_float(__shfl_xor_sync(0xffffffffu, o[i], 16)));
+            const int col = col0 + k * 16;
+            if (mine && col < p.hs) {
+              if (ACT32 || g.slot >= 0) {
+                float* f = g.slot < 0 ? reinterpret_cast<float*>(dst) : p.part_acc + slot * p.hs;
+#pragma unroll
+                for (int i = 0; i < 16; i += 4)
+                  *reinterpret_cast<float4*>(f + col + i) = make_float4(__uint_as_float(o[i]) * inv, __uint_as_float(o[i + 1]) * inv,
+                                                                        __uint_as_float(o[i + 2]) * inv, __uint_as_float(o[i + 3]) * inv);
+              } else {
+#pragma unroll
+                for (int i = 0; i < 16; i += 8)
+                  *reinterpret_cast<uint4*>(reinterpret_cast<__nv_bfloat16*>(dst) + col + i) =
+                      make_uint4(pack_bf16(__uint_as_float(o[i]) * inv, __uint_as_float(o[i + 1]) * inv), pack_bf16(__uint_as_float(o[i + 2]) * inv, __uint_as_float(o[i + 3]) * inv),
+                                 pack_bf16(__uint_as_float(o[i + 4]) * inv, __uint_as_float(o[i + 5]) * inv), pack_bf16(__uint_as_float(o[i + 6]) * inv, __uint_as_float(o[i + 7]) * inv));
+              }
+            }
+          }
+          tc_fence_before();   // O has been read before the query tile's barrier lets the next products start
         }
       }
+      if (!ok) break;
+      release_segment();
     }
   }
   tc_fence_before();
   __syncthreads();
   if (warp == TC_WARP_MMA) {
     tc_fence_after();
-    tmem_dealloc(tmem_base, TC_TMEM);
+    tmem_dealloc(tmem_base, PL::TMEM);
+  }
+}
+
+// Join of the items that several CTAs worked on: out = sum_s 2^(m_s - M) acc_s / sum_s 2^(m_s - M) l_s over their parts, in the order
+// of the CTAs.  Block x is the CTA where an item ended; a warp takes a row, a lane four elements.
+template <typename T>
+__global__ void __launch_bounds__(256) paged_join_kernel(const AttnArgs p) {
+  mca_pdl_launch_dependents();
+  mca_pdl_wait();
+  const int4 m0 = __ldcg(p.meta + 2 * blockIdx.x);
+  if (m0.x < 0) return;
+  const int heads = __ldcg(p.meta + 2 * blockIdx.x + 1).x;
+  const int first = m0.x, n = (int)blockIdx.x - first + 1, lane = threadIdx.x & 31;
+  const int step = p.hs / 4;
+  for (int r = blockIdx.y * 8 + (threadIdx.x >> 5); r < m0.w; r += gridDim.y * 8) {
+    auto slot = [&](int i) { return (2ll * (first + i) + (i == 0 ? 1 : 0)) * p.rows_max + r; };   // its last part, then their first ones
+    float M = -INFINITY;
+    for (int i = lane; i < n; i += 32) {
+      const float2 v = reinterpret_cast<const float2*>(p.part_ml)[slot(i)];
+      if (v.y != 0.f) M = fmaxf(M, v.x);
+    }
+#pragma unroll
+    for (int o = 16; o > 0; o >>= 1) M = fmaxf(M, __shfl_xor_sync(0xffffffffu, M, o));
+    float sum = 0.f;
+    float4 a = make_float4(0.f, 0.f, 0.f, 0.f);
+#pragma unroll 4
+    for (int i = 0; i < n; ++i) {
+      const float2 v = reinterpret_cast<const float2*>(p.part_ml)[slot(i)];
+      const float f = v.y == 0.f ? 0.f : fast_exp2(v.x - M);
+      sum = fmaf(v.y, f, sum);
+      if (lane < step) {
+        const float4 x = reinterpret_cast<const float4*>(p.part_acc + slot(i) * p.hs)[lane];
+        a.x = fmaf(x.x, f, a.x); a.y = fmaf(x.y, f, a.y); a.z = fmaf(x.z, f, a.z); a.w = fmaf(x.w, f, a.w);
+      }
+    }
+    if (lane < step) {
+      const float inv = sum == 0.f ? 0.f : 1.f / sum;
+      const int t = r / heads;
+      char* dst = p.out + (int64_t)(m0.y + t) * p.out_st + (m0.z + r - t * heads) * p.out_sh;
+      if constexpr (sizeof(T) == 4) reinterpret_cast<float4*>(dst)[lane] = make_float4(a.x * inv, a.y * inv, a.z * inv, a.w * inv);
+      else reinterpret_cast<uint2*>(dst)[lane] = make_uint2(pack_bf16(a.x * inv, a.y * inv), pack_bf16(a.z * inv, a.w * inv));
+    }
   }
 }
 
@@ -782,38 +1031,58 @@ __global__ void __launch_bounds__(TC_THREADS, 2) paged_tc_kernel(const __grid_co
 // Host
 // ---------------------------------------------------------------------------------------------------------------------
 struct Plan {
-  bool tc;
+  bool tc, few;
   int rows;       // query rows of a tile
-  int tiles, split_len, nsplit;
+  int tiles, split_len, nsplit;                             // fp32 kernel
+  int tile_shift, parts, ctas, least_units, rows_max;       // tensor-core kernel
+  bool join;
   int64_t bytes;  // of workspace
 };
 
-// Which kernel, and how the keys are split.
+// Which kernel, and how the keys are shared out.
 int make_plan(const McaPagedCache* c, const McaPagedBatch* b, int dtype, Plan* out) {
   const int group = c->n_heads / c->n_kv_heads;
   const int64_t most_rows = (int64_t)b->max_new * group;   // of one sequence and key/value head
   const bool act32 = dtype == MCA_DTYPE_F32;
+  *out = Plan{};
   out->tc = !act32 || (c->dtype == MCA_DTYPE_BF16 && most_rows > 4);
-  out->rows = out->tc ? (act32 ? 64 : 128) : (most_rows >= 4 ? 4 : (most_rows >= 2 ? 2 : 1));
+  if (out->tc) {
+    const int R = act32 ? 64 : 128;
+    out->rows = R;
+    // tokens of a tile: a power of two, for which a sequence's key tiles have a closed sum (a group of 3, 5 or 6 heads leaves a
+    // quarter or a third of the tile's rows empty)
+    while (group << (out->tile_shift + 1) <= R) ++out->tile_shift;
+    const int tile_tokens = 1 << out->tile_shift;
+    out->parts = mca_ceil_div(group, R);
+    out->few = b->max_new <= tile_tokens;
+    out->rows_max = std::min(tile_tokens, b->max_new) * std::min(group, R);
+    out->least_units = 2;
+    const int64_t tiles = out->few ? b->n_seqs : (int64_t)b->n_tokens / tile_tokens + b->n_seqs;
+    const double units = (double)tiles * out->parts * c->n_kv_heads * (b->max_len / KEYS + 1 + ITEM_UNITS);
+    out->ctas = (int)std::min((double)(out->few ? 148 : 296), std::max(1.0, std::ceil(units / out->least_units)));
+    out->join = b->max_len > KEYS && out->ctas > 1;   // an item of one key tile is one CTA's
+    out->bytes = out->join ? (int64_t)out->ctas * (2ll * out->rows_max * (c->head_size + 2) * 4 + 32) : 0;
+    return 0;
+  }
+  out->rows = most_rows >= 4 ? 4 : (most_rows >= 2 ? 2 : 1);
   const int64_t tiles = most_rows <= out->rows ? b->n_seqs : (int64_t)b->n_tokens * group / out->rows + b->n_seqs;
   if (tiles >= (1ll << 30)) return ERROR_PARAM_OUT_OF_RANGE;
   out->tiles = (int)tiles;
   const int64_t ctas = tiles * c->n_kv_heads;
-  const int slots = !out->tc && out->rows == 4 ? 148 : 296;
-  const int step = out->tc ? KEYS : 16, least = out->tc ? 2 * KEYS : 128;
+  const int slots = out->rows == 4 ? 148 : 296;
   // time in keys of one CTA: whole waves of (set-up + the keys of a split); more than one split also writes and joins partial results
-  const double setup = out->tc ? 512 : 64;
   const double part_keys = (double)b->n_tokens * c->n_heads * c->head_size * 8.0 / 5e6 * 128.0;   // 5 TB/s; 128 keys are about a microsecond
   double best = 1e300;
   int64_t len = 0;
-  for (int n = 1; n <= std::max(1, std::min(64, b->max_len / least)); ++n) {
-    const int64_t l = ((b->max_len + n - 1) / n + step - 1) / step * step;
-    const double cost = (double)((ctas * n + slots - 1) / slots) * (setup + (double)l) + (n > 1 ? 512 + n * part_keys : 0);
+  for (int n = 1; n <= std::max(1, std::min(64, b->max_len / 128)); ++n) {
+    const int64_t l = ((b->max_len + n - 1) / n + 15) / 16 * 16;
+    const double cost = (double)((ctas * n + slots - 1) / slots) * (64.0 + (double)l) + (n > 1 ? 512 + n * part_keys : 0);
     if (cost < best) { best = cost; len = l; }
   }
   out->split_len = (int)len;
   out->nsplit = (int)((b->max_len + len - 1) / len);
-  out->bytes = out->nsplit > 1 ? (int64_t)b->n_tokens * c->n_heads * out->nsplit * (c->head_size + 2) * 4 : 0;
+  out->join = out->nsplit > 1;
+  out->bytes = out->join ? (int64_t)b->n_tokens * c->n_heads * out->nsplit * (c->head_size + 2) * 4 : 0;
   return 0;
 }
 
@@ -828,14 +1097,18 @@ int page_map(CUtensorMap* map, const void* base, const McaPagedCache* c) {
   return r == CUDA_SUCCESS ? 0 : ERROR_PARAM_OUT_OF_RANGE;
 }
 
-template <int HDP, bool ACT32>
+template <int HDP, bool ACT32, bool FEW>
 int launch_tc(const McaPagedCache* c, const AttnArgs& a, cudaStream_t st) {
   CUtensorMap mk, mv;
   int e;
   if ((e = page_map(&mk, c->k_pages, c)) || (e = page_map(&mv, c->v_pages, c))) return e;
   static std::atomic<uint64_t> done{0};
-  if ((e = mca_smem_once(done, paged_tc_kernel<HDP, ACT32>, TcPlan<HDP>::BYTES))) return e;
-  return mca_launch_pdl(paged_tc_kernel<HDP, ACT32>, dim3(a.tiles + 1, a.n_kv, a.nsplit), dim3(TC_THREADS), TcPlan<HDP>::BYTES, st, mk, mv, a);
+  if ((e = mca_smem_once(done, paged_tc_kernel<HDP, ACT32, FEW>, TcPlan<HDP, FEW>::BYTES))) return e;
+  return mca_launch_pdl(paged_tc_kernel<HDP, ACT32, FEW>, dim3(a.ctas + 1), dim3(TC_THREADS), TcPlan<HDP, FEW>::BYTES, st, mk, mv, a);
+}
+template <bool ACT32, bool FEW>
+int launch_tc(const McaPagedCache* c, const AttnArgs& a, cudaStream_t st) {
+  return a.hs <= 64 ? launch_tc<64, ACT32, FEW>(c, a, st) : launch_tc<128, ACT32, FEW>(c, a, st);
 }
 template <typename CT, int HS>
 int launch_simt(int rows, const AttnArgs& a, cudaStream_t st) {
@@ -893,26 +1166,31 @@ int mca_paged_attention(const McaPagedCache* cache, const McaPagedBatch* batch, 
   a.n_heads = cache->n_heads; a.n_kv = cache->n_kv_heads; a.group = cache->n_heads / cache->n_kv_heads; a.hs = D;
   a.split_len = plan.split_len; a.nsplit = plan.nsplit; a.tiles = plan.tiles;
   a.scale_log2 = (scale == 0.f ? 1.0f / sqrtf((float)D) : scale) * LOG2E;
-  a.part_acc = static_cast<float*>(workspace);
-  a.part_ml = plan.nsplit > 1 ? a.part_acc + (int64_t)batch->n_tokens * cache->n_heads * plan.nsplit * D : nullptr;
+  a.tile_shift = plan.tile_shift; a.parts = plan.parts; a.items = plan.parts * cache->n_kv_heads;
+  a.ctas = plan.ctas; a.least_units = plan.least_units; a.warps = (plan.rows_max + 15) / 16; a.rows_max = plan.rows_max;
+  const int64_t slots = plan.tc ? 2ll * plan.ctas * plan.rows_max : (int64_t)batch->n_tokens * cache->n_heads * plan.nsplit;
+  a.part_acc = plan.join ? static_cast<float*>(workspace) : nullptr;
+  a.part_ml = plan.join ? a.part_acc + slots * D : nullptr;
+  a.meta = plan.join && plan.tc ? reinterpret_cast<int4*>(a.part_ml + slots * 2) : nullptr;
   cudaStream_t st = (cudaStream_t)stream;
+  const bool f32 = dtype == MCA_DTYPE_F32;
   if (plan.tc) {
-    if (dtype == MCA_DTYPE_F32) e = D <= 64 ? launch_tc<64, true>(cache, a, st) : launch_tc<128, true>(cache, a, st);
-    else e = D <= 64 ? launch_tc<64, false>(cache, a, st) : launch_tc<128, false>(cache, a, st);
-  } else {
-    switch (D) {
-#define MCA_PAGED_CASE(HS_) \
-      case HS_: e = csize == 2 ? launch_simt<__nv_bfloat16, HS_>(plan.rows, a, st) : launch_simt<float, HS_>(plan.rows, a, st); break;
-      MCA_PAGED_CASE(32) MCA_PAGED_CASE(48) MCA_PAGED_CASE(64) MCA_PAGED_CASE(96) MCA_PAGED_CASE(128)
-#undef MCA_PAGED_CASE
-      default: return ERROR_ATTN_UNSUPPORTED_SHAPE;
-    }
+    if (f32) e = plan.few ? launch_tc<true, true>(cache, a, st) : launch_tc<true, false>(cache, a, st);
+    else e = plan.few ? launch_tc<false, true>(cache, a, st) : launch_tc<false, false>(cache, a, st);
+    if (e || !plan.join) return e;
+    const dim3 grid(plan.ctas, std::min(4, mca_ceil_div(plan.rows_max, 8)));
+    return f32 ? mca_launch_pdl(paged_join_kernel<float>, grid, dim3(256), 0, st, a) : mca_launch_pdl(paged_join_kernel<__nv_bfloat16>, grid, dim3(256), 0, st, a);
   }
-  if (e || plan.nsplit == 1) return e;
-  const int64_t items = (int64_t)batch->n_tokens * cache->n_heads;
-  const dim3 grid((unsigned)((items + 3) / 4));
-  return dtype == MCA_DTYPE_F32 ? mca_launch_pdl(paged_join_kernel<float>, grid, dim3(128), 0, st, a)
-                                : mca_launch_pdl(paged_join_kernel<__nv_bfloat16>, grid, dim3(128), 0, st, a);
+  switch (D) {
+#define MCA_PAGED_CASE(HS_) \
+    case HS_: e = csize == 2 ? launch_simt<__nv_bfloat16, HS_>(plan.rows, a, st) : launch_simt<float, HS_>(plan.rows, a, st); break;
+    MCA_PAGED_CASE(32) MCA_PAGED_CASE(48) MCA_PAGED_CASE(64) MCA_PAGED_CASE(96) MCA_PAGED_CASE(128)
+#undef MCA_PAGED_CASE
+    default: return ERROR_ATTN_UNSUPPORTED_SHAPE;
+  }
+  if (e || !plan.join) return e;
+  const int64_t rows = (int64_t)batch->n_tokens * cache->n_heads;
+  return mca_launch_pdl(paged_simt_join_kernel, dim3((unsigned)((rows + 3) / 4)), dim3(128), 0, st, a);
 }
 
 int mca_paged_status(int* status4) {

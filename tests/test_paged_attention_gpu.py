@@ -176,3 +176,23 @@ def test_runs_alike():
         s.out.zero_()
         s.cache.attend(s.batch, s.q, s.out)
         assert torch.equal(first, s.out)
+
+
+@pytest.mark.parametrize("act,cache", TYPES)
+@pytest.mark.parametrize("hs", [64, 128])
+def test_many_key_tiles_for_each_block(act, cache, hs):
+    """Work enough that every block of the launch has several items, and items of many key tiles: single tokens."""
+    s = setup([(1, 100 + 531 * b % 4000) for b in range(24)], 16, 8, hs, 32, act, cache, seed=15, drop=[(3, 2), (7, 0)])
+    s.cache.attend(s.batch, s.q, s.out)
+    s.check()
+    assert s.cache.status() == (0, 0, 0, 0)
+
+
+@pytest.mark.parametrize("act,cache", TYPES)
+@pytest.mark.parametrize("hs", [64, 128])
+def test_many_key_tiles_for_each_block_of_chunks(act, cache, hs):
+    """The same for chunks of many tokens among single ones."""
+    s = setup([(300, 2000), (1, 1500), (129, 129), (1, 2900), (400, 420)], 16, 4, hs, 64, act, cache, seed=16)
+    s.cache.attend(s.batch, s.q, s.out)
+    s.check()
+    assert s.cache.status() == (0, 0, 0, 0)
