@@ -74,17 +74,21 @@ __device__ __forceinline__ bool find_tile(const Batch& t, int group, int R, int 
   return false;
 }
 
-// What one CTA more than the tiles does: reports the sequences that are refused and writes zeros over their rows.
+// What one CTA more than the work needs does: reports the sequences that are refused and writes zeros over their rows.
 template <typename T> __device__ void look_over(const AttnArgs& p) {
-  for (int b = 0; b < p.batch.n_seqs; ++b) {
-    const Sequence s = paged::sequence(p.batch, b);
-    if (s.good) continue;
-    if (threadIdx.x == 0) paged::refuse(paged::REFUSED_LENGTHS, b, s.length);
-    const int lo = max(s.start, 0), hi = min(p.batch.starts[b + 1], p.batch.n_tokens);
-    const int64_t n = (int64_t)max(hi - lo, 0) * p.n_heads * p.hs;
-    for (int64_t i = threadIdx.x; i < n; i += blockDim.x) {
-      const int e = (int)(i % p.hs), h = (int)(i / p.hs % p.n_heads), t = lo + (int)(i / p.hs / p.n_heads);
-      reinterpret_cast<T*>(p.out + t * p.out_st + h * p.out_sh)[e] = T(0.f);
+  for (int b0 = 0; b0 < p.batch.n_seqs; b0 += blockDim.x) {
+    const int mine = b0 + threadIdx.x;
+    const bool bad = mine < p.batch.n_seqs && !paged::sequence(p.batch, mine).good;
+    if (bad) paged::refuse(paged::REFUSED_LENGTHS, mine, p.batch.lengths[mine]);
+    if (!__syncthreads_or(bad)) continue;
+    for (int b = b0; b < min(b0 + (int)blockDim.x, p.batch.n_seqs); ++b) {
+      if (paged::sequence(p.batch, b).good) continue;
+      const int lo = max(p.batch.starts[b], 0), hi = min(p.batch.starts[b + 1], p.batch.n_tokens);
+      const int64_t n = (int64_t)max(hi - lo, 0) * p.n_heads * p.hs;
+      for (int64_t i = threadIdx.x; i < n; i += blockDim.x) {
+        const int e = (int)(i % p.hs), h = (int)(i / p.hs % p.n_heads), t = lo + (int)(i / p.hs / p.n_heads);
+        reinterpret_cast<T*>(p.out + t * p.out_st + h * p.out_sh)[e] = T(0.f);
+      }
     }
   }
 }
@@ -728,34 +732,40 @@ __global__ void __launch_bounds__(TC_THREADS, (TcPlan<HDP, FEW>::CTAS)) paged_tc
       const Segment& g = *gp;
       {
         // ---------------------------------------------------------------- the query tile, 16-byte pieces in the swizzled layout
-        for (int i = tid; i < g.rows * CH; i += 256) {
-          const int r = i / CH, ch = i - r * CH;
-          const int t = r / g.heads;
-          const char* src = p.q + (int64_t)(g.token0 + t) * p.q_st + (g.head0 + r - t * g.heads) * p.q_sh;
-          const bool in = ch * 8 < p.hs;
-          const uint32_t sub = PL::OFF_Q + (uint32_t)(ch >> 3) * PL::SUB_BYTES;
-          if constexpr (ACT32) {
-            float x[8];
+        constexpr int QN = R * CH / 256;       // pieces of a thread: eight elements each; their loads go out together
+        uint4 raw[QN][ACT32 ? 2 : 1];
 #pragma unroll
-            for (int k = 0; k < 8; ++k) x[k] = 0.f;
-            if (in) {
-              const float4 a = mca_ld_f4(reinterpret_cast<const float*>(src) + ch * 8), b = mca_ld_f4(reinterpret_cast<const float*>(src) + ch * 8 + 4);
-              x[0] = a.x; x[1] = a.y; x[2] = a.z; x[3] = a.w; x[4] = b.x; x[5] = b.y; x[6] = b.z; x[7] = b.w;
-            }
+        for (int i = 0; i < QN; ++i) {
+          const int r = (i * 256 + tid) / CH, ch = tid % CH;
+#pragma unroll
+          for (int k = 0; k < (ACT32 ? 2 : 1); ++k) raw[i][k] = make_uint4(0, 0, 0, 0);
+          if (r < g.rows && ch * 8 < p.hs) {
+            const int t = r / g.heads;
+            const uint4* src = reinterpret_cast<const uint4*>(p.q + (int64_t)(g.token0 + t) * p.q_st + (g.head0 + r - t * g.heads) * p.q_sh);
+#pragma unroll
+            for (int k = 0; k < (ACT32 ? 2 : 1); ++k) raw[i][k] = src[ch * (ACT32 ? 2 : 1) + k];
+          }
+        }
+#pragma unroll
+        for (int i = 0; i < QN; ++i) {
+          const int r = (i * 256 + tid) / CH, ch = tid % CH;
+          const uint32_t sub = PL::OFF_Q + (uint32_t)(ch >> 3) * PL::SUB_BYTES;
+          if (r >= g.rows) continue;
+          if constexpr (ACT32) {
+            const uint32_t* x = reinterpret_cast<const uint32_t*>(raw[i]);
             uint32_t hi[4], lo[4];
 #pragma unroll
             for (int k = 0; k < 4; ++k) {
-              hi[k] = pack_bf16(x[2 * k], x[2 * k + 1]);
-              lo[k] = pack_bf16(x[2 * k] - __uint_as_float(hi[k] << 16), x[2 * k + 1] - __uint_as_float(hi[k] & 0xffff0000u));
+              const float a = __uint_as_float(x[2 * k]), b = __uint_as_float(x[2 * k + 1]);
+              hi[k] = pack_bf16(a, b);
+              lo[k] = pack_bf16(a - __uint_as_float(hi[k] << 16), b - __uint_as_float(hi[k] & 0xffff0000u));
             }
             const int r_hi = (r >> 4) * 32 + (r & 15);
             const uint32_t at = sub + (uint32_t)(r_hi * 128 + (((ch & 7) ^ (r_hi & 7)) << 4));
             *reinterpret_cast<uint4*>(smem + at) = make_uint4(hi[0], hi[1], hi[2], hi[3]);
             *reinterpret_cast<uint4*>(smem + at + 16 * 128) = make_uint4(lo[0], lo[1], lo[2], lo[3]);   // 16 rows on: the same swizzle
           } else {
-            uint4 v = make_uint4(0, 0, 0, 0);
-            if (in) v = *(reinterpret_cast<const uint4*>(src) + ch);
-            *reinterpret_cast<uint4*>(smem + sub + (uint32_t)(r * 128 + (((ch & 7) ^ (r & 7)) << 4))) = v;
+            *reinterpret_cast<uint4*>(smem + sub + (uint32_t)(r * 128 + (((ch & 7) ^ (r & 7)) << 4))) = raw[i][0];
           }
         }
         asm volatile("fence.proxy.async.shared::cta;" ::: "memory");

@@ -57,16 +57,16 @@ def _dtype(t, what):
 
 def _heads(t, what, shape, dtype, device):
     """A (..., heads, head_size) tensor as the C side sees it; rows of heads are read where they lie."""
-    if t.dtype != dtype or t.device != device or tuple(t.shape) != shape:
-        raise ValueError(f"{what}: {shape} of {dtype} on {device} is wanted, got {tuple(t.shape)} of {t.dtype} on {t.device}")
     s = t.stride()
+    if t.shape != shape or t.dtype is not dtype or t.device != device:
+        raise ValueError(f"{what}: {tuple(shape)} of {dtype} on {device} is wanted, got {tuple(t.shape)} of {t.dtype} on {t.device}")
     if s[-1] != 1:
         raise ValueError(f"{what}: a head's elements have to be contiguous")
     return McaHeads(t.data_ptr(), s[0] if len(s) == 4 else 0, s[-3], s[-2])
 
 
 def _indices(t, what, shape, device):
-    if t.dtype != torch.int32 or t.device != device or not t.is_contiguous() or tuple(t.shape) != shape:
+    if t.dtype is not torch.int32 or t.shape != shape or t.device != device or not t.is_contiguous():
         raise ValueError(f"{what}: contiguous int32 of shape {shape} on {device} is wanted")
     return t.data_ptr()
 
@@ -79,12 +79,20 @@ def _vector(t, what, size, device):
     return t.data_ptr()
 
 
-def _on(device, call):
-    """``call(stream)`` with the device current, on its current stream."""
-    if torch.cuda.current_device() == device.index:
-        return call(torch.cuda.current_stream(device).cuda_stream)
-    with torch.cuda.device(device):
-        return call(torch.cuda.current_stream(device).cuda_stream)
+# the current stream's handle; without building a Stream object where torch offers that
+_stream_handle = getattr(torch._C, "_cuda_getCurrentRawStream", None) or (lambda index: torch.cuda.current_stream(index).cuda_stream)
+
+
+def _call(device, name, function, *args):
+    """``function(*args, stream)`` with the device current, on its current stream."""
+    index = device.index
+    if torch.cuda.current_device() == index:
+        rc = function(*args, _stream_handle(index))
+    else:
+        with torch.cuda.device(device):
+            rc = function(*args, _stream_handle(index))
+    if rc:
+        raise PagedError(rc, name)
 
 
 class QkNormRope:
@@ -140,10 +148,8 @@ class QkNormRope:
         dev, qs, ks = q.device, (B, T, H, D), (B, T, KV, D)
         a = [_heads(q, "q", qs, q.dtype, dev), _heads(q_out, "q_out", qs, q.dtype, dev)]
         b = [None, None] if k is None else [C.byref(_heads(k, "k", ks, q.dtype, dev)), C.byref(_heads(k_out, "k_out", ks, q.dtype, dev))]
-        rc = _on(dev, lambda st: self._lib.mca_qk_norm_rope_forward(C.byref(self.c), C.byref(a[0]), b[0], pos, dt, B, T, H, KV, D,
-                                                                    C.byref(a[1]), b[1], st))
-        if rc:
-            raise PagedError(rc, "mca_qk_norm_rope_forward")
+        _call(dev, "mca_qk_norm_rope_forward", self._lib.mca_qk_norm_rope_forward, C.byref(self.c), C.byref(a[0]), b[0], pos, dt, B, T, H, KV, D,
+              C.byref(a[1]), b[1])
 
     def backward(self, q, k, dq_out, dk_out, dq, dk, positions=None, weight_grads=True):
         """From the forward's inputs and the gradients of its outputs: fills dq, dk and returns (dq_weight, dk_weight), float32,
@@ -157,11 +163,8 @@ class QkNormRope:
         need = self._lib.mca_qk_norm_rope_backward_scratch_floats(D) if any(want) else 0
         scratch = torch.empty(need, device=dev) if need > 0 else None
         ptr = [None if t is None else t.data_ptr() for t in dw]
-        rc = _on(dev, lambda st: self._lib.mca_qk_norm_rope_backward(
-            C.byref(self.c), a[0], b[0], pos, a[1], b[1], dt, B, T, H, KV, D, a[2], b[2], ptr[0], ptr[1],
-            None if scratch is None else scratch.data_ptr(), max(need, 0), st))
-        if rc:
-            raise PagedError(rc, "mca_qk_norm_rope_backward")
+        _call(dev, "mca_qk_norm_rope_backward", self._lib.mca_qk_norm_rope_backward, C.byref(self.c), a[0], b[0], pos, a[1], b[1], dt, B, T, H,
+              KV, D, a[2], b[2], ptr[0], ptr[1], None if scratch is None else scratch.data_ptr(), max(need, 0))
         return tuple(dw)
 
 
@@ -169,7 +172,7 @@ class PagedBatch:
     """A step's new tokens (see ``PagedCache.batch``)."""
 
     def __init__(self, c, n_tokens, keep):
-        self.c, self.n_tokens, self._keep = c, n_tokens, keep
+        self.c, self.ref, self.n_tokens, self._keep = c, C.byref(c), n_tokens, keep
 
 
 class PagedCache:
@@ -186,17 +189,17 @@ class PagedCache:
         self._keep = (k_pages, v_pages)
         self.device, self.n_heads, self.kv_heads, self.head_size, self.page_size = k_pages.device, int(n_heads), kv, hs, page
         self.c = McaPagedCache(k_pages.data_ptr(), v_pages.data_ptr(), k_pages.stride(0), n_pages, page, self.n_heads, kv, hs, _dtype(k_pages, "k_pages"))
+        self._ref = C.byref(self.c)
 
     def batch(self, starts, lengths, page_table, n_tokens, max_new, max_len):
         """The new tokens of sequence b are rows [starts[b], starts[b + 1]) of the token tensors and the last of its lengths[b]
         positions; page_table[b, i] is the page of positions [i page_size, (i + 1) page_size), -1 where it is not held.  All int32 on
         the device.  n_tokens: rows of the token tensors; max_new, max_len: upper bounds of the new tokens and of the positions of a
         sequence."""
-        n = lengths.shape[0]
-        c = McaPagedBatch(_indices(starts, "starts", (n + 1,), self.device), _indices(lengths, "lengths", (n,), self.device),
-                          _indices(page_table, "page_table", (n, page_table.shape[-1]), self.device), page_table.shape[-1], n, int(n_tokens),
-                          int(max_new), int(max_len))
-        return PagedBatch(c, int(n_tokens), (starts, lengths, page_table))
+        n, stride, dev = lengths.shape[0], page_table.shape[-1], self.device
+        c = McaPagedBatch(_indices(starts, "starts", (n + 1,), dev), _indices(lengths, "lengths", (n,), dev),
+                          _indices(page_table, "page_table", (n, stride), dev), stride, n, n_tokens, max_new, max_len)
+        return PagedBatch(c, n_tokens, (starts, lengths, page_table))
 
     def append(self, batch, rotation, q, k, v, q_out):
         """Norm and rotation of the new tokens' q into q_out and of k into the pages; v into its pages.  q, q_out (n_tokens, heads,
@@ -206,10 +209,8 @@ class PagedCache:
         dt, qs, ks = _dtype(q, "q"), (n, self.n_heads, self.head_size), (n, self.kv_heads, self.head_size)
         a = (_heads(q, "q", qs, q.dtype, dev), _heads(k, "k", ks, q.dtype, dev), _heads(v, "v", ks, q.dtype, dev),
              _heads(q_out, "q_out", qs, q.dtype, dev))
-        rc = _on(dev, lambda st: self._lib.mca_paged_append(C.byref(self.c), C.byref(batch.c), C.byref(rotation.c), dt, C.byref(a[0]),
-                                                            C.byref(a[1]), C.byref(a[2]), C.byref(a[3]), st))
-        if rc:
-            raise PagedError(rc, "mca_paged_append")
+        _call(dev, "mca_paged_append", self._lib.mca_paged_append, self._ref, batch.ref, C.byref(rotation.c), dt, C.byref(a[0]), C.byref(a[1]),
+              C.byref(a[2]), C.byref(a[3]))
 
     def attend(self, batch, q, out, scale=None):
         """out = attention of the new tokens' q over their sequences' pages (their own keys among them); both (n_tokens, heads,
@@ -217,20 +218,19 @@ class PagedCache:
         dev, shape = self.device, (batch.n_tokens, self.n_heads, self.head_size)
         dt = _dtype(q, "q")
         a, o = _heads(q, "q", shape, q.dtype, dev), _heads(out, "out", shape, q.dtype, dev)
-        need = self._lib.mca_paged_attention_workspace_bytes(C.byref(self.c), C.byref(batch.c), dt)
+        need = self._lib.mca_paged_attention_workspace_bytes(self._ref, batch.ref, dt)
         # of the current stream's allocator (or a captured graph's own pool): no two calls that overlap share it
         work = torch.empty(need, dtype=torch.uint8, device=dev) if need > 0 else None
-        rc = _on(dev, lambda st: self._lib.mca_paged_attention(C.byref(self.c), C.byref(batch.c), dt, C.byref(a), scale or 0.0, C.byref(o),
-                                                               None if work is None else work.data_ptr(), max(need, 0), st))
-        if rc:
-            raise PagedError(rc, "mca_paged_attention")
+        _call(dev, "mca_paged_attention", self._lib.mca_paged_attention, self._ref, batch.ref, dt, C.byref(a), scale or 0.0, C.byref(o),
+              None if work is None else work.data_ptr(), max(need, 0))
 
     def status(self):
         """What the calls on this device refused since the last time this was asked: (kind, detail, detail, how many), all zero if
         nothing.  Waits for the device."""
         torch.cuda.synchronize(self.device)
         st = (C.c_int * 4)()
-        rc = _on(self.device, lambda _: self._lib.mca_paged_status(st))
+        with torch.cuda.device(self.device):
+            rc = self._lib.mca_paged_status(st)
         if rc:
             raise PagedError(rc, "mca_paged_status")
         return tuple(st)
