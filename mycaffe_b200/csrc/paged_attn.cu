@@ -34,8 +34,8 @@ struct AttnArgs {
   int n_heads, n_kv, group, hs;
   int split_len, nsplit, tiles;
   float scale_log2;         // scale x log2(e): the softmax runs on powers of two
-  float* part_acc;          // partial results: fp32 kernel (n_tokens, n_heads, nsplit, hs), tensor-core kernel (ctas, 2, rows_max, hs)
-  float* part_ml;           // the same with 2 in place of hs: reference point (log2), sum
+  float* part_acc;          // partial results: fp32 kernel (n_tokens, n_heads, nsplit, hs), tensor-core kernel (ctas, 2, hs / 4, rows_max, 4)
+  float* part_ml;           // (n_tokens, n_heads, nsplit, 2) and (ctas, 2, rows_max, 2): reference point (log2), sum
   // tensor-core kernel
   int tile_shift, parts, items;    // log2 of the tokens of a tile; tiles that share a token's group of heads; parts x key/value heads
   int ctas, least_units, warps, rows_max;
@@ -728,24 +728,30 @@ __global__ void __launch_bounds__(TC_THREADS, (TcPlan<HDP, FEW>::CTAS)) paged_tc
     float* red_m = red_l + 128;
     const float scale = p.scale_log2;
     const float2 scale2 = make_float2(scale, scale);
-    while (const Segment* gp = next_segment(18)) {
+    constexpr int QN = R * CH / 256, QV = ACT32 ? 2 : 1;   // pieces of the query tile of a thread: eight elements, QV vectors each
+    uint4 raw[QN][QV];
+    auto load_query = [&](const Segment& g) {   // all loads go out together
+#pragma unroll
+      for (int i = 0; i < QN; ++i) {
+        const int r = (i * 256 + tid) / CH, ch = tid % CH;
+#pragma unroll
+        for (int k = 0; k < QV; ++k) raw[i][k] = make_uint4(0, 0, 0, 0);
+        if (r < g.rows && ch * 8 < p.hs) {
+          const int t = r / g.heads;
+          const uint4* src = reinterpret_cast<const uint4*>(p.q + (int64_t)(g.token0 + t) * p.q_st + (g.head0 + r - t * g.heads) * p.q_sh);
+#pragma unroll
+          for (int k = 0; k < QV; ++k) raw[i][k] = src[ch * QV + k];
+        }
+      }
+    };
+    const Segment* gp = next_segment(18);
+    if (FEW && gp != nullptr) load_query(*gp);
+    while (gp != nullptr) {
       const Segment& g = *gp;
+      const Segment* gn = nullptr;   // the part after it
       {
         // ---------------------------------------------------------------- the query tile, 16-byte pieces in the swizzled layout
-        constexpr int QN = R * CH / 256;       // pieces of a thread: eight elements each; their loads go out together
-        uint4 raw[QN][ACT32 ? 2 : 1];
-#pragma unroll
-        for (int i = 0; i < QN; ++i) {
-          const int r = (i * 256 + tid) / CH, ch = tid % CH;
-#pragma unroll
-          for (int k = 0; k < (ACT32 ? 2 : 1); ++k) raw[i][k] = make_uint4(0, 0, 0, 0);
-          if (r < g.rows && ch * 8 < p.hs) {
-            const int t = r / g.heads;
-            const uint4* src = reinterpret_cast<const uint4*>(p.q + (int64_t)(g.token0 + t) * p.q_st + (g.head0 + r - t * g.heads) * p.q_sh);
-#pragma unroll
-            for (int k = 0; k < (ACT32 ? 2 : 1); ++k) raw[i][k] = src[ch * (ACT32 ? 2 : 1) + k];
-          }
-        }
+        if (!FEW) load_query(g);   // no registers to hold them from before the last part's end
 #pragma unroll
         for (int i = 0; i < QN; ++i) {
           const int r = (i * 256 + tid) / CH, ch = tid % CH;
@@ -936,6 +942,13 @@ __global__ void __launch_bounds__(TC_THREADS, (TcPlan<HDP, FEW>::CTAS)) paged_tc
         }
         // ---------------------------------------------------------------- epilogue: a lane a row, warps w and w + 4 half the columns each.  All eight wait for the
         // item's last product: it has read the query tile and left O, which the next item's overwrite
+        const int at = item;
+        if (ok) {   // the next part's query rows are asked for meanwhile
+          ++item;
+          gn = next_segment(17);
+          if (FEW && gn != nullptr) load_query(*gn);
+          item = at;
+        }
         if (ok) ok = __all_sync(0xffffffffu, mbar_wait(bar(TB_DONE), (uint32_t)(item & 1), status, 34, c));
         if (ok) ok = __all_sync(0xffffffffu, mbar_wait(bar(TB_RED), (uint32_t)(item & 1), status, 36, c));
         const int first_row = ACT32 ? (warp & 3) * 16 : (warp & 3) * 32;
@@ -948,7 +961,7 @@ __global__ void __launch_bounds__(TC_THREADS, (TcPlan<HDP, FEW>::CTAS)) paged_tc
           const bool mine = r < g.rows && (!ACT32 || lane < 16);
           const int rr = min(r, g.rows - 1), t = rr / g.heads;
           const float sum = red_l[rr];
-          const float inv = g.slot >= 0 ? 1.f : (sum == 0.f ? 0.f : 1.f / sum);
+          const float inv = sum == 0.f ? 0.f : 1.f / sum;
           char* dst = p.out + (int64_t)(g.token0 + t) * p.out_st + (g.head0 + rr - t * g.heads) * p.out_sh;
           const int64_t slot = (int64_t)g.slot * p.rows_max + rr;
           if (g.slot >= 0 && mine && col0 == 0) {
@@ -965,12 +978,16 @@ __global__ void __launch_bounds__(TC_THREADS, (TcPlan<HDP, FEW>::CTAS)) paged_tc
               for (int i = 0; i < 16; ++i) o[i] = __float_as_uint(__uint_as_float(o[i]) + __uint_as_float(__shfl_xor_sync(0xffffffffu, o[i], 16)));
             const int col = col0 + k * 16;
             if (mine && col < p.hs) {
-              if (ACT32 || g.slot >= 0) {
-                float* f = g.slot < 0 ? reinterpret_cast<float*>(dst) : p.part_acc + slot * p.hs;
+              if (g.slot >= 0) {   // the lanes' rows side by side
+                float4* f = reinterpret_cast<float4*>(p.part_acc) + ((int64_t)g.slot * (p.hs / 4) + col / 4) * p.rows_max + rr;
+#pragma unroll
+                for (int i = 0; i < 4; ++i)
+                  f[(int64_t)i * p.rows_max] = make_float4(__uint_as_float(o[4 * i]), __uint_as_float(o[4 * i + 1]), __uint_as_float(o[4 * i + 2]), __uint_as_float(o[4 * i + 3]));
+              } else if constexpr (ACT32) {
 #pragma unroll
                 for (int i = 0; i < 16; i += 4)
-                  *reinterpret_cast<float4*>(f + col + i) = make_float4(__uint_as_float(o[i]) * inv, __uint_as_float(o[i + 1]) * inv,
-                                                                        __uint_as_float(o[i + 2]) * inv, __uint_as_float(o[i + 3]) * inv);
+                  *reinterpret_cast<float4*>(reinterpret_cast<float*>(dst) + col + i) = make_float4(
+                      __uint_as_float(o[i]) * inv, __uint_as_float(o[i + 1]) * inv, __uint_as_float(o[i + 2]) * inv, __uint_as_float(o[i + 3]) * inv);
               } else {
 #pragma unroll
                 for (int i = 0; i < 16; i += 8)
@@ -985,6 +1002,7 @@ __global__ void __launch_bounds__(TC_THREADS, (TcPlan<HDP, FEW>::CTAS)) paged_tc
       }
       if (!ok) break;
       release_segment();
+      gp = gn;
     }
   }
   tc_fence_before();
@@ -996,44 +1014,42 @@ __global__ void __launch_bounds__(TC_THREADS, (TcPlan<HDP, FEW>::CTAS)) paged_tc
 }
 
 // Join of the items that several CTAs worked on: out = sum_s 2^(m_s - M) acc_s / sum_s 2^(m_s - M) l_s over their parts, in the order
-// of the CTAs.  Block x is the CTA where an item ended; a warp takes a row, a lane four elements.
+// of the CTAs.  Block x is the CTA where an item ended; a thread takes four elements of a row, the lanes of a warp neighbouring rows,
+// as the parts lie.
 template <typename T>
 __global__ void __launch_bounds__(256) paged_join_kernel(const AttnArgs p) {
   mca_pdl_launch_dependents();
   mca_pdl_wait();
   const int4 m0 = __ldcg(p.meta + 2 * blockIdx.x);
-  if (m0.x < 0) return;
   const int heads = __ldcg(p.meta + 2 * blockIdx.x + 1).x;
-  const int first = m0.x, n = (int)blockIdx.x - first + 1, lane = threadIdx.x & 31;
-  const int step = p.hs / 4;
-  for (int r = blockIdx.y * 8 + (threadIdx.x >> 5); r < m0.w; r += gridDim.y * 8) {
-    auto slot = [&](int i) { return (2ll * (first + i) + (i == 0 ? 1 : 0)) * p.rows_max + r; };   // its last part, then their first ones
+  if (m0.x < 0) return;
+  const int first = m0.x, n = (int)blockIdx.x - first + 1, rows = m0.w, quads = p.hs / 4;
+  const float2* ml = reinterpret_cast<const float2*>(p.part_ml);
+  const float4* acc = reinterpret_cast<const float4*>(p.part_acc);
+  for (int i = blockIdx.y * 256 + threadIdx.x; i < rows * quads; i += gridDim.y * 256) {
+    const int col = i / rows, r = i - col * rows;
+    auto slot = [&](int k) { return 2ll * (first + k) + (k == 0 ? 1 : 0); };   // the first CTA's last part, then the others' first ones
     float M = -INFINITY;
-    for (int i = lane; i < n; i += 32) {
-      const float2 v = reinterpret_cast<const float2*>(p.part_ml)[slot(i)];
+#pragma unroll 4
+    for (int k = 0; k < n; ++k) {
+      const float2 v = ml[slot(k) * p.rows_max + r];
       if (v.y != 0.f) M = fmaxf(M, v.x);
     }
-#pragma unroll
-    for (int o = 16; o > 0; o >>= 1) M = fmaxf(M, __shfl_xor_sync(0xffffffffu, M, o));
     float sum = 0.f;
     float4 a = make_float4(0.f, 0.f, 0.f, 0.f);
 #pragma unroll 4
-    for (int i = 0; i < n; ++i) {
-      const float2 v = reinterpret_cast<const float2*>(p.part_ml)[slot(i)];
+    for (int k = 0; k < n; ++k) {
+      const float2 v = ml[slot(k) * p.rows_max + r];
+      const float4 x = acc[(slot(k) * quads + col) * p.rows_max + r];
       const float f = v.y == 0.f ? 0.f : fast_exp2(v.x - M);
       sum = fmaf(v.y, f, sum);
-      if (lane < step) {
-        const float4 x = reinterpret_cast<const float4*>(p.part_acc + slot(i) * p.hs)[lane];
-        a.x = fmaf(x.x, f, a.x); a.y = fmaf(x.y, f, a.y); a.z = fmaf(x.z, f, a.z); a.w = fmaf(x.w, f, a.w);
-      }
+      a.x = fmaf(x.x, f, a.x); a.y = fmaf(x.y, f, a.y); a.z = fmaf(x.z, f, a.z); a.w = fmaf(x.w, f, a.w);
     }
-    if (lane < step) {
-      const float inv = sum == 0.f ? 0.f : 1.f / sum;
-      const int t = r / heads;
-      char* dst = p.out + (int64_t)(m0.y + t) * p.out_st + (m0.z + r - t * heads) * p.out_sh;
-      if constexpr (sizeof(T) == 4) reinterpret_cast<float4*>(dst)[lane] = make_float4(a.x * inv, a.y * inv, a.z * inv, a.w * inv);
-      else reinterpret_cast<uint2*>(dst)[lane] = make_uint2(pack_bf16(a.x * inv, a.y * inv), pack_bf16(a.z * inv, a.w * inv));
-    }
+    const float inv = sum == 0.f ? 0.f : 1.f / sum;
+    const int t = r / heads;
+    char* dst = p.out + (int64_t)(m0.y + t) * p.out_st + (m0.z + r - t * heads) * p.out_sh;
+    if constexpr (sizeof(T) == 4) reinterpret_cast<float4*>(dst)[col] = make_float4(a.x * inv, a.y * inv, a.z * inv, a.w * inv);
+    else reinterpret_cast<uint2*>(dst)[col] = make_uint2(pack_bf16(a.x * inv, a.y * inv), pack_bf16(a.z * inv, a.w * inv));
   }
 }
 
@@ -1188,7 +1204,7 @@ int mca_paged_attention(const McaPagedCache* cache, const McaPagedBatch* batch, 
     if (f32) e = plan.few ? launch_tc<true, true>(cache, a, st) : launch_tc<true, false>(cache, a, st);
     else e = plan.few ? launch_tc<false, true>(cache, a, st) : launch_tc<false, false>(cache, a, st);
     if (e || !plan.join) return e;
-    const dim3 grid(plan.ctas, std::min(4, mca_ceil_div(plan.rows_max, 8)));
+    const dim3 grid(plan.ctas, std::min(8, mca_ceil_div(plan.rows_max * D / 4, 512)));   // two pieces a thread
     return f32 ? mca_launch_pdl(paged_join_kernel<float>, grid, dim3(256), 0, st, a) : mca_launch_pdl(paged_join_kernel<__nv_bfloat16>, grid, dim3(256), 0, st, a);
   }
   switch (D) {
