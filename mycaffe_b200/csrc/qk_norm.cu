@@ -20,6 +20,9 @@ using paged::Batch;
 constexpr int THREADS = 256;
 constexpr int HEADS = 4;       // of one token that a group takes at once, forward
 constexpr int HEADS_BWD = 2;   // backward: two tensors to load
+// CTAs per SM that registers are left for: fp32 rows are four elements a piece and fit in 80, bf16 ones are eight; with 80 they spill
+// (2 x 4095 x (32 + 8) heads of 128, forward and backward: 91 us with two CTAs, 160 with three; fp32, 8 x 1024 x 24 of 64: 52 and 48).
+template <typename T> constexpr int CTAS = sizeof(T) == 4 ? 3 : 2;
 constexpr int BWD_CTAS = 148 * 4;
 
 template <typename T> struct Piece;   // 16 bytes of a row
@@ -71,6 +74,35 @@ __device__ __forceinline__ void store_part(__nv_bfloat16* row, int gl, int half,
   }
 }
 
+// Two elements an instruction.
+__device__ __forceinline__ float2 mul2(float2 a, float2 b) {
+  uint64_t d;
+  asm("mul.rn.f32x2 %0, %1, %2;" : "=l"(d) : "l"(*reinterpret_cast<uint64_t*>(&a)), "l"(*reinterpret_cast<uint64_t*>(&b)));
+  return *reinterpret_cast<float2*>(&d);
+}
+__device__ __forceinline__ float2 fma2(float2 a, float2 b, float2 c) {
+  uint64_t d;
+  asm("fma.rn.f32x2 %0, %1, %2, %3;"
+      : "=l"(d) : "l"(*reinterpret_cast<uint64_t*>(&a)), "l"(*reinterpret_cast<uint64_t*>(&b)), "l"(*reinterpret_cast<uint64_t*>(&c)));
+  return *reinterpret_cast<float2*>(&d);
+}
+template <int VEC> __device__ __forceinline__ float2 two(const Part<VEC>& x, int i) { return make_float2(x.v[2 * i], x.v[2 * i + 1]); }
+template <int VEC> __device__ __forceinline__ void put(Part<VEC>& x, int i, float2 t) { x.v[2 * i] = t.x; x.v[2 * i + 1] = t.y; }
+template <int VEC> __device__ __forceinline__ float dot(const Part<VEC>& a, const Part<VEC>& b) {
+  float2 s = make_float2(0.f, 0.f);
+#pragma unroll
+  for (int i = 0; i < VEC; ++i) s = fma2(two(a, i), two(b, i), s);
+  return s.x + s.y;
+}
+template <int VEC> __device__ __forceinline__ void times(Part<VEC>& a, const Part<VEC>& b) {
+#pragma unroll
+  for (int i = 0; i < VEC; ++i) put(a, i, mul2(two(a, i), two(b, i)));
+}
+template <int VEC> __device__ __forceinline__ void times(Part<VEC>& a, float f) {
+#pragma unroll
+  for (int i = 0; i < VEC; ++i) put(a, i, mul2(two(a, i), make_float2(f, f)));
+}
+
 // Floats of a (D)-vector (a weight) at the places of a lane's part.
 template <int VEC>
 __device__ __forceinline__ void load_weight(const float* w, int gl, int half, Part<VEC>& x) {
@@ -102,14 +134,23 @@ __device__ __forceinline__ void load_angles(const float* row, int gl, int half, 
       }
   }
 }
+// By the angles (c, s), or back with s negated.
 template <int VEC, bool HALVES>
-__device__ __forceinline__ void rotate(Part<VEC>& x, const float (&c)[VEC], const float (&s)[VEC], float sign) {
+__device__ __forceinline__ void rotate(Part<VEC>& x, const float (&c)[VEC], const float (&s)[VEC]) {
+  if constexpr (HALVES) {
 #pragma unroll
-  for (int i = 0; i < VEC; ++i) {
-    const int a = HALVES ? i : 2 * i, b = HALVES ? VEC + i : 2 * i + 1;
-    const float x0 = x.v[a], x1 = x.v[b], si = sign * s[i];
-    x.v[a] = x0 * c[i] - x1 * si;
-    x.v[b] = x0 * si + x1 * c[i];
+    for (int i = 0; i < VEC / 2; ++i) {
+      const float2 a = two(x, i), b = two(x, VEC / 2 + i), ci = make_float2(c[2 * i], c[2 * i + 1]), si = make_float2(s[2 * i], s[2 * i + 1]);
+      put(x, i, fma2(b, make_float2(-si.x, -si.y), mul2(a, ci)));
+      put(x, VEC / 2 + i, fma2(a, si, mul2(b, ci)));
+    }
+  } else {
+#pragma unroll
+    for (int i = 0; i < VEC; ++i) {
+      const float x0 = x.v[2 * i], x1 = x.v[2 * i + 1];
+      x.v[2 * i] = x0 * c[i] - x1 * s[i];
+      x.v[2 * i + 1] = x0 * s[i] + x1 * c[i];
+    }
   }
 }
 
@@ -152,7 +193,7 @@ __device__ __forceinline__ int64_t angle_row(const RotArgs& r, int pos, bool* ba
 }
 
 template <typename T, int G, bool HALVES>
-__global__ void __launch_bounds__(THREADS) qk_norm_rope_kernel(const NormArgs p) {
+__global__ void __launch_bounds__(THREADS, CTAS<T>) qk_norm_rope_kernel(const NormArgs p) {
   constexpr int VEC = Piece<T>::VEC;
   constexpr int GROUPS = THREADS / G;
   mca_pdl_launch_dependents();
@@ -177,20 +218,19 @@ __global__ void __launch_bounds__(THREADS) qk_norm_rope_kernel(const NormArgs p)
     const int h0 = (int)(un - token * chunks) * HEADS;
     const int b = (int)(token / (uint32_t)p.T), t = (int)(token - (uint32_t)b * p.T);
     const bool mine = live && in;
+    const int pos = p.positions != nullptr ? p.positions[token] : t;
+    bool bad;   // a position that has no angles: zeros all the way
+    const int64_t ar = angle_row(p.r, pos, &bad);
     uint4 raw[HEADS][2];
 #pragma unroll
     for (int i = 0; i < HEADS; ++i) {
-      if (mine && h0 + i < heads) {
+      raw[i][0] = raw[i][1] = make_uint4(0, 0, 0, 0);
+      if (mine && !bad && h0 + i < heads) {
         const char* row = at(p.x[kind], b, t, h0 + i);
         raw[i][0] = reinterpret_cast<const uint4*>(row)[gl];
         raw[i][1] = reinterpret_cast<const uint4*>(row + half * sizeof(T))[gl];
-      } else {
-        raw[i][0] = raw[i][1] = make_uint4(0, 0, 0, 0);
       }
     }
-    const int pos = p.positions != nullptr ? p.positions[token] : t;
-    bool bad;
-    const int64_t ar = angle_row(p.r, pos, &bad);
     float c[VEC], s[VEC];
     if (p.r.cos_table != nullptr && mine && !bad) {
       load_angles<VEC, HALVES>(p.r.cos_table + ar, gl, half, c);
@@ -206,24 +246,18 @@ __global__ void __launch_bounds__(THREADS) qk_norm_rope_kernel(const NormArgs p)
       Piece<T>::unpack(raw[i][0], x.v);
       Piece<T>::unpack(raw[i][1], x.v + VEC);
       if (p.r.norm) {
-        float q = 0.f;
-#pragma unroll
-        for (int j = 0; j < 2 * VEC; ++j) q = fmaf(x.v[j], x.v[j], q);
-        const float inv = 1.0f / sqrtf(group_sum<G>(q) * inv_d + p.r.eps);
-#pragma unroll
-        for (int j = 0; j < 2 * VEC; ++j) x.v[j] = x.v[j] * inv * w.v[j];
+        const float inv = rsqrtf(group_sum<G>(dot(x, x)) * inv_d + p.r.eps);
+        times(x, bad ? 0.f : inv);
+        times(x, w);
       }
-      if (p.r.cos_table != nullptr) rotate<VEC, HALVES>(x, c, s, 1.f);
-      if (bad)   // zero, whatever the row holds
-#pragma unroll
-        for (int j = 0; j < 2 * VEC; ++j) x.v[j] = 0.f;
+      if (p.r.cos_table != nullptr) rotate<VEC, HALVES>(x, c, s);
       if (mine && h0 + i < heads) store_part<T>(reinterpret_cast<T*>(const_cast<char*>(at(p.out[kind], b, t, h0 + i))), gl, half, x);
     }
   }
 }
 
 template <typename T, int G, bool HALVES>
-__global__ void __launch_bounds__(THREADS) qk_norm_rope_bwd_kernel(const NormArgs p) {
+__global__ void __launch_bounds__(THREADS, CTAS<T>) qk_norm_rope_bwd_kernel(const NormArgs p) {
   constexpr int VEC = Piece<T>::VEC;
   constexpr int GROUPS = THREADS / G;
   __shared__ float s_dw[GROUPS * G * 2 * VEC];
@@ -249,11 +283,14 @@ __global__ void __launch_bounds__(THREADS) qk_norm_rope_bwd_kernel(const NormArg
     const int h0 = (int)(un - token * chunks) * HEADS_BWD;
     const int b = (int)(token / (uint32_t)p.T), t = (int)(token - (uint32_t)b * p.T);
     const bool mine = live && in;
+    const int pos = p.positions != nullptr ? p.positions[token] : t;
+    bool bad;   // a position that has no angles: the forward's row is a constant zero
+    const int64_t ar = angle_row(p.r, pos, &bad);
     uint4 rg[HEADS_BWD][2], rx[HEADS_BWD][2];
 #pragma unroll
     for (int i = 0; i < HEADS_BWD; ++i) {
       rx[i][0] = rx[i][1] = rg[i][0] = rg[i][1] = make_uint4(0, 0, 0, 0);
-      if (mine && h0 + i < heads) {
+      if (mine && !bad && h0 + i < heads) {
         const char* row = at(p.g[kind], b, t, h0 + i);
         rg[i][0] = reinterpret_cast<const uint4*>(row)[gl];
         rg[i][1] = reinterpret_cast<const uint4*>(row + half * sizeof(T))[gl];
@@ -264,13 +301,12 @@ __global__ void __launch_bounds__(THREADS) qk_norm_rope_bwd_kernel(const NormArg
         }
       }
     }
-    const int pos = p.positions != nullptr ? p.positions[token] : t;
-    bool bad;
-    const int64_t ar = angle_row(p.r, pos, &bad);
     float c[VEC], s[VEC];
     if (p.r.cos_table != nullptr && mine && !bad) {
       load_angles<VEC, HALVES>(p.r.cos_table + ar, gl, half, c);
       load_angles<VEC, HALVES>(p.r.sin_table + ar, gl, half, s);
+#pragma unroll
+      for (int i = 0; i < VEC; ++i) s[i] = -s[i];
     } else {
 #pragma unroll
       for (int i = 0; i < VEC; ++i) { c[i] = 1.f; s[i] = 0.f; }
@@ -281,35 +317,23 @@ __global__ void __launch_bounds__(THREADS) qk_norm_rope_bwd_kernel(const NormArg
       Part<VEC> g;
       Piece<T>::unpack(rg[i][0], g.v);
       Piece<T>::unpack(rg[i][1], g.v + VEC);
-      if (bad)   // the forward's row is a constant zero
-#pragma unroll
-        for (int j = 0; j < 2 * VEC; ++j) g.v[j] = 0.f;
-      if (p.r.cos_table != nullptr) rotate<VEC, HALVES>(g, c, s, -1.f);
+      if (p.r.cos_table != nullptr) rotate<VEC, HALVES>(g, c, s);
       if (p.r.norm) {
         Part<VEC> x;
         Piece<T>::unpack(rx[i][0], x.v);
         Piece<T>::unpack(rx[i][1], x.v + VEC);
-        if (bad)
+        float inv = rsqrtf(group_sum<G>(dot(x, x)) * inv_d + p.r.eps);
+        if (bad) inv = 0.f;
+        times(x, inv);
+        // rows that are not there have a zero g (and a finite x, but for eps 0): they add nothing
+        if (mine && h0 + i < heads)
 #pragma unroll
-          for (int j = 0; j < 2 * VEC; ++j) x.v[j] = 0.f;
-        float q = 0.f;
+          for (int j = 0; j < VEC; ++j) put(dw, j, fma2(two(g, j), two(x, j), two(dw, j)));
+        times(g, w);
+        const float m = -group_sum<G>(dot(g, x)) * inv_d;
 #pragma unroll
-        for (int j = 0; j < 2 * VEC; ++j) q = fmaf(x.v[j], x.v[j], q);
-        const float inv = 1.0f / sqrtf(group_sum<G>(q) * inv_d + p.r.eps);
-        float m = 0.f;
-#pragma unroll
-        for (int j = 0; j < 2 * VEC; ++j) {
-          x.v[j] *= inv;
-          if (mine && h0 + i < heads) dw.v[j] = fmaf(g.v[j], x.v[j], dw.v[j]);
-          g.v[j] *= w.v[j];
-          m = fmaf(g.v[j], x.v[j], m);
-        }
-        m = group_sum<G>(m) * inv_d;
-#pragma unroll
-        for (int j = 0; j < 2 * VEC; ++j) g.v[j] = inv * (g.v[j] - x.v[j] * m);
-        if (bad)
-#pragma unroll
-          for (int j = 0; j < 2 * VEC; ++j) g.v[j] = 0.f;   // inv of a zero row without eps is infinite
+        for (int j = 0; j < VEC; ++j) put(g, j, fma2(two(x, j), make_float2(m, m), two(g, j)));
+        times(g, inv);
       }
       if (mine && h0 + i < heads) store_part<T>(reinterpret_cast<T*>(const_cast<char*>(at(p.out[kind], b, t, h0 + i))), gl, half, g);
     }
@@ -339,7 +363,8 @@ __global__ void __launch_bounds__(1024) qk_norm_dw_kernel(const float* partial, 
   const int col = blockIdx.y * 32 + threadIdx.x;
   float sum = 0.f;
   if (col < D)
-    for (int i = lo + threadIdx.y; i < hi; i += 32) sum += mca_ld_f1(partial + (int64_t)i * D + col);
+#pragma unroll 8
+    for (int i = lo + threadIdx.y; i < hi; i += 32) sum += __ldcg(partial + (int64_t)i * D + col);
   s[threadIdx.y][threadIdx.x] = sum;
   __syncthreads();
   if (threadIdx.y == 0 && col < D) {
@@ -360,7 +385,7 @@ struct AppendArgs {
 };
 
 template <typename T, typename CT, int G, bool HALVES>
-__global__ void __launch_bounds__(THREADS) paged_append_kernel(const AppendArgs p) {
+__global__ void __launch_bounds__(THREADS, CTAS<T>) paged_append_kernel(const AppendArgs p) {
   constexpr int VEC = Piece<T>::VEC;
   constexpr int GROUPS = THREADS / G;
   mca_pdl_launch_dependents();
@@ -441,14 +466,11 @@ __global__ void __launch_bounds__(THREADS) paged_append_kernel(const AppendArgs 
       Piece<T>::unpack(raw[i][0], x.v);
       Piece<T>::unpack(raw[i][1], x.v + VEC);
       if (norm) {
-        float q = 0.f;
-#pragma unroll
-        for (int j = 0; j < 2 * VEC; ++j) q = fmaf(x.v[j], x.v[j], q);
-        const float inv = 1.0f / sqrtf(group_sum<G>(q) * inv_d + p.r.eps);
-#pragma unroll
-        for (int j = 0; j < 2 * VEC; ++j) x.v[j] = x.v[j] * inv * w.v[j];
+        const float inv = rsqrtf(group_sum<G>(dot(x, x)) * inv_d + p.r.eps);
+        times(x, inv);
+        times(x, w);
       }
-      if (turn) rotate<VEC, HALVES>(x, c, s, 1.f);   // never of values: 0 x infinity is none of theirs
+      if (turn) rotate<VEC, HALVES>(x, c, s);   // never of values: 0 x infinity is none of theirs
       if (zero)
 #pragma unroll
         for (int j = 0; j < 2 * VEC; ++j) x.v[j] = 0.f;
