@@ -3,13 +3,15 @@
 //   out_t = sum_j p_tj v_j / sum_j p_tj,  p_tj = exp(scale q_t . k_j - m_t),  j = 0 .. position(t)
 //
 // in one pass over the keys with the running maximum and sum.  The query heads that share a key/value head are rows of one
-// tile (row = token x group + head), so that a page is read once for all of them.  Three kernels:
+// tile (row = token x group + head), so that a page is read once for all of them.  The kernels:
 //
 //   paged_tc_kernel      bf16 pages: S = Q K^T and O += P V on the tensor cores (tcgen05, TMEM), pages by TMA.
-//   paged_simt_kernel    fp32 activations: exact fp32 products, a lane group per cache row.
+//   paged_simt_kernel    fp32 activations, up to four rows: exact fp32 products, a lane group per cache row.
+//   paged_tile_kernel    fp32 pages, more rows: exact fp32 products on tiles in shared memory.
 //   paged_join_kernel    where few rows meet a long cache the keys are cut into splits, joined here by their maxima and sums.
 #include <algorithm>
 #include <cmath>
+#include <type_traits>
 
 #define MCA_TU_FAIL_FAMILY MCA_FAIL_PAGED
 #include "paged_common.cuh"
@@ -286,6 +288,214 @@ __global__ void __launch_bounds__(SIMT_THREADS, R <= 2 ? 2 : 1) paged_simt_kerne
   }
 }
 
+// More rows than a lane group's registers hold: tiles of 32 rows x 64 keys in shared memory.  A thread forms 4 x 4 logits, then 4 rows
+// x HS / 16 columns of the output; 16 threads share their rows, so the softmax's maxima and sums are shuffles and the output's
+// factors are at hand.  Bound by the fp32 pipes (two FMAs an instruction); the keys of the next tile arrive under this one's
+// softmax and second product, its values under the next first product, and other CTAs of the SM fill the waits.
+// Four prompts of up to 200 tokens over 512 keys, 6 heads of 48: 79 us with four rows a CTA, a lane group a key.
+constexpr int TILE_ROWS = 32, TILE_KEYS = 64, TILE_THREADS = 128;
+template <int HS> struct TilePlan {
+  static constexpr int QP = HS + 4, PP = TILE_ROWS + 4;   // row pitches: 16-byte reads of neighbouring rows fall in different banks
+  static constexpr int OFF_K = TILE_ROWS * QP, OFF_V = OFF_K + TILE_KEYS * QP, OFF_P = OFF_V + TILE_KEYS * HS, FLOATS = OFF_P + TILE_KEYS * PP;
+  static constexpr size_t BYTES = FLOATS * sizeof(float);
+  static constexpr int COLS = HS / 16, VW = COLS % 4 == 0 ? 4 : (COLS % 2 == 0 ? 2 : 1);   // columns of a thread, in pieces of VW, 16 VW apart
+};
+template <int HS>
+__global__ void __launch_bounds__(TILE_THREADS) paged_tile_kernel(const AttnArgs p) {
+  using T = TilePlan<HS>;
+  extern __shared__ __align__(16) float sm[];
+  __shared__ int64_t s_off[2][TILE_KEYS];   // byte offset of each key's row of the head; -1: not there
+  float *sq_ = sm, *sk = sm + T::OFF_K, *sv = sm + T::OFF_V, *sp = sm + T::OFF_P;
+  mca_pdl_launch_dependents();
+  mca_pdl_wait();
+  if ((int)blockIdx.x == p.tiles) {
+    if (blockIdx.y == 0 && blockIdx.z == 0) look_over<float>(p);
+    return;
+  }
+  int seq, row0;
+  Sequence sq;
+  if (!find_tile(p.batch, p.group, TILE_ROWS, p.tiles - 1 - (int)blockIdx.x, &seq, &row0, &sq)) return;   // those of a chunk's end see the most keys
+  const int kvh = blockIdx.y, split = blockIdx.z, tid = threadIdx.x;
+  const int rg = tid >> 4, kg = tid & 15;
+  const int rows = min(TILE_ROWS, sq.count * p.group - row0);
+  const int pos0 = sq.length - sq.count;
+  const int first = pos0 + row0 / p.group, last = pos0 + (row0 + rows - 1) / p.group;   // the last key the first row sees, and any row
+  const int r_begin = split * p.split_len;
+  if (r_begin > last) return;
+  const int r_end = min(last + 1, r_begin + p.split_len);
+  const int n = (r_end - r_begin + TILE_KEYS - 1) / TILE_KEYS;
+  const int in_page = (1 << p.batch.page_shift) - 1;
+
+  auto look_up = [&](int j) {   // rows of key tile j
+    if (tid >= TILE_KEYS || j >= n) return;
+    const int key = r_begin + j * TILE_KEYS + tid;
+    int64_t off = -1;
+    if (key < r_end) {
+      const int page = page_of(p.batch, seq, key, kvh == 0);
+      if (page >= 0) off = page * p.page_bytes + (int64_t)(key & in_page) * p.row_bytes + (int64_t)kvh * HS * 4;
+    }
+    s_off[j & 1][tid] = off;
+  };
+  auto fetch = [&](const char* pages, float* dst, int pitch, int j) {
+    if (j < n)
+      for (int i = tid; i < TILE_KEYS * (HS / 4); i += TILE_THREADS) {
+        const int r = i / (HS / 4), c = i % (HS / 4);
+        const int64_t off = s_off[j & 1][r];
+        float* at = dst + r * pitch + c * 4;
+        if (off >= 0) mca_cp_async16((uint32_t)__cvta_generic_to_shared(at), pages + off + c * 16);
+        else *reinterpret_cast<float4*>(at) = make_float4(0.f, 0.f, 0.f, 0.f);
+      }
+    mca_cp_async_commit();
+  };
+
+  look_up(0);
+  for (int i = tid; i < TILE_ROWS * (HS / 4); i += TILE_THREADS) {
+    const int r = i / (HS / 4), c = i % (HS / 4);
+    float4 v = make_float4(0.f, 0.f, 0.f, 0.f);
+    if (r < rows) {
+      const int row = row0 + r, t = row / p.group, h = kvh * p.group + row - t * p.group;
+      v = mca_ld_f4(reinterpret_cast<const float*>(p.q + (int64_t)(sq.start + t) * p.q_st + h * p.q_sh) + c * 4);
+      v.x *= p.scale_log2; v.y *= p.scale_log2; v.z *= p.scale_log2; v.w *= p.scale_log2;
+    }
+    *reinterpret_cast<float4*>(sq_ + r * T::QP + c * 4) = v;
+  }
+  __syncthreads();
+  fetch(p.k_pages, sk, T::QP, 0);
+  fetch(p.v_pages, sv, HS, 0);
+
+  int lim[4];
+  float m[4], l[4];
+  float acc[4][T::COLS];
+#pragma unroll
+  for (int i = 0; i < 4; ++i) {
+    const int r = rg * 4 + i;
+    lim[i] = r < rows ? pos0 + (row0 + r) / p.group : -1;
+    m[i] = -INFINITY; l[i] = 0.f;
+#pragma unroll
+    for (int c = 0; c < T::COLS; ++c) acc[i][c] = 0.f;
+  }
+  for (int j = 0; j < n; ++j) {
+    const int key0 = r_begin + j * TILE_KEYS;
+    look_up(j + 1);
+    mca_cp_async_wait<1>();      // K(j)
+    __syncthreads();
+    float2 s2[4][4];
+#pragma unroll
+    for (int i = 0; i < 4; ++i)
+#pragma unroll
+      for (int k = 0; k < 4; ++k) s2[i][k] = make_float2(0.f, 0.f);
+#pragma unroll 4
+    for (int d = 0; d < HS; d += 4) {
+      float4 a[4], b[4];
+#pragma unroll
+      for (int i = 0; i < 4; ++i) a[i] = *reinterpret_cast<const float4*>(sq_ + (rg * 4 + i) * T::QP + d);
+#pragma unroll
+      for (int k = 0; k < 4; ++k) b[k] = *reinterpret_cast<const float4*>(sk + (kg + 16 * k) * T::QP + d);
+#pragma unroll
+      for (int i = 0; i < 4; ++i)
+#pragma unroll
+        for (int k = 0; k < 4; ++k) {
+          s2[i][k] = tc::ffma2(make_float2(a[i].x, a[i].y), make_float2(b[k].x, b[k].y), s2[i][k]);
+          s2[i][k] = tc::ffma2(make_float2(a[i].z, a[i].w), make_float2(b[k].z, b[k].w), s2[i][k]);
+        }
+    }
+    bool there[4];
+#pragma unroll
+    for (int k = 0; k < 4; ++k) there[k] = s_off[j & 1][kg + 16 * k] >= 0;
+    __syncthreads();
+    fetch(p.k_pages, sk, T::QP, j + 1);
+    float f[4], pr[4][4];
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+      float mx = -INFINITY;
+#pragma unroll
+      for (int k = 0; k < 4; ++k) {
+        const float v = s2[i][k].x + s2[i][k].y;
+        pr[i][k] = there[k] && key0 + kg + 16 * k <= lim[i] ? v : -INFINITY;
+        mx = fmaxf(mx, pr[i][k]);
+      }
+#pragma unroll
+      for (int o = 8; o > 0; o >>= 1) mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, o));
+      const float m_new = fmaxf(m[i], mx);
+      const float ref = m_new == -INFINITY ? 0.f : m_new;
+      f[i] = m[i] == -INFINITY ? 0.f : tc::fast_exp2(m[i] - ref);
+      m[i] = m_new;
+      float sum = 0.f;
+#pragma unroll
+      for (int k = 0; k < 4; ++k) {
+        pr[i][k] = tc::fast_exp2(pr[i][k] - ref);
+        sum += pr[i][k];
+      }
+      l[i] = fmaf(l[i], f[i], sum);   // this thread's part of the row's sum
+#pragma unroll
+      for (int c = 0; c < T::COLS; ++c) acc[i][c] *= f[i];
+    }
+#pragma unroll
+    for (int k = 0; k < 4; ++k)
+      *reinterpret_cast<float4*>(sp + (kg + 16 * k) * T::PP + rg * 4) = make_float4(pr[0][k], pr[1][k], pr[2][k], pr[3][k]);
+    mca_cp_async_wait<1>();      // V(j)
+    __syncthreads();
+    auto second = [&](auto hidden) {   // hidden: some rows do not see all keys, and 0 x infinity is not 0
+#pragma unroll 4
+      for (int key = 0; key < TILE_KEYS; ++key) {
+        const float4 w = *reinterpret_cast<const float4*>(sp + key * T::PP + rg * 4);
+        const float wi[4] = {w.x, w.y, w.z, w.w};
+        float v[T::COLS];
+#pragma unroll
+        for (int c = 0; c < T::COLS / T::VW; ++c) {
+          const float* at = sv + key * HS + c * 16 * T::VW + kg * T::VW;
+          if constexpr (T::VW == 4) {
+            const float4 t = *reinterpret_cast<const float4*>(at);
+            v[4 * c] = t.x; v[4 * c + 1] = t.y; v[4 * c + 2] = t.z; v[4 * c + 3] = t.w;
+          } else if constexpr (T::VW == 2) {
+            const float2 t = *reinterpret_cast<const float2*>(at);
+            v[2 * c] = t.x; v[2 * c + 1] = t.y;
+          } else {
+            v[c] = *at;
+          }
+        }
+#pragma unroll
+        for (int i = 0; i < 4; ++i) {
+          if (decltype(hidden)::value && key0 + key > lim[i]) continue;
+          if constexpr (T::COLS % 2 == 0) {
+#pragma unroll
+            for (int c = 0; c < T::COLS; c += 2) {
+              const float2 t = tc::ffma2(make_float2(wi[i], wi[i]), make_float2(v[c], v[c + 1]), make_float2(acc[i][c], acc[i][c + 1]));
+              acc[i][c] = t.x; acc[i][c + 1] = t.y;
+            }
+          } else {
+#pragma unroll
+            for (int c = 0; c < T::COLS; ++c) acc[i][c] = fmaf(wi[i], v[c], acc[i][c]);
+          }
+        }
+      }
+    };
+    if (key0 + TILE_KEYS - 1 > first) second(std::true_type{});
+    else second(std::false_type{});
+    __syncthreads();
+    fetch(p.v_pages, sv, HS, j + 1);
+  }
+  mca_cp_async_wait<0>();
+#pragma unroll
+  for (int i = 0; i < 4; ++i) {
+    float sum = l[i];
+#pragma unroll
+    for (int o = 8; o > 0; o >>= 1) sum += __shfl_xor_sync(0xffffffffu, sum, o);
+    const int r = rg * 4 + i;
+    if (r >= rows) continue;
+    const int row = row0 + r, t = row / p.group, h = kvh * p.group + row - t * p.group;
+    const int64_t slot = ((int64_t)(sq.start + t) * p.n_heads + h) * p.nsplit + split;
+    const float inv = p.nsplit > 1 ? 1.f : (sum == 0.f ? 0.f : 1.f / sum);
+    float* dst = p.nsplit > 1 ? p.part_acc + slot * HS : reinterpret_cast<float*>(p.out + (int64_t)(sq.start + t) * p.out_st + h * p.out_sh);
+#pragma unroll
+    for (int c = 0; c < T::COLS; ++c) dst[c / T::VW * 16 * T::VW + kg * T::VW + c % T::VW] = acc[i][c] * inv;
+    if (p.nsplit > 1 && kg == 0) {
+      p.part_ml[slot * 2] = m[i];
+      p.part_ml[slot * 2 + 1] = sum;
+    }
+  }
+}
+
 // ---------------------------------------------------------------------------------------------------------------------
 // Join of the splits: out = sum_s 2^(m_s - M) acc_s / sum_s 2^(m_s - M) l_s.  A warp per (token, head), a lane four elements.
 // ---------------------------------------------------------------------------------------------------------------------
@@ -523,9 +733,57 @@ template <int R> __device__ __forceinline__ Segment segment(const AttnArgs& p, c
   return g;
 }
 
+// Values of a key tile that not every row may see (rows v0 on): 0 x infinity is not 0.  Behind the last key (z0 on) they become zeros;
+// those of the later tokens become zeros where they are not finite, and the rows that do see them get them in the end (add_odd).  The
+// work of `threads` threads; were there any of this one's?
+template <int HDP> __device__ __forceinline__ bool clear_odd(uint32_t v, int v0, int z0, int thread, int threads) {
+  constexpr int CH = HDP / 8, SUB_BYTES = KEYS * 128;
+  auto at = [&](int i) { return v + (uint32_t)(((i % CH) >> 3) * SUB_BYTES + i / CH * 128 + (i & 7) * 16); };
+  for (int i = max(z0, v0) * CH + thread; i < KEYS * CH; i += threads)
+    asm volatile("st.shared.v4.u32 [%0], {%1, %1, %1, %1};" ::"r"(at(i)), "r"(0u) : "memory");
+  bool any = false;
+#pragma unroll 2
+  for (int i = v0 * CH + thread; i < min(z0, KEYS) * CH; i += threads) {
+    uint32_t w[4];
+    asm volatile("ld.shared.v4.u32 {%0, %1, %2, %3}, [%4];" : "=r"(w[0]), "=r"(w[1]), "=r"(w[2]), "=r"(w[3]) : "r"(at(i)) : "memory");
+    // an exponent of all ones carries into the sign's place
+    uint32_t odd = 0;
+#pragma unroll
+    for (int k = 0; k < 4; ++k) odd |= (w[k] & 0x7f807f80u) + 0x00800080u;
+    if (odd & 0x80008000u) {
+      any = true;
+#pragma unroll
+      for (int k = 0; k < 4; ++k) {
+        const uint32_t o = ((w[k] & 0x7f807f80u) + 0x00800080u) & 0x80008000u;
+        if (o & 0x8000u) w[k] &= 0xffff0000u;
+        if (o & 0x80000000u) w[k] &= 0xffffu;
+      }
+      asm volatile("st.shared.v4.u32 [%0], {%1, %2, %3, %4};" ::"r"(at(i)), "r"(w[0]), "r"(w[1]), "r"(w[2]), "r"(w[3]) : "memory");
+    }
+  }
+  asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
+  return any;
+}
+// Adds the values that clear_odd took out, of the later tokens that the row sees (its last key), to `n` columns of what the thread
+// has just written: the output (bf16 where T is) or the part's sums, whose pieces of four lie `pitch` floats apart.
+template <typename T> __device__ __noinline__ void add_odd(const AttnArgs& p, const Segment& g, int last, int col, int n, T* out, int pitch) {
+  for (int key = max(g.k_begin, g.pos + 1); key <= min(last, g.k_end - 1); ++key) {
+    const int page = page_of(p.batch, g.seq, key, false);
+    if (page < 0) continue;
+    const __nv_bfloat16* v = reinterpret_cast<const __nv_bfloat16*>(p.v_pages + page * p.page_bytes + (int64_t)(key & ((1 << p.batch.page_shift) - 1)) * p.row_bytes) +
+                             g.kvh * p.hs;
+    for (int i = col; i < col + n; ++i) {
+      const float x = __bfloat162float(v[i]);
+      if (isfinite(x)) continue;
+      T* at = out + (int64_t)(i >> 2) * pitch + (i & 3);
+      *at = T(float(*at) + x);
+    }
+  }
+}
+
 template <int HDP, bool ACT32, bool FEW>
 __global__ void __launch_bounds__(TC_THREADS, (TcPlan<HDP, FEW>::CTAS)) paged_tc_kernel(const __grid_constant__ CUtensorMap map_k,
-                                                                                       const __grid_constant__ CUtensorMap map_v, const AttnArgs p) {
+                                                                                       const __grid_constant__ CUtensorMap map_v, const __grid_constant__ AttnArgs p) {
   using PL = TcPlan<HDP, FEW>;
   constexpr int STG = PL::STG;
   constexpr int R = ACT32 ? 64 : 128;   // query rows of a tile
@@ -554,6 +812,7 @@ __global__ void __launch_bounds__(TC_THREADS, (TcPlan<HDP, FEW>::CTAS)) paged_tc
     prefetch_tensormap(&map_v);
   }
   if (tid == 0) {
+    *reinterpret_cast<volatile int*>(smem + PL::OFF_BAR + TB_COUNT * 8 + 8) = 0;
     for (int i = 0; i < TB_COUNT; ++i) {
       const bool by_softmax = (i >= TB_P1 && i < TB_O) || i == TB_RED;
       mbar_init(bar(i), i == TB_Q ? 8u : (by_softmax ? (uint32_t)p.warps : (i >= TB_GE ? 9u : 1u)));
@@ -571,6 +830,7 @@ __global__ void __launch_bounds__(TC_THREADS, (TcPlan<HDP, FEW>::CTAS)) paged_tc
     return;
   }
   bool ok = true;
+  volatile int* const s_odd = reinterpret_cast<volatile int*>(smem + PL::OFF_BAR + TB_COUNT * 8 + 8);   // the last part that values were taken out of, plus one
   int c = 0;      // key tiles so far: stages and phases go by it
   int item = 0;   // parts of items so far
   Segment* const ring = reinterpret_cast<Segment*>(smem + PL::OFF_SEG);
@@ -797,6 +1057,12 @@ __global__ void __launch_bounds__(TC_THREADS, (TcPlan<HDP, FEW>::CTAS)) paged_tc
           float m_used[2] = {-INFINITY, -INFINITY}, l[2] = {0.f, 0.f};
           for (int j = 0; j < g.n; ++j, ++c) {
             const uint32_t t_s = t_row + (FEW ? (uint32_t)(c & 1) * 128u : 0u);
+            const int key0 = g.k_begin + j * KEYS;
+            if (key0 + KEYS - 1 > g.pos) {   // g.pos: the last key the tile's first row sees.  (Here, while there are registers for it)
+              ok = __all_sync(0xffffffffu, mbar_wait(bar(TB_VF + c % STG), (uint32_t)((c / STG) & 1), status, 31, c));
+              if (!ok) break;
+              if (clear_odd<HDP>(smem_base + PL::OFF_V + (c % STG) * PL::TILE_BYTES, max(g.pos + 1 - key0, 0), g.last + 1 - key0, rank * 32 + lane, p.warps * 32)) *s_odd = item + 1;
+            }
             ok = __all_sync(0xffffffffu, mbar_wait(bar(TB_S + (FEW ? c & 1 : 0)), (uint32_t)((FEW ? c >> 1 : c) & 1), status, 30, c));
             if (!ok) break;
             tc_fence_after();
@@ -819,23 +1085,10 @@ __global__ void __launch_bounds__(TC_THREADS, (TcPlan<HDP, FEW>::CTAS)) paged_tc
               tmem_ldq256_x8(t_s + 64, s + 32);
               tmem_wait_ld();
             }
-            const int key0 = g.k_begin + j * KEYS;
-            if (key0 + KEYS - 1 > g.pos) {   // g.pos: the last key the tile's first row sees
+            if (key0 + KEYS - 1 > g.pos) {
 #pragma unroll
               for (int i = 0; i < 64; ++i)
                 if (key0 + 8 * (i >> 2) + 2 * quad + (i & 1) > lim[(i >> 1) & 1]) s[i] = 0xff800000u;
-              if (key0 + KEYS > g.last + 1) {
-                // what lies behind the last key is nobody's: its values become zeros, since 0 x infinity is not
-                ok = __all_sync(0xffffffffu, mbar_wait(bar(TB_VF + c % STG), (uint32_t)((c / STG) & 1), status, 31, c));
-                if (!ok) break;
-                uint8_t* v = smem + PL::OFF_V + (c % STG) * PL::TILE_BYTES;
-                const int z0 = g.last + 1 - key0;
-                for (int i = rank * 32 + lane; i < (KEYS - z0) * CH; i += p.warps * 32) {
-                  const int r = z0 + i / CH, ch = i % CH;
-                  *reinterpret_cast<uint4*>(v + (ch >> 3) * PL::SUB_BYTES + r * 128 + (ch & 7) * 16) = make_uint4(0, 0, 0, 0);
-                }
-                asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
-              }
             }
             if (holes) {
 #pragma unroll 1
@@ -997,6 +1250,12 @@ __global__ void __launch_bounds__(TC_THREADS, (TcPlan<HDP, FEW>::CTAS)) paged_tc
               }
             }
           }
+          if (*s_odd == item + 1 && mine) {
+            const int n = min(OC, p.hs - col0);
+            if (g.slot >= 0) add_odd<float>(p, g, g.pos + t, col0, n, p.part_acc + ((int64_t)g.slot * (p.hs / 4) * p.rows_max + rr) * 4, p.rows_max * 4);
+            else if constexpr (ACT32) add_odd<float>(p, g, g.pos + t, col0, n, reinterpret_cast<float*>(dst), 4);
+            else add_odd<__nv_bfloat16>(p, g, g.pos + t, col0, n, reinterpret_cast<__nv_bfloat16*>(dst), 4);
+          }
           tc_fence_before();   // O has been read before the query tile's barrier lets the next products start
         }
       }
@@ -1090,18 +1349,21 @@ int make_plan(const McaPagedCache* c, const McaPagedBatch* b, int dtype, Plan* o
     out->bytes = out->join ? (int64_t)out->ctas * (2ll * out->rows_max * (c->head_size + 2) * 4 + 32) : 0;
     return 0;
   }
-  out->rows = most_rows >= 4 ? 4 : (most_rows >= 2 ? 2 : 1);
+  // fp32 pages: eight rows and more on tiles (where a lane group a key reads them twice or more); bf16 ones come here with up to four
+  out->rows = most_rows >= 8 ? TILE_ROWS : (most_rows >= 3 ? 4 : (most_rows >= 2 ? 2 : 1));
   const int64_t tiles = most_rows <= out->rows ? b->n_seqs : (int64_t)b->n_tokens * group / out->rows + b->n_seqs;
   if (tiles >= (1ll << 30)) return ERROR_PARAM_OUT_OF_RANGE;
   out->tiles = (int)tiles;
   const int64_t ctas = tiles * c->n_kv_heads;
-  const int slots = out->rows == 4 ? 148 : 296;
+  const int tile_bytes = (TILE_ROWS + TILE_KEYS) * (c->head_size + 4) * 4 + TILE_KEYS * (c->head_size + TILE_ROWS + 4) * 4 + 2048;
+  const int slots = out->rows == TILE_ROWS ? 148 * (227 * 1024 / tile_bytes) : (out->rows == 4 ? 148 : 296);
   // time in keys of one CTA: whole waves of (set-up + the keys of a split); more than one split also writes and joins partial results
   const double part_keys = (double)b->n_tokens * c->n_heads * c->head_size * 8.0 / 5e6 * 128.0;   // 5 TB/s; 128 keys are about a microsecond
   double best = 1e300;
   int64_t len = 0;
+  const int step = out->rows == TILE_ROWS ? TILE_KEYS : 16;
   for (int n = 1; n <= std::max(1, std::min(64, b->max_len / 128)); ++n) {
-    const int64_t l = ((b->max_len + n - 1) / n + 15) / 16 * 16;
+    const int64_t l = ((b->max_len + n - 1) / n + step - 1) / step * step;
     const double cost = (double)((ctas * n + slots - 1) / slots) * (64.0 + (double)l) + (n > 1 ? 512 + n * part_keys : 0);
     if (cost < best) { best = cost; len = l; }
   }
@@ -1153,6 +1415,14 @@ int launch_simt(int rows, const AttnArgs& a, cudaStream_t st) {
       if ((e = mca_smem_once(done4, paged_simt_kernel<CT, HS, 4>, smem))) return e;
       return mca_launch_pdl(paged_simt_kernel<CT, HS, 4>, grid, dim3(SIMT_THREADS), smem, st, a);
   }
+}
+
+template <int HS>
+int launch_tile(const AttnArgs& a, cudaStream_t st) {
+  static std::atomic<uint64_t> done{0};
+  const int e = mca_smem_once(done, paged_tile_kernel<HS>, TilePlan<HS>::BYTES);
+  if (e) return e;
+  return mca_launch_pdl(paged_tile_kernel<HS>, dim3(a.tiles + 1, a.n_kv, a.nsplit), dim3(TILE_THREADS), TilePlan<HS>::BYTES, st, a);
 }
 
 int check_types(const McaPagedCache* c, int dtype) {
@@ -1207,7 +1477,14 @@ int mca_paged_attention(const McaPagedCache* cache, const McaPagedBatch* batch, 
     const dim3 grid(plan.ctas, std::min(8, mca_ceil_div(plan.rows_max * D / 4, 512)));   // two pieces a thread
     return f32 ? mca_launch_pdl(paged_join_kernel<float>, grid, dim3(256), 0, st, a) : mca_launch_pdl(paged_join_kernel<__nv_bfloat16>, grid, dim3(256), 0, st, a);
   }
-  switch (D) {
+  if (plan.rows == TILE_ROWS) {
+    switch (D) {
+#define MCA_PAGED_CASE(HS_) case HS_: e = launch_tile<HS_>(a, st); break;
+      MCA_PAGED_CASE(32) MCA_PAGED_CASE(48) MCA_PAGED_CASE(64) MCA_PAGED_CASE(96) MCA_PAGED_CASE(128)
+#undef MCA_PAGED_CASE
+      default: return ERROR_ATTN_UNSUPPORTED_SHAPE;
+    }
+  } else switch (D) {
 #define MCA_PAGED_CASE(HS_) \
     case HS_: e = csize == 2 ? launch_simt<__nv_bfloat16, HS_>(plan.rows, a, st) : launch_simt<float, HS_>(plan.rows, a, st); break;
     MCA_PAGED_CASE(32) MCA_PAGED_CASE(48) MCA_PAGED_CASE(64) MCA_PAGED_CASE(96) MCA_PAGED_CASE(128)

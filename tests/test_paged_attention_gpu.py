@@ -196,3 +196,37 @@ def test_many_key_tiles_for_each_block_of_chunks(act, cache, hs):
     s.cache.attend(s.batch, s.q, s.out)
     s.check()
     assert s.cache.status() == (0, 0, 0, 0)
+
+
+@pytest.mark.parametrize("act,cache", TYPES)
+@pytest.mark.parametrize("hs", [48, 128])
+@pytest.mark.parametrize("long", [False, True])
+def test_values_that_are_not_finite_reach_only_the_tokens_that_see_them(act, cache, hs, long):
+    """A later token of the same chunk holds an infinity or NaN: the tokens before it come out as without it."""
+    n = 3000 if long else 100
+    s = setup([(40, n), (1, 30)], 4, 2, hs, 16, act, cache, seed=17)
+    clean = [v.clone() for v in s.v], [k.clone() for k in s.k]
+    at = [(n - 25, 0, 5, math.inf), (n - 12, 1, hs - 1, math.nan), (n - 12, 1, 0, -math.inf)]
+    for pos, h, col, x in at:
+        s.v_pages[int(s.table[0, pos // 16]), pos % 16, h, col] = x
+        s.v[0][pos, h, col] = 0.0
+    s.k_pages[int(s.table[0, (n - 3) // 16]), (n - 3) % 16] = math.nan      # the last three tokens see a NaN logit
+    s.cache.attend(s.batch, s.q, s.out)
+    ref, tol = s.exact()
+    hit = torch.zeros_like(ref, dtype=torch.bool)
+    for pos, h, col, _ in at:
+        hit[pos - (n - 40):40, 2 * h:2 * h + 2, col] = True
+    hit[37:40] = True
+    out = s.out.double()
+    assert not torch.isfinite(out[hit]).any()
+    assert torch.isfinite(out[~hit]).all()
+    assert ((out - ref).abs() <= tol)[~hit].all()
+    assert torch.isinf(out[15:28, :2, 5]).all() and (out[15:28, :2, 5] > 0).all()
+
+
+@pytest.mark.parametrize("hs", [32, 48, 64, 96, 128])
+def test_fp32_tiles(hs):
+    """Rows that fill fp32 tiles and leave one ragged, over splits and pages that are gone."""
+    s = setup([(31, 31), (33, 700), (64, 64), (9, 2100), (100, 130)], 6, 2, hs, 16, "f32", "f32", seed=18, drop=[(1, 0), (1, 5), (3, 100)])
+    s.cache.attend(s.batch, s.q, s.out)
+    s.check()
