@@ -1357,14 +1357,16 @@ int make_plan(const McaPagedCache* c, const McaPagedBatch* b, int dtype, Plan* o
   const int64_t ctas = tiles * c->n_kv_heads;
   const int tile_bytes = (TILE_ROWS + TILE_KEYS) * (c->head_size + 4) * 4 + TILE_KEYS * (c->head_size + TILE_ROWS + 4) * 4 + 2048;
   const int slots = out->rows == TILE_ROWS ? 148 * (227 * 1024 / tile_bytes) : (out->rows == 4 ? 148 : 296);
-  // time in keys of one CTA: whole waves of (set-up + the keys of a split); more than one split also writes and joins partial results
-  const double part_keys = (double)b->n_tokens * c->n_heads * c->head_size * 8.0 / 5e6 * 128.0;   // 5 TB/s; 128 keys are about a microsecond
+  // time in keys of one CTA: whole waves of (set-up + the keys of a split); more than one split also writes partial results (at some 5 TB/s)
+  // and joins them in some 4 us.  128 keys take a lane group's CTA about a microsecond, a tile's eight.
+  const double key_us = (out->rows == TILE_ROWS ? 8.0 : 1.0) / 128.0;
+  const double part_keys = (double)b->n_tokens * c->n_heads * c->head_size * 8.0 / 5e6 / key_us, join_keys = 4.0 / key_us;
   double best = 1e300;
   int64_t len = 0;
   const int step = out->rows == TILE_ROWS ? TILE_KEYS : 16;
   for (int n = 1; n <= std::max(1, std::min(64, b->max_len / 128)); ++n) {
     const int64_t l = ((b->max_len + n - 1) / n + step - 1) / step * step;
-    const double cost = (double)((ctas * n + slots - 1) / slots) * (64.0 + (double)l) + (n > 1 ? 512 + n * part_keys : 0);
+    const double cost = (double)((ctas * n + slots - 1) / slots) * (64.0 + (double)l) + (n > 1 ? join_keys + n * part_keys : 0);
     if (cost < best) { best = cost; len = l; }
   }
   out->split_len = (int)len;
