@@ -108,7 +108,8 @@ __device__ __forceinline__ int page_of(const Batch& t, int seq, int pos, bool te
 // ---------------------------------------------------------------------------------------------------------------------
 constexpr int SIMT_THREADS = 256, SIMT_WARPS = SIMT_THREADS / 32;
 
-// Elements of a row one lane holds: a group of HS / EPL lanes (a power of two) covers a row with 16-byte pieces.
+// Elements of a row one lane holds: a group of HS / EPL lanes (a power of two) covers a row with 16-byte pieces.  (Half as many, so that
+// two CTAs of four query rows fit an SM, take twice the shuffles: 16 tokens over 2000 fp32 keys, 32 / 8 heads of 128, 68 us for 61.)
 template <typename CT, int HS> struct Lanes {
   static constexpr int VEC = 16 / (int)sizeof(CT);
   static constexpr int EPL = HS % 48 == 0 ? (VEC == 4 ? 12 : 24) : 16;
@@ -222,9 +223,10 @@ __global__ void __launch_bounds__(SIMT_THREADS, R <= 2 ? 2 : 1) paged_simt_kerne
     }
 #pragma unroll
     for (int x = 0; x < R; ++x) {
-      float s = 0.f;
+      float2 s2 = make_float2(0.f, 0.f);   // two products an instruction
 #pragma unroll
-      for (int i = 0; i < EPL; ++i) s = fmaf(q[x][i], kx[i], s);
+      for (int i = 0; i < EPL; i += 2) s2 = tc::ffma2(make_float2(q[x][i], q[x][i + 1]), make_float2(kx[i], kx[i + 1]), s2);
+      float s = s2.x + s2.y;
 #pragma unroll
       for (int o = G / 2; o > 0; o >>= 1) s += __shfl_xor_sync(0xffffffffu, s, o);
       if (valid && row <= lim[x]) {
@@ -238,7 +240,10 @@ __global__ void __launch_bounds__(SIMT_THREADS, R <= 2 ? 2 : 1) paged_simt_kerne
         const float w = tc::fast_exp2(s - m[x]);
         l[x] += w;
 #pragma unroll
-        for (int i = 0; i < EPL; ++i) acc[x][i] = fmaf(w, vx[i], acc[x][i]);
+        for (int i = 0; i < EPL; i += 2) {
+          const float2 a = tc::ffma2(make_float2(w, w), make_float2(vx[i], vx[i + 1]), make_float2(acc[x][i], acc[x][i + 1]));
+          acc[x][i] = a.x; acc[x][i + 1] = a.y;
+        }
       }
     }
   }
@@ -1330,7 +1335,9 @@ int make_plan(const McaPagedCache* c, const McaPagedBatch* b, int dtype, Plan* o
   const int64_t most_rows = (int64_t)b->max_new * group;   // of one sequence and key/value head
   const bool act32 = dtype == MCA_DTYPE_F32;
   *out = Plan{};
-  out->tc = !act32 || (c->dtype == MCA_DTYPE_BF16 && most_rows > 4);
+  // bf16 pages: the tensor-core kernel, but for fp32 queries that share their keys with none (16 tokens over 2000 keys of 32 heads of
+  // 128: 76 us in exact fp32 here, bound by memory either way; with 4 queries to a key 65 us there and 31 on the tensor cores)
+  out->tc = !act32 || (c->dtype == MCA_DTYPE_BF16 && most_rows > 1);
   if (out->tc) {
     const int R = act32 ? 64 : 128;
     out->rows = R;
@@ -1349,8 +1356,8 @@ int make_plan(const McaPagedCache* c, const McaPagedBatch* b, int dtype, Plan* o
     out->bytes = out->join ? (int64_t)out->ctas * (2ll * out->rows_max * (c->head_size + 2) * 4 + 32) : 0;
     return 0;
   }
-  // fp32 pages: eight rows and more on tiles (where a lane group a key reads them twice or more); bf16 ones come here with up to four
-  out->rows = most_rows >= 8 ? TILE_ROWS : (most_rows >= 3 ? 4 : (most_rows >= 2 ? 2 : 1));
+  // fp32 pages: more than eight rows on tiles, fewer a lane group a key, four rows a CTA
+  out->rows = most_rows > 8 ? TILE_ROWS : (most_rows > 2 ? 4 : (int)most_rows);
   const int64_t tiles = most_rows <= out->rows ? b->n_seqs : (int64_t)b->n_tokens * group / out->rows + b->n_seqs;
   if (tiles >= (1ll << 30)) return ERROR_PARAM_OUT_OF_RANGE;
   out->tiles = (int)tiles;
@@ -1400,25 +1407,6 @@ template <bool ACT32, bool FEW>
 int launch_tc(const McaPagedCache* c, const AttnArgs& a, cudaStream_t st) {
   return a.hs <= 64 ? launch_tc<64, ACT32, FEW>(c, a, st) : launch_tc<128, ACT32, FEW>(c, a, st);
 }
-template <typename CT, int HS>
-int launch_simt(int rows, const AttnArgs& a, cudaStream_t st) {
-  constexpr size_t smem = Lanes<CT, HS>::RING;
-  static std::atomic<uint64_t> done1{0}, done2{0}, done4{0};
-  const dim3 grid(a.tiles + 1, a.n_kv, a.nsplit);
-  int e;
-  switch (rows) {
-    case 1:
-      if ((e = mca_smem_once(done1, paged_simt_kernel<CT, HS, 1>, smem))) return e;
-      return mca_launch_pdl(paged_simt_kernel<CT, HS, 1>, grid, dim3(SIMT_THREADS), smem, st, a);
-    case 2:
-      if ((e = mca_smem_once(done2, paged_simt_kernel<CT, HS, 2>, smem))) return e;
-      return mca_launch_pdl(paged_simt_kernel<CT, HS, 2>, grid, dim3(SIMT_THREADS), smem, st, a);
-    default:
-      if ((e = mca_smem_once(done4, paged_simt_kernel<CT, HS, 4>, smem))) return e;
-      return mca_launch_pdl(paged_simt_kernel<CT, HS, 4>, grid, dim3(SIMT_THREADS), smem, st, a);
-  }
-}
-
 template <int HS>
 int launch_tile(const AttnArgs& a, cudaStream_t st) {
   static std::atomic<uint64_t> done{0};
@@ -1427,6 +1415,24 @@ int launch_tile(const AttnArgs& a, cudaStream_t st) {
   return mca_launch_pdl(paged_tile_kernel<HS>, dim3(a.tiles + 1, a.n_kv, a.nsplit), dim3(TILE_THREADS), TilePlan<HS>::BYTES, st, a);
 }
 
+template <typename CT, int HS, int R>
+int launch_simt(const AttnArgs& a, cudaStream_t st) {
+  constexpr size_t smem = Lanes<CT, HS>::RING;
+  static std::atomic<uint64_t> done{0};
+  const int e = mca_smem_once(done, paged_simt_kernel<CT, HS, R>, smem);
+  if (e) return e;
+  return mca_launch_pdl(paged_simt_kernel<CT, HS, R>, dim3(a.tiles + 1, a.n_kv, a.nsplit), dim3(SIMT_THREADS), smem, st, a);
+}
+template <int HS>
+int launch_f32(int rows, bool bf16_pages, const AttnArgs& a, cudaStream_t st) {
+  if (bf16_pages) return launch_simt<__nv_bfloat16, HS, 1>(a, st);
+  switch (rows) {
+    case 1: return launch_simt<float, HS, 1>(a, st);
+    case 2: return launch_simt<float, HS, 2>(a, st);
+    case 4: return launch_simt<float, HS, 4>(a, st);
+    default: return launch_tile<HS>(a, st);
+  }
+}
 int check_types(const McaPagedCache* c, int dtype) {
   if (dtype != MCA_DTYPE_F32 && dtype != MCA_DTYPE_BF16) return ERROR_ATTN_UNSUPPORTED_SHAPE;
   if (dtype == MCA_DTYPE_BF16 && c->dtype != MCA_DTYPE_BF16) return ERROR_ATTN_UNSUPPORTED_SHAPE;
@@ -1479,16 +1485,8 @@ int mca_paged_attention(const McaPagedCache* cache, const McaPagedBatch* batch, 
     const dim3 grid(plan.ctas, std::min(8, mca_ceil_div(plan.rows_max * D / 4, 512)));   // two pieces a thread
     return f32 ? mca_launch_pdl(paged_join_kernel<float>, grid, dim3(256), 0, st, a) : mca_launch_pdl(paged_join_kernel<__nv_bfloat16>, grid, dim3(256), 0, st, a);
   }
-  if (plan.rows == TILE_ROWS) {
-    switch (D) {
-#define MCA_PAGED_CASE(HS_) case HS_: e = launch_tile<HS_>(a, st); break;
-      MCA_PAGED_CASE(32) MCA_PAGED_CASE(48) MCA_PAGED_CASE(64) MCA_PAGED_CASE(96) MCA_PAGED_CASE(128)
-#undef MCA_PAGED_CASE
-      default: return ERROR_ATTN_UNSUPPORTED_SHAPE;
-    }
-  } else switch (D) {
-#define MCA_PAGED_CASE(HS_) \
-    case HS_: e = csize == 2 ? launch_simt<__nv_bfloat16, HS_>(plan.rows, a, st) : launch_simt<float, HS_>(plan.rows, a, st); break;
+  switch (D) {
+#define MCA_PAGED_CASE(HS_) case HS_: e = launch_f32<HS_>(plan.rows, csize == 2, a, st); break;
     MCA_PAGED_CASE(32) MCA_PAGED_CASE(48) MCA_PAGED_CASE(64) MCA_PAGED_CASE(96) MCA_PAGED_CASE(128)
 #undef MCA_PAGED_CASE
     default: return ERROR_ATTN_UNSUPPORTED_SHAPE;
