@@ -69,6 +69,8 @@ namespace MyCaffe.common
         internal const int DECODE_CREATE = 2010, DECODE_FREE = 2011, DECODE_STEP = 2012, DECODE_QKV = 2013, DECODE_OUT = 2014;
         internal const int DECODE_FFN = 2015, DECODE_LOGITS = 2016, TFT_ATTN_FWD = 2020, TFT_ATTN_BWD = 2021;
         internal const int SET_ASYNC = 2030, SET_TIMING = 2031, RMSNORM_FWD = 2040, RMSNORM_BWD = 2041;
+        internal const int QK_NORM_ROPE_FWD = 2042, QK_NORM_ROPE_BWD = 2043, PAGED_CREATE = 2060, PAGED_FREE = 2061, PAGED_APPEND = 2062, PAGED_ATTN = 2063;
+        internal const int QK_NORM = 1, ROPE_HALVES = 2;
         internal const int QUERY_VERSION = 2050, QUERY_COUNTERS = 2051;
         internal const int DTYPE_F32 = 0, DTYPE_TF32 = 1, DTYPE_BF16 = 2, FLAG_CAUSAL_IMPLICIT = 1;
         // llama2 extension (CudaExtension.llm32.cpp:20-26) and the id added to it
@@ -220,6 +222,39 @@ namespace MyCaffe.common
         }
 
         // ---- extensions (CudaDnn.cs:3703-3812): the llama2 route ----
+
+        // ---- paged cache and per-head norm with rotation (added ids) -------------------------------------------------------
+        public long CreatePaged(int nPages, int nPageSize, int nHeads, int nKvHeads, int nHeadSize, bool bCacheBf16, int nTableLen, float fTheta,
+                                int nFlags = 0, float fEps = 1e-5f)
+        {
+            return (long)RunFloatEx2(AttnFn.PAGED_CREATE, new float[] { fTheta, fEps },
+                                     new long[] { nPages, nPageSize, nHeads, nKvHeads, nHeadSize, bCacheBf16 ? 1 : 0, nTableLen, nFlags })[0];
+        }
+        public void FreePaged(long h) { RunFloat(AttnFn.PAGED_FREE, new float[] { h }); }
+        public void PagedAppend(long hPaged, long hQ, long hK, long hV, long hWq, long hWk, long hKpages, long hVpages, long hStarts, long hLengths,
+                                long hTable, int nTableStride, int nSeqs, int nTokens, int nMaxNew, int nMaxLen, long hQout)
+        {
+            RunFloatEx2(AttnFn.PAGED_APPEND, null, new long[] { hPaged, hQ, hK, hV, hWq, hWk, hKpages, hVpages, hStarts, hLengths, hTable, nTableStride,
+                                                                nSeqs, nTokens, nMaxNew, nMaxLen, hQout });
+        }
+        public void PagedAttention(long hPaged, long hQ, long hKpages, long hVpages, long hStarts, long hLengths, long hTable, int nTableStride,
+                                   int nSeqs, int nTokens, int nMaxNew, int nMaxLen, long hOut)
+        {
+            RunFloatEx2(AttnFn.PAGED_ATTN, null, new long[] { hPaged, hQ, hKpages, hVpages, hStarts, hLengths, hTable, nTableStride, nSeqs, nTokens,
+                                                              nMaxNew, nMaxLen, hOut });
+        }
+        public void QkNormRopeForward(long hRope, long hQ, long hK, long hWq, long hWk, int nBatch, int nSeqLen, int nHeads, int nKvHeads, int nSize,
+                                      long hQout, long hKout, float fEps = 1e-5f, int nFlags = AttnFn.QK_NORM)
+        {
+            RunFloatEx2(AttnFn.QK_NORM_ROPE_FWD, new float[] { fEps }, new long[] { hRope, hQ, hK, hWq, hWk, nFlags, nBatch, nSeqLen, nHeads, nKvHeads,
+                                                                                    nSize, hQout, hKout });
+        }
+        public void QkNormRopeBackward(long hRope, long hQ, long hK, long hWq, long hWk, int nBatch, int nSeqLen, int nHeads, int nKvHeads, int nSize,
+                                       long hdQout, long hdKout, long hdQ, long hdK, long hdWq, long hdWk, float fEps = 1e-5f, int nFlags = AttnFn.QK_NORM)
+        {
+            RunFloatEx2(AttnFn.QK_NORM_ROPE_BWD, new float[] { fEps }, new long[] { hRope, hQ, hK, hWq, hWk, nFlags, nBatch, nSeqLen, nHeads, nKvHeads,
+                                                                                    nSize, hdQout, hdKout, hdQ, hdK, hdWq, hdWk });
+        }
 
         public long CreateExtension(string strExtensionDllPath) { return (long)RunFloatEx(AttnFn.CREATE_EXTENSION, null, strExtensionDllPath)[0]; }
         public void FreeExtension(long hExtension) { RunFloat(AttnFn.FREE_EXTENSION, new float[] { hExtension }); }

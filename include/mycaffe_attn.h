@@ -93,6 +93,15 @@ typedef char* MCA_LPTSTR;
 #define MCA_FN_TFT_ATTN_BWD 2021   /* longs {hQ,hK,hV,hMask,hdOut,hdAttn,B,H,Nq,Nk,d,hdQ,hdK,hdV} (hMask, hdAttn may be 0) */
 #define MCA_FN_RMSNORM_FWD 2040    /* floats {eps}; longs {hX,hW (0: none),hY,hInvRms,rows,inner}: RMSNormLayer forward in one pass */
 #define MCA_FN_RMSNORM_BWD 2041    /* longs {hX,hW,hdY,hInvRms,hdX,hdW (0: frozen),rows,inner}: its backward */
+#define MCA_FN_QK_NORM_ROPE_FWD 2042 /* floats {eps}; longs {hRope (0: no rotation),hQ,hK,hWq,hWk,flags (MCA_QK_NORM | MCA_ROPE_HALVES),B,T,H,KV,D,
+                                      hQout,hKout}: norm of each head and rotation, tensors (B,T,heads,D) of either element type; hK 0 with KV 0 */
+#define MCA_FN_QK_NORM_ROPE_BWD 2043 /* floats {eps}; longs {hRope,hQ,hK,hWq,hWk,flags,B,T,H,KV,D,hdQout,hdKout,hdQ,hdK,hdWq,hdWk (0: none)} */
+#define MCA_FN_PAGED_CREATE 2060   /* floats {theta (<= 0: no rotation), eps}; longs {nPages,pageSize,nHeads,nKvHeads,headSize,cacheBf16,tableLen,
+                                      flags} -> hPaged */
+#define MCA_FN_PAGED_FREE 2061     /* floats {hPaged} */
+#define MCA_FN_PAGED_APPEND 2062   /* longs {hPaged,hQ,hK,hV,hWq,hWk (0: none),hKpages,hVpages,hStarts,hLengths,hTable,tableStride,nSeqs,nTokens,maxNew,
+                                      maxLen,hQout}: mca_paged_append; starts, lengths, table hold int32 values */
+#define MCA_FN_PAGED_ATTN 2063     /* longs {hPaged,hQ,hKpages,hVpages,hStarts,hLengths,hTable,tableStride,nSeqs,nTokens,maxNew,maxLen,hOut} */
 #define MCA_FN_SET_ASYNC 2030      /* longs {0|1}: 1 = do not synchronise the stream after each call (default 0, as the reference) */
 #define MCA_FN_SET_TIMING 2031     /* longs {0|1}: 1 = bracket every dispatched call with CUDA events (read with MCA_FN_QUERY_COUNTERS) */
 #define MCA_FN_WAIT_PROBE 2032     /* longs {hAttn, limitMicroseconds}: runs mca_wait_probe on the handle's status words, then reports

@@ -91,6 +91,17 @@ struct DecodeHandle {
   int64_t scratch_floats = 0;
 };
 
+// A layer's paged cache as the dispatch ids see it: its geometry, the rotation's tables, and the attention's workspace (grow-only; the
+// calls of a kernel index follow one another on one stream).
+struct PagedHandle {
+  McaPagedCache cache = {};
+  McaQkRotation rotation = {};
+  float *cos_t = nullptr, *sin_t = nullptr;
+  void* work = nullptr;
+  int64_t work_bytes = 0;
+  void release() { cudaFree(cos_t); cudaFree(sin_t); cudaFree(work); }
+};
+
 struct LayerNormHandle {
   int64_t rows = 0;
   int inner = 0;
@@ -127,6 +138,7 @@ struct Kernel {
   std::unordered_map<long, AttnHandle> attn;
   std::unordered_map<long, RopeHandle> rope;
   std::unordered_map<long, DecodeHandle> decode;
+  std::unordered_map<long, PagedHandle> paged;
   std::unordered_map<long, LayerNormHandle> layernorm;
   float* norm_scratch = nullptr;   // grow-only: dW partials of the RMSNorm backward
   int64_t norm_scratch_floats = 0;
@@ -153,6 +165,7 @@ struct Kernel {
   // What a handle sees of it: no more than it asked for, so that its kernels, and its gradients' last bits, do not depend on which other
   // handles there are.
   int64_t ds_room(const AttnHandle& a) const { return std::min(a.ds_floats, ds_ws_floats); }
+  bool paged_pending = false;   // a paged call was made in asynchronous mode and its status words are unread
   bool synced = false;     // the call being dispatched has already synchronised the stream behind its last launch
   bool by_word = false;    // the call being dispatched is waited for by the done word (see sync_call)
   bool fail_words = false; // this device's kernels raise its failure words (see g_fail)
@@ -216,7 +229,7 @@ bool arm_fail_words(int dev) {   // under g_table_lock, with dev current
   if (!(g_fail_armed >> dev & 1)) {
     int* row = g_fail.row(dev);
     if (mca_set_fail_words_fwd(row) || mca_set_fail_words_bwd(row) || mca_set_fail_words_probe(row) || mca_set_fail_words_decode(row) ||
-        mca_set_fail_words_proj(row)) {
+        mca_set_fail_words_proj(row) || mca_set_fail_words_qk_norm(row) || mca_set_fail_words_paged(row)) {
       cudaGetLastError();
       return false;
     }
@@ -683,6 +696,7 @@ long tc_status(Kernel* k, AttnHandle& a) {
   if (k->async) { a.status_pending = true; return 0; }
   return read_status(k, a);
 }
+long paged_status(Kernel* k);
 long sync_and_collect_status(Kernel* k) {
   const long se = sync_call(k);
   if (se) return se;
@@ -691,6 +705,11 @@ long sync_and_collect_status(Kernel* k) {
     if (!kv.second.status_pending) continue;
     kv.second.status_pending = false;
     const long e = read_status(k, kv.second);
+    if (e && !first) first = e;
+  }
+  if (k->paged_pending) {
+    k->paged_pending = false;
+    const long e = paged_status(k);
     if (e && !first) first = e;
   }
   return first;
@@ -1260,6 +1279,199 @@ long rmsnorm_run(Kernel* k, long lInput, float* pf, long llInput, MCA_LONGLONG* 
   return mca_rmsnorm_backward_f32(x, w, dy, inv, dx, dw, k->norm_scratch, k->norm_scratch_floats, rows, (int)inner, 0);
 }
 
+// ---- per-head norm with rotation, paged cache ids -------------------------------------------
+
+// Memory of either element type; the first handle of a call says which (*bf16 < 0), the others have to agree.
+long check_activations(Kernel* k, long h, int64_t need, int* bf16, void** out) {
+  MemItem* m = k->get(h);
+  if (!m) return ERROR_MEMORY_NOT_FOUND;
+  if (*bf16 < 0) *bf16 = m->bf16 ? 1 : 0;
+  return check_any(k, h, need, *bf16 != 0, out);
+}
+bool in_range(const MCA_LONGLONG* v, int n, MCA_LONGLONG least) {   // each is an int of at least `least`
+  for (int i = 0; i < n; ++i)
+    if (v[i] < least || v[i] > INT32_MAX) return false;
+  return true;
+}
+
+// floats {eps}; longs {hRope (0: no rotation),hQ,hK,hWq,hWk,flags,B,T,H,KV,D,hQout,hKout}; backward: {...,D,hdQout,hdKout,hdQ,hdK,hdWq,hdWk}.
+// Tensors (B,T,heads,D); hK, its outputs and the weights may be 0.
+long qk_norm_rope_run(Kernel* k, long lInput, float* pf, long llInput, MCA_LONGLONG* pl, bool backward) {
+  long e;
+  const int want = backward ? 17 : 13;
+  if ((e = verify_in(lInput, pf, 1, 1)) || (e = verify_in(llInput, pl, want, want))) return e;
+  if (!in_range(pl + 5, 1, 0) || !in_range(pl + 6, 3, 1) || !in_range(pl + 9, 1, 0) || !in_range(pl + 10, 1, 1)) return ERROR_PARAM_OUT_OF_RANGE;
+  const int B = (int)pl[6], T = (int)pl[7], H = (int)pl[8], KV = (int)pl[9], D = (int)pl[10];
+  if (D > 256 || H > 65535 || KV > 65535 || (int64_t)B * T > INT32_MAX) return ERROR_PARAM_OUT_OF_RANGE;
+  McaQkRotation r = {};
+  r.flags = (int)pl[5]; r.eps = pf[0];
+  if (pl[0] != 0) {
+    auto it = k->rope.find((long)pl[0]);
+    if (it == k->rope.end()) return ERROR_ROPE_NOT_INITIALIZED;
+    if (it->second.D != D || it->second.T < T) return ERROR_PARAM_OUT_OF_RANGE;
+    r.cos_table = it->second.cos_t; r.sin_table = it->second.sin_t; r.table_len = it->second.T;
+  }
+  float* w[2] = {nullptr, nullptr};
+  for (int i = 0; i < 2; ++i)
+    if (pl[3 + i] != 0 && (e = check_f32(k, (long)pl[3 + i], D, &w[i]))) return e;
+  r.q_weight = w[0]; r.k_weight = w[1];
+  int bf16 = -1;
+  auto heads = [&](long h, int n, McaHeads* out) -> long {
+    *out = McaHeads{nullptr, (int64_t)T * n * D, (int64_t)n * D, D};
+    return check_activations(k, h, (int64_t)B * T * n * D, &bf16, &out->data);
+  };
+  McaHeads t[6];   // q, k, then what follows in pairs
+  const int pairs = backward ? 3 : 2;
+  for (int i = 0; i < pairs; ++i) {
+    const MCA_LONGLONG* h = i == 0 ? pl + 1 : pl + 11 + 2 * (i - 1);
+    if ((e = heads((long)h[0], H, &t[2 * i]))) return e;
+    if (KV > 0 && (e = heads((long)h[1], KV, &t[2 * i + 1]))) return e;
+  }
+  const McaHeads* kv[3] = {KV > 0 ? &t[1] : nullptr, KV > 0 ? &t[3] : nullptr, KV > 0 ? &t[5] : nullptr};
+  const int dtype = bf16 ? MCA_DTYPE_BF16 : MCA_DTYPE_F32;
+  if (!backward) return mca_qk_norm_rope_forward(&r, &t[0], kv[0], nullptr, dtype, B, T, H, KV, D, &t[2], kv[1], 0);
+  float* dw[2] = {nullptr, nullptr};
+  for (int i = 0; i < 2; ++i)
+    if (pl[15 + i] != 0 && (e = check_f32(k, (long)pl[15 + i], D, &dw[i]))) return e;
+  if (dw[0] || dw[1]) {
+    const int64_t need = mca_qk_norm_rope_backward_scratch_floats(D);
+    if (need > k->norm_scratch_floats) {
+      cudaFree(k->norm_scratch);
+      k->norm_scratch = nullptr; k->norm_scratch_floats = 0;
+      if (cudaMalloc(&k->norm_scratch, (size_t)need * sizeof(float)) != cudaSuccess) { cudaGetLastError(); return ERROR_MEMORY_OUT; }
+      k->norm_scratch_floats = need;
+    }
+  }
+  return mca_qk_norm_rope_backward(&r, &t[0], kv[0], nullptr, &t[2], kv[1], dtype, B, T, H, KV, D, &t[4], kv[2], dw[0], dw[1], k->norm_scratch,
+                                   k->norm_scratch_floats, 0);
+}
+
+long paged_create(Kernel* k, long lInput, float* pf, long llInput, MCA_LONGLONG* pl, MCA_LONG* plOutput, float** ppOutput) {
+  long e;  // floats {theta, eps}; longs {nPages,pageSize,nHeads,nKvHeads,headSize,cacheBf16,tableLen,flags}
+  if ((e = verify_in(lInput, pf, 2, 2)) || (e = verify_in(llInput, pl, 8, 8)) || (e = verify_out(plOutput, ppOutput))) return e;
+  if (!in_range(pl, 5, 1) || !in_range(pl + 6, 1, 0) || !in_range(pl + 7, 1, 0)) return ERROR_PARAM_OUT_OF_RANGE;
+  PagedHandle p;
+  McaPagedCache& c = p.cache;
+  c.n_pages = (int)pl[0]; c.page_size = (int)pl[1]; c.n_heads = (int)pl[2]; c.n_kv_heads = (int)pl[3]; c.head_size = (int)pl[4];
+  c.dtype = pl[5] != 0 ? MCA_DTYPE_BF16 : MCA_DTYPE_F32;
+  if (!mca_decode_head_size_supported(c.head_size)) return ERROR_ATTN_UNSUPPORTED_SHAPE;
+  if (c.n_heads % c.n_kv_heads || c.n_heads > 65535 || c.page_size < 16 || c.page_size > 65536 || (c.page_size & (c.page_size - 1))) return ERROR_PARAM_OUT_OF_RANGE;
+  if (pl[7] & ~(MCA_QK_NORM | MCA_ROPE_HALVES)) return ERROR_PARAM_OUT_OF_RANGE;
+  c.page_stride = (int64_t)c.page_size * c.n_kv_heads * c.head_size;
+  p.rotation.flags = (int)pl[7]; p.rotation.eps = pf[1];
+  if (pf[0] > 0.f) {   // theta <= 0: no rotation, as DECODE_CREATE
+    if (pl[6] < 1 || pl[6] > (1 << 24)) return ERROR_PARAM_OUT_OF_RANGE;
+    const size_t n = (size_t)pl[6] * (c.head_size / 2);
+    std::vector<float> cs, sn;
+    try {
+      cs.resize(n); sn.resize(n);
+    } catch (const std::bad_alloc&) {
+      return ERROR_MEMORY_OUT;
+    }
+    mca_rope_tables_host((int)pl[6], c.head_size, pf[0], cs.data(), sn.data());
+    if (cudaMalloc(&p.cos_t, n * 4) != cudaSuccess || cudaMalloc(&p.sin_t, n * 4) != cudaSuccess) { cudaGetLastError(); p.release(); return ERROR_MEMORY_OUT; }
+    cudaMemcpy(p.cos_t, cs.data(), n * 4, cudaMemcpyHostToDevice);
+    cudaMemcpy(p.sin_t, sn.data(), n * 4, cudaMemcpyHostToDevice);
+    p.rotation.cos_table = p.cos_t; p.rotation.sin_table = p.sin_t; p.rotation.table_len = (int)pl[6];
+  }
+  const long h = k->next_handle++;
+  k->paged[h] = p;
+  return set_out((float)h, plOutput, ppOutput);
+}
+
+long paged_free(Kernel* k, long lInput, float* pf) {
+  long e;
+  if ((e = verify_in(lInput, pf, 1, 1))) return e;
+  auto it = k->paged.find((long)pf[0]);
+  if (it == k->paged.end()) return ERROR_PARAM_OUT_OF_RANGE;
+  cudaStreamSynchronize(0);
+  it->second.release();
+  k->paged.erase(it);
+  return 0;
+}
+
+// The status words after the stream has been waited for.
+long paged_status(Kernel* k) {
+  if (!may_have_failed(k, MCA_FAIL_PAGED)) return 0;
+  lower_fail_word(k, MCA_FAIL_PAGED);
+  int st[4] = {0, 0, 0, 0};
+  const long e = mca_paged_status(st);
+  if (e || st[0] == 0) return e;
+  static const char* const what[5] = {"", "sequence with bad lengths", "page id outside the pool or page not held: sequence", "position outside the tables: token row",
+                                      "bounded wait gave up at stage"};
+  char buf[128];
+  snprintf(buf, sizeof(buf), "%s %d (%d), %d refused", what[st[0] > 4 ? 0 : st[0]], st[1], st[2], st[3]);
+  k->last_detail = buf;
+  return st[0] == 4 ? ERROR_ATTN_KERNEL_TIMEOUT : ERROR_PARAM_OUT_OF_RANGE;
+}
+long paged_result(Kernel* k, long e) {
+  if (e) return e;
+  if (k->async) { k->paged_pending = true; return 0; }
+  if ((e = sync_call(k))) return e;
+  return paged_status(k);
+}
+
+// What APPEND and ATTN share: the handle, its pages, and the batch {hStarts,hLengths,hTable,tableStride,nSeqs,nTokens,maxNew,maxLen} at `b`.
+long paged_batch(Kernel* k, MCA_LONGLONG hPaged, MCA_LONGLONG hK, MCA_LONGLONG hV, const MCA_LONGLONG* b, PagedHandle** out, McaPagedCache* cache,
+                 McaPagedBatch* batch) {
+  long e;
+  auto it = k->paged.find((long)hPaged);
+  if (it == k->paged.end()) return ERROR_PARAM_OUT_OF_RANGE;
+  if (!in_range(b + 3, 2, 1) || !in_range(b + 5, 1, 0) || !in_range(b + 6, 2, 1)) return ERROR_PARAM_OUT_OF_RANGE;
+  *out = &it->second;
+  *cache = it->second.cache;
+  const int64_t n = (int64_t)cache->n_pages * cache->page_stride;
+  const bool bf16 = cache->dtype == MCA_DTYPE_BF16;
+  if ((e = check_any(k, (long)hK, n, bf16, &cache->k_pages)) || (e = check_any(k, (long)hV, n, bf16, &cache->v_pages))) return e;
+  float *starts, *lengths, *table;   // int32 values in 4-byte elements, as DECODE_STEP's positions
+  if ((e = check_f32(k, (long)b[0], b[4] + 1, &starts)) || (e = check_f32(k, (long)b[1], b[4], &lengths)) || (e = check_f32(k, (long)b[2], b[3] * b[4], &table))) return e;
+  *batch = McaPagedBatch{(const int*)starts, (const int*)lengths, (const int*)table, (int)b[3], (int)b[4], (int)b[5], (int)b[6], (int)b[7]};
+  return 0;
+}
+
+long paged_append(Kernel* k, long llInput, MCA_LONGLONG* pl) {
+  long e;  // longs {hPaged,hQ,hK,hV,hWq,hWk,hKpages,hVpages,hStarts,hLengths,hTable,tableStride,nSeqs,nTokens,maxNew,maxLen,hQout}
+  if ((e = verify_in(llInput, pl, 17, 17))) return e;
+  PagedHandle* p;
+  McaPagedCache c;
+  McaPagedBatch b;
+  if ((e = paged_batch(k, pl[0], pl[6], pl[7], pl + 8, &p, &c, &b))) return e;
+  McaQkRotation r = p->rotation;
+  float* w[2] = {nullptr, nullptr};
+  for (int i = 0; i < 2; ++i)
+    if (pl[4 + i] != 0 && (e = check_f32(k, (long)pl[4 + i], c.head_size, &w[i]))) return e;
+  r.q_weight = w[0]; r.k_weight = w[1];
+  int bf16 = -1;
+  const int64_t qn = (int64_t)c.n_heads * c.head_size, kn = (int64_t)c.n_kv_heads * c.head_size;
+  McaHeads q{nullptr, 0, qn, c.head_size}, kk{nullptr, 0, kn, c.head_size}, v = kk, qo = q;
+  if ((e = check_activations(k, (long)pl[1], b.n_tokens * qn, &bf16, &q.data)) || (e = check_activations(k, (long)pl[2], b.n_tokens * kn, &bf16, &kk.data)) ||
+      (e = check_activations(k, (long)pl[3], b.n_tokens * kn, &bf16, &v.data)) || (e = check_activations(k, (long)pl[16], b.n_tokens * qn, &bf16, &qo.data)))
+    return e;
+  return paged_result(k, mca_paged_append(&c, &b, &r, bf16 ? MCA_DTYPE_BF16 : MCA_DTYPE_F32, &q, &kk, &v, &qo, 0));
+}
+
+long paged_attn(Kernel* k, long llInput, MCA_LONGLONG* pl) {
+  long e;  // longs {hPaged,hQ,hKpages,hVpages,hStarts,hLengths,hTable,tableStride,nSeqs,nTokens,maxNew,maxLen,hOut}
+  if ((e = verify_in(llInput, pl, 13, 13))) return e;
+  PagedHandle* p;
+  McaPagedCache c;
+  McaPagedBatch b;
+  if ((e = paged_batch(k, pl[0], pl[2], pl[3], pl + 4, &p, &c, &b))) return e;
+  int bf16 = -1;
+  const int64_t qn = (int64_t)c.n_heads * c.head_size;
+  McaHeads q{nullptr, 0, qn, c.head_size}, out = q;
+  if ((e = check_activations(k, (long)pl[1], b.n_tokens * qn, &bf16, &q.data)) || (e = check_activations(k, (long)pl[12], b.n_tokens * qn, &bf16, &out.data))) return e;
+  const int dtype = bf16 ? MCA_DTYPE_BF16 : MCA_DTYPE_F32;
+  const int64_t need = mca_paged_attention_workspace_bytes(&c, &b, dtype);
+  if (need > p->work_bytes) {
+    cudaFree(p->work);
+    p->work = nullptr; p->work_bytes = 0;
+    if (cudaMalloc(&p->work, (size_t)need) != cudaSuccess) { cudaGetLastError(); return ERROR_MEMORY_OUT; }
+    p->work_bytes = need;
+  }
+  return paged_result(k, mca_paged_attention(&c, &b, dtype, &q, 0.f, &out, p->work, p->work_bytes, 0));   // where need is -1 it says why
+}
+
 long tft_fwd(Kernel* k, long llInput, MCA_LONGLONG* pl) {
   long e;
   if ((e = verify_in(llInput, pl, 11, 11))) return e;
@@ -1402,6 +1614,7 @@ void kernel_cleanup(long idx) {
   for (auto& kv : k->layernorm) cudaFree(kv.second.stdev);
   cudaFree(k->norm_scratch);
   for (auto& kv : k->decode) { cudaFree(kv.second.fr); cudaFree(kv.second.fi); cudaFree(kv.second.scratch); }
+  for (auto& kv : k->paged) kv.second.release();
   for (void* p : k->host_bufs) cudaFreeHost(p);
   if (k->h_answer) cudaFreeHost(k->h_answer);
   for (auto& kv : k->extensions) if (kv.second.lib) dlclose(kv.second.lib);
@@ -1484,6 +1697,12 @@ long run(Kernel* k, long fn, float* pf, long lInput, MCA_LONGLONG* pl, long llIn
     case MCA_FN_DECODE_OUT: return finish(k, decode_out(k, llInput, pl));
     case MCA_FN_DECODE_FFN: return finish(k, decode_ffn(k, lInput, pf, llInput, pl));
     case MCA_FN_DECODE_LOGITS: return finish(k, decode_logits(k, lInput, pf, llInput, pl));
+    case MCA_FN_QK_NORM_ROPE_FWD: return finish(k, qk_norm_rope_run(k, lInput, pf, llInput, pl, false));
+    case MCA_FN_QK_NORM_ROPE_BWD: return finish(k, qk_norm_rope_run(k, lInput, pf, llInput, pl, true));
+    case MCA_FN_PAGED_CREATE: return paged_create(k, lInput, pf, llInput, pl, plOutput, ppOutput);
+    case MCA_FN_PAGED_FREE: return paged_free(k, lInput, pf);
+    case MCA_FN_PAGED_APPEND: return finish(k, paged_append(k, llInput, pl));
+    case MCA_FN_PAGED_ATTN: return finish(k, paged_attn(k, llInput, pl));
     case MCA_FN_TFT_ATTN_FWD: return finish(k, tft_fwd(k, llInput, pl));
     case MCA_FN_TFT_ATTN_BWD: return finish(k, tft_bwd(k, llInput, pl));
     case MCA_FN_ATTN_FWD_HOST:

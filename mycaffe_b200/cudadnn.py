@@ -315,6 +315,35 @@ class CudaDnn:
     def RopeBackward(self, hRope, n, hX, hYdiff, hXdiff):
         self._call(ids.CUDA_FN_ROPE_BWD, [hRope, n, hX, hYdiff, hXdiff])
 
+    # ------------------------------------------------------------------ extensions: per-head norm with rotation, paged cache
+    def QkNormRopeForward(self, hRope, hQ, hK, hWq, hWk, nBatch, nSeqLen, nHeads, nKvHeads, nSize, hQout, hKout, fEps=1e-5,
+                          nFlags=ids.MCA_QK_NORM):
+        """y = rotate(w * x / rms(x)) for every query and key head of (B,T,heads,size) tensors; hRope 0: no rotation."""
+        self._call(ids.MCA_FN_QK_NORM_ROPE_FWD, [hRope, hQ, hK, hWq, hWk, nFlags, nBatch, nSeqLen, nHeads, nKvHeads, nSize, hQout, hKout],
+                   [float(fEps)])
+
+    def QkNormRopeBackward(self, hRope, hQ, hK, hWq, hWk, nBatch, nSeqLen, nHeads, nKvHeads, nSize, hdQout, hdKout, hdQ, hdK, hdWq=0, hdWk=0,
+                           fEps=1e-5, nFlags=ids.MCA_QK_NORM):
+        self._call(ids.MCA_FN_QK_NORM_ROPE_BWD, [hRope, hQ, hK, hWq, hWk, nFlags, nBatch, nSeqLen, nHeads, nKvHeads, nSize, hdQout, hdKout, hdQ,
+                                                 hdK, hdWq, hdWk], [float(fEps)])
+
+    def CreatePaged(self, nPages, nPageSize, nHeads, nKvHeads, nHeadSize, bCacheBf16=False, nTableLen=0, fTheta=0.0, nFlags=0, fEps=1e-5) -> int:
+        """A paged key/value cache of one layer; its pages live in two memory handles of nPages * nPageSize * nKvHeads * nHeadSize elements."""
+        return int(self._invoke(ids.MCA_FN_PAGED_CREATE, [float(fTheta), float(fEps)],
+                                [nPages, nPageSize, nHeads, nKvHeads, nHeadSize, 1 if bCacheBf16 else 0, nTableLen, nFlags])[0])
+
+    def FreePaged(self, h):
+        self._invoke(ids.MCA_FN_PAGED_FREE, [float(h)])
+
+    def PagedAppend(self, hPaged, hQ, hK, hV, hWq, hWk, hKpages, hVpages, hStarts, hLengths, hTable, nTableStride, nSeqs, nTokens, nMaxNew,
+                    nMaxLen, hQout):
+        self._call(ids.MCA_FN_PAGED_APPEND, [hPaged, hQ, hK, hV, hWq, hWk, hKpages, hVpages, hStarts, hLengths, hTable, nTableStride, nSeqs,
+                                             nTokens, nMaxNew, nMaxLen, hQout])
+
+    def PagedAttention(self, hPaged, hQ, hKpages, hVpages, hStarts, hLengths, hTable, nTableStride, nSeqs, nTokens, nMaxNew, nMaxLen, hOut):
+        self._call(ids.MCA_FN_PAGED_ATTN, [hPaged, hQ, hKpages, hVpages, hStarts, hLengths, hTable, nTableStride, nSeqs, nTokens, nMaxNew,
+                                           nMaxLen, hOut])
+
     # ------------------------------------------------------------------ extensions: decode, TFT
     def CreateDecode(self, nBatch, nHeads, nKvHeads, nHeadSize, nSeqLen, bCacheBf16=False, fTheta=10000.0) -> int:
         return int(self._invoke(ids.MCA_FN_DECODE_CREATE, [float(fTheta)],

@@ -18,8 +18,6 @@ import torch
 from . import _lib
 from . import function_ids as ids
 
-MCA_QK_NORM, MCA_ROPE_HALVES = 1, 2
-
 
 class McaHeads(C.Structure):
     _fields_ = [("data", C.c_void_p), ("stride_b", C.c_int64), ("stride_t", C.c_int64), ("stride_h", C.c_int64)]
@@ -123,7 +121,7 @@ class QkNormRope:
         self.weights = (q_weight is not None, k_weight is not None)
         self.c = McaQkRotation(_vector(q_weight, "q_weight", self.head_size, self.device), _vector(k_weight, "k_weight", self.head_size, self.device),
                                None if cos is None else _vector(cos, "cos", cos.numel(), self.device), None if sin is None else sin.data_ptr(),
-                               0 if cos is None else cos.shape[0], (MCA_QK_NORM if norm else 0) | (MCA_ROPE_HALVES if halves else 0), float(eps))
+                               0 if cos is None else cos.shape[0], (ids.MCA_QK_NORM if norm else 0) | (ids.MCA_ROPE_HALVES if halves else 0), float(eps))
 
     def check(self, head_size, device):
         if self.head_size not in (None, head_size):

@@ -230,3 +230,89 @@ def test_fp32_tiles(hs):
     s = setup([(31, 31), (33, 700), (64, 64), (9, 2100), (100, 130)], 6, 2, hs, 16, "f32", "f32", seed=18, drop=[(1, 0), (1, 5), (3, 100)])
     s.cache.attend(s.batch, s.q, s.out)
     s.check()
+
+
+@pytest.mark.parametrize("bf16", [False, True])
+def test_function_ids(bf16):
+    """Append and attention, and the norm with its backward, through handles and function ids as a MyCaffe layer calls them."""
+    import numpy as np
+    from mycaffe_b200 import CudaDnn, function_ids as ids, paged
+    from mycaffe_b200.cudadnn import CudaDnnError
+    rng = np.random.default_rng(0)
+    cuda = CudaDnn(0)
+    new = cuda.AllocMemoryBf16 if bf16 else cuda.AllocMemory
+    H, KV, D, page, seqs = 4, 2, 64, 16, [(1, 1), (20, 50), (1, 40)]
+    need = [-(-n // page) for _, n in seqs]
+    pages, T = sum(need), sum(n for n, _ in seqs)
+    table = np.full((3, 4), -1, np.int32)
+    order = rng.permutation(pages)
+    for b, n in enumerate(need):
+        table[b, :n] = order[sum(need[:b]):sum(need[:b]) + n]
+    ints = {}
+    for name, a in dict(starts=np.cumsum([0] + [n for n, _ in seqs]), lengths=[n for _, n in seqs], table=table).items():
+        a = np.ascontiguousarray(a, np.int32)
+        ints[name] = cuda.AllocMemory(a.size)
+        cuda.SetMemoryInt32(ints[name], a.reshape(-1))
+    w = 1 + 0.2 * rng.standard_normal(D).astype(np.float32)
+    hw = cuda.AllocMemory(w)
+    kv0 = [rng.standard_normal((pages, page, KV, D)).astype(np.float32) for _ in range(2)]
+    hK, hV = new(kv0[0]), new(kv0[1])
+    q, k, v = (rng.standard_normal((T, h, D)).astype(np.float32) for h in (H, KV, KV))
+    hq, hk, hv, hqo, ho = new(q), new(k), new(v), new(q.size), new(q.size)
+    hP = cuda.CreatePaged(pages, page, H, KV, D, bf16, 64, 10000.0, ids.MCA_QK_NORM | ids.MCA_ROPE_HALVES)
+    args = (hK, hV, ints["starts"], ints["lengths"], ints["table"], 4, 3, T, 20, 50)
+    cuda.PagedAppend(hP, hq, hk, hv, hw, hw, *args, hqo)
+    cuda.PagedAttention(hP, hqo, *args, ho)
+    # the same through the tensors' own calls
+    dt = torch.bfloat16 if bf16 else torch.float32
+    t = lambda a: torch.tensor(a, device="cuda").to(dt)
+    kt, vt = t(kv0[0]), t(kv0[1])
+    inv = 10000.0 ** (-np.arange(0, D, 2) / D)
+    ang = torch.tensor(np.arange(64)[:, None] * inv[None], device="cuda")
+    rot = paged.QkNormRope(ang.cos().float(), ang.sin().float(), torch.tensor(w, device="cuda"), torch.tensor(w, device="cuda"), halves=True)
+    cache = paged.PagedCache(kt, vt, H)
+    i = lambda a: torch.tensor(np.ascontiguousarray(a, np.int32), device="cuda")
+    b = cache.batch(i(np.cumsum([0] + [n for n, _ in seqs])), i([n for _, n in seqs]), i(table), T, 20, 50)
+    qo, out = torch.empty(T, H, D, device="cuda", dtype=dt), torch.empty(T, H, D, device="cuda", dtype=dt)
+    cache.append(b, rot, t(q), t(k), t(v), qo)
+    cache.attend(b, qo, out)
+    # the tables differ in their last bits (powf, cosf in fp32 at the library's host): 1e-5 of unit-sized values, or one step of bf16
+    tol = 2.0 ** -7 if bf16 else 1e-4
+    for h, ref in ((hqo, qo), (hK, kt), (hV, vt), (ho, out)):
+        got = cuda.GetMemory(h, ref.numel()).reshape(ref.shape)
+        ref = ref.float().cpu().numpy()
+        assert np.abs(got - ref).max() <= tol * np.abs(ref).max()
+    # a refused sequence comes back as an error, with its number
+    cuda.SetMemoryInt32(ints["lengths"], np.array([1, 5, 40], np.int32))
+    with pytest.raises(CudaDnnError) as err:
+        cuda.PagedAttention(hP, hqo, *args, ho)
+    assert err.value.code == ids.ERROR_PARAM_OUT_OF_RANGE and "1 (5)" in err.value.native_message
+    cuda.SetAsync(True)
+    cuda.PagedAttention(hP, hqo, *args, ho)
+    with pytest.raises(CudaDnnError):
+        cuda.SynchronizeDevice()
+    cuda.SetAsync(False)
+    with pytest.raises(CudaDnnError):
+        cuda.PagedAttention(hP + 100, hqo, *args, ho)
+    with pytest.raises(CudaDnnError):
+        cuda.PagedAttention(hP, cuda.AllocMemory(q.size - 4), *args, ho)
+    # training form
+    B, S = 2, 16
+    x = [rng.standard_normal((B, S, h, D)).astype(np.float32) for h in (H, KV, H, KV)]
+    hx = [new(a) for a in x]
+    hR = cuda.CreateRope(0, 0, x[0].size, B, S, H, D)
+    hy, hd = [new(a.size) for a in x[:2]], [new(a.size) for a in x[:2]]
+    hdw = [cuda.AllocMemory(D) for _ in range(2)]
+    cuda.QkNormRopeForward(hR, hx[0], hx[1], hw, hw, B, S, H, KV, D, *hy)
+    cuda.QkNormRopeBackward(hR, hx[0], hx[1], hw, hw, B, S, H, KV, D, hx[2], hx[3], *hd, *hdw)
+    tx = [t(a) for a in x]
+    rot = paged.QkNormRope(ang.cos().float(), ang.sin().float(), torch.tensor(w, device="cuda"), torch.tensor(w, device="cuda"))
+    y, d = [torch.empty_like(a) for a in tx[:2]], [torch.empty_like(a) for a in tx[:2]]
+    rot.forward(tx[0], tx[1], *y)
+    dw = rot.backward(*tx, *d)
+    for h, ref in zip(hy + hd + hdw, y + d + list(dw)):
+        got = cuda.GetMemory(h, ref.numel()).reshape(ref.shape)
+        ref = ref.float().cpu().numpy()
+        assert np.abs(got - ref).max() <= tol * np.abs(ref).max()
+    cuda.FreePaged(hP)
+    cuda.Dispose()
