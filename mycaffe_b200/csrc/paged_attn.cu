@@ -1062,14 +1062,16 @@ __global__ void __launch_bounds__(TC_THREADS, (TcPlan<HDP, FEW>::CTAS)) paged_tc
           float m_used[2] = {-INFINITY, -INFINITY}, l[2] = {0.f, 0.f};
           for (int j = 0; j < g.n; ++j, ++c) {
             const uint32_t t_s = t_row + (FEW ? (uint32_t)(c & 1) * 128u : 0u);
+            ok = __all_sync(0xffffffffu, mbar_wait(bar(TB_S + (FEW ? c & 1 : 0)), (uint32_t)((FEW ? c >> 1 : c) & 1), status, 30, c));
+            if (!ok) break;
             const int key0 = g.k_begin + j * KEYS;
-            if (key0 + KEYS - 1 > g.pos) {   // g.pos: the last key the tile's first row sees.  (Here, while there are registers for it)
+            // g.pos: the last key the tile's first row sees.  Here, while there are registers for it, and not before S is there: with one stage,
+            // S says that the values before these have arrived and been used, so that the parity waited for is these values' own
+            if (key0 + KEYS - 1 > g.pos) {
               ok = __all_sync(0xffffffffu, mbar_wait(bar(TB_VF + c % STG), (uint32_t)((c / STG) & 1), status, 31, c));
               if (!ok) break;
               if (clear_odd<HDP>(smem_base + PL::OFF_V + (c % STG) * PL::TILE_BYTES, max(g.pos + 1 - key0, 0), g.last + 1 - key0, rank * 32 + lane, p.warps * 32)) *s_odd = item + 1;
             }
-            ok = __all_sync(0xffffffffu, mbar_wait(bar(TB_S + (FEW ? c & 1 : 0)), (uint32_t)((FEW ? c >> 1 : c) & 1), status, 30, c));
-            if (!ok) break;
             tc_fence_after();
             // s[4g + 2h + e] = logit of row r0 + 8h, key 8g + 2 quad + e
             uint32_t s[64];

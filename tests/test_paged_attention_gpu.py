@@ -316,3 +316,19 @@ def test_function_ids(bf16):
         assert np.abs(got - ref).max() <= tol * np.abs(ref).max()
     cuda.FreePaged(hP)
     cuda.Dispose()
+
+
+@pytest.mark.parametrize("hs,page", [(128, 16), (128, 128), (64, 32)])
+def test_long_mixed_step_runs_alike(hs, page):
+    """Chunks among single tokens over long caches, in which values arrive late: right, and the same bits each time."""
+    s = setup([(300, 3300), (219, 2500)] + [(1, 3000 - 190 * b) for b in range(12)], 32, 8, hs, page, "bf16", "bf16", seed=19)
+    flush = torch.empty(1 << 28, dtype=torch.uint8, device="cuda")
+    first = None
+    for _ in range(12):
+        flush.zero_()                                  # the pages come from memory, not from the cache
+        s.out.fill_(7.0)
+        s.cache.attend(s.batch, s.q, s.out)
+        first = s.out.clone() if first is None else first
+        assert torch.equal(first, s.out)
+    s.check()
+    assert s.cache.status() == (0, 0, 0, 0)
