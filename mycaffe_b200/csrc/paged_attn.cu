@@ -41,6 +41,7 @@ struct AttnArgs {
   // tensor-core kernel
   int tile_shift, parts, items;    // log2 of the tokens of a tile; tiles that share a token's group of heads; parts x key/value heads
   int ctas, least_units, warps, rows_max;
+  int row_shift;            // the join's: log2 of the rows' threads
   int span, inner;          // CTAs that share the work of `inner` heads: all of both, or ctas / items and one
   int4* meta;               // (ctas, 2): the item that ends in a CTA and began in another: {that CTA or -1, token row, head, rows}, {heads}
 };
@@ -1288,42 +1289,55 @@ __global__ void __launch_bounds__(TC_THREADS, (TcPlan<HDP, FEW>::CTAS)) paged_tc
 }
 
 // Join of the items that several CTAs worked on: out = sum_s 2^(m_s - M) acc_s / sum_s 2^(m_s - M) l_s over their parts, in the order
-// of the CTAs.  Block x is the CTA where an item ended; a thread takes four elements of a row, the lanes of a warp neighbouring rows,
-// as the parts lie.
+// of the CTAs.  Block x is the CTA where an item ended; 2^row_shift neighbouring threads take its rows, as the parts lie, and each
+// JOIN_QUADS pieces of four elements.
+constexpr int JOIN_QUADS = 4;
 template <typename T>
 __global__ void __launch_bounds__(256) paged_join_kernel(const AttnArgs p) {
   mca_pdl_launch_dependents();
   mca_pdl_wait();
   const int4 m0 = __ldcg(p.meta + 2 * blockIdx.x);
   const int heads = __ldcg(p.meta + 2 * blockIdx.x + 1).x;
-  if (m0.x < 0) return;
-  const int first = m0.x, n = (int)blockIdx.x - first + 1, rows = m0.w, quads = p.hs / 4;
-  const float2* ml = reinterpret_cast<const float2*>(p.part_ml);
-  const float4* acc = reinterpret_cast<const float4*>(p.part_acc);
-  for (int i = blockIdx.y * 256 + threadIdx.x; i < rows * quads; i += gridDim.y * 256) {
-    const int col = i / rows, r = i - col * rows;
-    auto slot = [&](int k) { return 2ll * (first + k) + (k == 0 ? 1 : 0); };   // the first CTA's last part, then the others' first ones
-    float M = -INFINITY;
+  const int r = threadIdx.x & ((1 << p.row_shift) - 1), lanes = 256 >> p.row_shift, quads = p.hs / 4;
+  const int q0 = blockIdx.y * lanes * JOIN_QUADS + (threadIdx.x >> p.row_shift);
+  if (m0.x < 0 || r >= m0.w || q0 >= quads) return;
+  const int first = m0.x, n = (int)blockIdx.x - first + 1;
+  auto slot = [&](int k) { return 2ll * (first + k) + (k == 0 ? 1 : 0); };   // the first CTA's last part, then the others' first ones
+  const float2* ml = reinterpret_cast<const float2*>(p.part_ml) + r;
+  const float4* acc = reinterpret_cast<const float4*>(p.part_acc) + r;
+  float M = -INFINITY;
 #pragma unroll 4
-    for (int k = 0; k < n; ++k) {
-      const float2 v = ml[slot(k) * p.rows_max + r];
-      if (v.y != 0.f) M = fmaxf(M, v.x);
+  for (int k = 0; k < n; ++k) {
+    const float2 v = ml[slot(k) * p.rows_max];
+    if (v.y != 0.f) M = fmaxf(M, v.x);
+  }
+  float sum = 0.f;
+  float4 a[JOIN_QUADS];
+#pragma unroll
+  for (int i = 0; i < JOIN_QUADS; ++i) a[i] = make_float4(0.f, 0.f, 0.f, 0.f);
+#pragma unroll 2
+  for (int k = 0; k < n; ++k) {
+    const float2 v = ml[slot(k) * p.rows_max];
+    float4 x[JOIN_QUADS];
+#pragma unroll
+    for (int i = 0; i < JOIN_QUADS; ++i)
+      if (q0 + i * lanes < quads) x[i] = acc[(slot(k) * quads + q0 + i * lanes) * p.rows_max];
+    const float f = v.y == 0.f ? 0.f : fast_exp2(v.x - M);
+    sum = fmaf(v.y, f, sum);
+#pragma unroll
+    for (int i = 0; i < JOIN_QUADS; ++i) {
+      a[i].x = fmaf(x[i].x, f, a[i].x); a[i].y = fmaf(x[i].y, f, a[i].y); a[i].z = fmaf(x[i].z, f, a[i].z); a[i].w = fmaf(x[i].w, f, a[i].w);
     }
-    float sum = 0.f;
-    float4 a = make_float4(0.f, 0.f, 0.f, 0.f);
-#pragma unroll 4
-    for (int k = 0; k < n; ++k) {
-      const float2 v = ml[slot(k) * p.rows_max + r];
-      const float4 x = acc[(slot(k) * quads + col) * p.rows_max + r];
-      const float f = v.y == 0.f ? 0.f : fast_exp2(v.x - M);
-      sum = fmaf(v.y, f, sum);
-      a.x = fmaf(x.x, f, a.x); a.y = fmaf(x.y, f, a.y); a.z = fmaf(x.z, f, a.z); a.w = fmaf(x.w, f, a.w);
-    }
-    const float inv = sum == 0.f ? 0.f : 1.f / sum;
-    const int t = r / heads;
-    char* dst = p.out + (int64_t)(m0.y + t) * p.out_st + (m0.z + r - t * heads) * p.out_sh;
-    if constexpr (sizeof(T) == 4) reinterpret_cast<float4*>(dst)[col] = make_float4(a.x * inv, a.y * inv, a.z * inv, a.w * inv);
-    else reinterpret_cast<uint2*>(dst)[col] = make_uint2(pack_bf16(a.x * inv, a.y * inv), pack_bf16(a.z * inv, a.w * inv));
+  }
+  const float inv = sum == 0.f ? 0.f : 1.f / sum;
+  const int t = r / heads;
+  char* dst = p.out + (int64_t)(m0.y + t) * p.out_st + (m0.z + r - t * heads) * p.out_sh;
+#pragma unroll
+  for (int i = 0; i < JOIN_QUADS; ++i) {
+    const int q = q0 + i * lanes;
+    if (q >= quads) continue;
+    if constexpr (sizeof(T) == 4) reinterpret_cast<float4*>(dst)[q] = make_float4(a[i].x * inv, a[i].y * inv, a[i].z * inv, a[i].w * inv);
+    else reinterpret_cast<uint2*>(dst)[q] = make_uint2(pack_bf16(a[i].x * inv, a[i].y * inv), pack_bf16(a[i].z * inv, a[i].w * inv));
   }
 }
 
@@ -1488,6 +1502,8 @@ int mca_paged_attention(const McaPagedCache* cache, const McaPagedBatch* batch, 
   a.scale_log2 = (scale == 0.f ? 1.0f / sqrtf((float)D) : scale) * LOG2E;
   a.tile_shift = plan.tile_shift; a.parts = plan.parts; a.items = plan.parts * cache->n_kv_heads;
   a.ctas = plan.ctas; a.span = plan.span; a.inner = plan.inner; a.least_units = plan.least_units; a.warps = (plan.rows_max + 15) / 16; a.rows_max = plan.rows_max;
+  a.row_shift = 0;
+  while (1 << a.row_shift < plan.rows_max) ++a.row_shift;
   const int64_t slots = plan.tc ? 2ll * plan.ctas * plan.rows_max : (int64_t)batch->n_tokens * cache->n_heads * plan.nsplit;
   a.part_acc = plan.join ? static_cast<float*>(workspace) : nullptr;
   a.part_ml = plan.join ? a.part_acc + slots * D : nullptr;
@@ -1498,7 +1514,7 @@ int mca_paged_attention(const McaPagedCache* cache, const McaPagedBatch* batch, 
     if (f32) e = plan.few ? launch_tc<true, true>(cache, a, st) : launch_tc<true, false>(cache, a, st);
     else e = plan.few ? launch_tc<false, true>(cache, a, st) : launch_tc<false, false>(cache, a, st);
     if (e || !plan.join) return e;
-    const dim3 grid(plan.ctas, std::min(8, mca_ceil_div(plan.rows_max * D / 4, 512)));   // two pieces a thread
+    const dim3 grid(plan.ctas, mca_ceil_div(D / 4, (256 >> a.row_shift) * JOIN_QUADS));
     return f32 ? mca_launch_pdl(paged_join_kernel<float>, grid, dim3(256), 0, st, a) : mca_launch_pdl(paged_join_kernel<__nv_bfloat16>, grid, dim3(256), 0, st, a);
   }
   switch (D) {
