@@ -540,7 +540,7 @@ typedef struct McaPagedCache {
 } McaPagedCache;
 /* The new tokens of a step: those of sequence b are rows [starts[b], starts[b+1]) of the token tensors, the last of its
  * lengths[b] positions (so lengths counts them: token i of the sequence has position lengths[b] - (starts[b+1] - starts[b]) + i).
- * starts rises from 0 on; a sequence may have none.  Rows behind starts[n_seqs], up to n_tokens, are not read and not written.
+ * starts rises from 0 on; a sequence may have none (its length and pages are then not looked at).  Rows behind starts[n_seqs], up to n_tokens, are not read and not written.
  * starts, lengths and page_table are device memory; what the host knows of them is an upper bound: no sequence has more than max_new
  * new tokens or max_len positions (max_len <= table_stride * page_size).  A sequence outside these bounds, or with fewer positions
  * than new tokens, is refused on the device: nothing of it is read or stored, those of its rows that lie below n_tokens are zero, and

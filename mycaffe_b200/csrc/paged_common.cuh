@@ -46,7 +46,9 @@ __device__ __forceinline__ Sequence sequence(const Batch& t, int b) {
   s.start = t.starts[b];
   s.count = t.starts[b + 1] - s.start;
   s.length = t.lengths[b];
-  s.good = s.start >= 0 && s.count >= 0 && s.count <= t.max_new && s.start <= t.n_tokens - s.count && s.length >= s.count && s.length <= t.max_len;
+  // a sequence without new tokens may have any length: nothing of it is read
+  s.good = s.start >= 0 && s.count >= 0 && s.count <= t.max_new && s.start <= t.n_tokens - s.count &&
+           (s.count == 0 || (s.length >= s.count && s.length <= t.max_len));
   return s;
 }
 // The sequence a token row belongs to: the last one that starts at or before it; -1: none (a row behind the last sequence).

@@ -70,6 +70,10 @@ def test_padding_and_sequences_without_tokens(act, cache):
     s = setup([(0, 50), (3, 10), (0, 0), (1, 40), (0, 17)], 4, 4, 64, 16, act, cache, seed=6, pad=9, max_new=50, max_len=64)
     s.cache.attend(s.batch, s.q, s.out)
     s.check()                                   # rows behind the last sequence: still 7
+    s.lengths[0], s.lengths[2], s.lengths[4] = 1 << 20, -3, 0     # lengths of sequences without tokens are not looked at
+    s.out.fill_(7.0)
+    s.cache.attend(s.batch, s.q, s.out)
+    s.check()
     assert s.cache.status() == (0, 0, 0, 0)
 
 
