@@ -18,11 +18,13 @@ namespace {
 using paged::Batch;
 
 constexpr int THREADS = 256;
-constexpr int HEADS = 4;       // of one token that a group takes at once, forward
-constexpr int HEADS_BWD = 2;   // backward: two tensors to load
-// CTAs per SM that registers are left for: fp32 rows are four elements a piece and fit in 80, bf16 ones are eight; with 80 they spill
-// (2 x 4095 x (32 + 8) heads of 128, forward and backward: 91 us with two CTAs, 160 with three; fp32, 8 x 1024 x 24 of 64: 52 and 48).
-template <typename T> constexpr int CTAS = sizeof(T) == 4 ? 3 : 2;
+// Heads of one token that a group takes at once, forward and backward, and the CTAs per SM that registers are left for.  fp32 rows are four
+// elements a piece and gain from more warps (8 x 1024 x 24 heads of 64, forward and backward: 48.1 us with four and two heads and three CTAs,
+// 45.8 so); bf16 ones are eight, are bound by the instructions of a piece and spill in fewer registers (2 x 4095 x 40 heads of 128: 91 us,
+// with three CTAs 160, with pieces of four 112).
+template <typename T> constexpr int HEADS = sizeof(T) == 4 ? 2 : 4;
+template <typename T> constexpr int HEADS_BWD = sizeof(T) == 4 ? 1 : 2;
+template <typename T> constexpr int CTAS = sizeof(T) == 4 ? 4 : 2;
 constexpr int BWD_CTAS = 148 * 4;
 
 template <typename T> struct Piece;   // 16 bytes of a row
@@ -177,12 +179,26 @@ struct RotArgs {
   float eps;
 };
 
+// Quotients by a divisor of the launch, of numerators below 2^31, from its reciprocal scaled to 33 bits (T. Granlund and P. Montgomery,
+// "Division by invariant integers using multiplication", PLDI 1994): an integer division is some twenty instructions.
+struct Divisor {
+  uint32_t mul, shift;
+  __device__ __forceinline__ uint32_t operator()(uint32_t n) const { return (__umulhi(n, mul) + n) >> shift; }
+};
+inline Divisor divisor(int d) {
+  Divisor r{0, 0};
+  while ((1ll << r.shift) < d) ++r.shift;
+  r.mul = (uint32_t)(((1ull << 32) * ((1ull << r.shift) - (uint64_t)d)) / (uint64_t)d + 1);
+  return r;
+}
+
 struct NormArgs {
   RotArgs r;
   View x[2], out[2];        // queries, keys.  Backward: x and dx
   View g[2];                // backward: gradients of the outputs
   const int* positions;
   int B, T, heads[2], ctas_q;
+  Divisor by_chunks[2], by_t;
   float* partial;           // backward: (CTAs, D), or null
 };
 
@@ -203,7 +219,7 @@ __global__ void __launch_bounds__(THREADS, CTAS<T>) qk_norm_rope_kernel(const No
   const int gl = threadIdx.x % G, grp = threadIdx.x / G;
   const int half = p.r.D / 2;
   const bool in = gl * VEC < half;
-  const int heads = p.heads[kind], chunks = mca_ceil_div(heads, HEADS);
+  const int heads = p.heads[kind], chunks = mca_ceil_div(heads, HEADS<T>);
   const int64_t units = (int64_t)p.B * p.T * chunks;
   Part<VEC> w;
 #pragma unroll
@@ -214,16 +230,16 @@ __global__ void __launch_bounds__(THREADS, CTAS<T>) qk_norm_rope_kernel(const No
     const int64_t unit = u0 + grp;
     const bool live = unit < units;
     const uint32_t un = live ? (uint32_t)unit : 0u;
-    const uint32_t token = un / (uint32_t)chunks;
-    const int h0 = (int)(un - token * chunks) * HEADS;
-    const int b = (int)(token / (uint32_t)p.T), t = (int)(token - (uint32_t)b * p.T);
+    const uint32_t token = p.by_chunks[kind](un);
+    const int h0 = (int)(un - token * chunks) * HEADS<T>;
+    const int b = (int)p.by_t(token), t = (int)token - b * p.T;
     const bool mine = live && in;
     const int pos = p.positions != nullptr ? p.positions[token] : t;
     bool bad;   // a position that has no angles: zeros all the way
     const int64_t ar = angle_row(p.r, pos, &bad);
-    uint4 raw[HEADS][2];
+    uint4 raw[HEADS<T>][2];
 #pragma unroll
-    for (int i = 0; i < HEADS; ++i) {
+    for (int i = 0; i < HEADS<T>; ++i) {
       raw[i][0] = raw[i][1] = make_uint4(0, 0, 0, 0);
       if (mine && !bad && h0 + i < heads) {
         const char* row = at(p.x[kind], b, t, h0 + i);
@@ -241,7 +257,7 @@ __global__ void __launch_bounds__(THREADS, CTAS<T>) qk_norm_rope_kernel(const No
       if (bad && live && gl == 0 && h0 == 0 && kind == 0) paged::refuse(paged::REFUSED_POSITION, (int)token, pos);
     }
 #pragma unroll
-    for (int i = 0; i < HEADS; ++i) {
+    for (int i = 0; i < HEADS<T>; ++i) {
       Part<VEC> x;
       Piece<T>::unpack(raw[i][0], x.v);
       Piece<T>::unpack(raw[i][1], x.v + VEC);
@@ -268,7 +284,7 @@ __global__ void __launch_bounds__(THREADS, CTAS<T>) qk_norm_rope_bwd_kernel(cons
   const int gl = threadIdx.x % G, grp = threadIdx.x / G;
   const int half = p.r.D / 2;
   const bool in = gl * VEC < half;
-  const int heads = p.heads[kind], chunks = mca_ceil_div(heads, HEADS_BWD);
+  const int heads = p.heads[kind], chunks = mca_ceil_div(heads, HEADS_BWD<T>);
   const int64_t units = (int64_t)p.B * p.T * chunks;
   Part<VEC> w, dw;
 #pragma unroll
@@ -279,16 +295,16 @@ __global__ void __launch_bounds__(THREADS, CTAS<T>) qk_norm_rope_bwd_kernel(cons
     const int64_t unit = u0 + grp;
     const bool live = unit < units;
     const uint32_t un = live ? (uint32_t)unit : 0u;
-    const uint32_t token = un / (uint32_t)chunks;
-    const int h0 = (int)(un - token * chunks) * HEADS_BWD;
-    const int b = (int)(token / (uint32_t)p.T), t = (int)(token - (uint32_t)b * p.T);
+    const uint32_t token = p.by_chunks[kind](un);
+    const int h0 = (int)(un - token * chunks) * HEADS_BWD<T>;
+    const int b = (int)p.by_t(token), t = (int)token - b * p.T;
     const bool mine = live && in;
     const int pos = p.positions != nullptr ? p.positions[token] : t;
     bool bad;   // a position that has no angles: the forward's row is a constant zero
     const int64_t ar = angle_row(p.r, pos, &bad);
-    uint4 rg[HEADS_BWD][2], rx[HEADS_BWD][2];
+    uint4 rg[HEADS_BWD<T>][2], rx[HEADS_BWD<T>][2];
 #pragma unroll
-    for (int i = 0; i < HEADS_BWD; ++i) {
+    for (int i = 0; i < HEADS_BWD<T>; ++i) {
       rx[i][0] = rx[i][1] = rg[i][0] = rg[i][1] = make_uint4(0, 0, 0, 0);
       if (mine && !bad && h0 + i < heads) {
         const char* row = at(p.g[kind], b, t, h0 + i);
@@ -313,7 +329,7 @@ __global__ void __launch_bounds__(THREADS, CTAS<T>) qk_norm_rope_bwd_kernel(cons
       if (bad && live && gl == 0 && h0 == 0 && kind == 0) paged::refuse(paged::REFUSED_POSITION, (int)token, pos);
     }
 #pragma unroll
-    for (int i = 0; i < HEADS_BWD; ++i) {
+    for (int i = 0; i < HEADS_BWD<T>; ++i) {
       Part<VEC> g;
       Piece<T>::unpack(rg[i][0], g.v);
       Piece<T>::unpack(rg[i][1], g.v + VEC);
@@ -382,6 +398,7 @@ struct AppendArgs {
   char *k_pages, *v_pages;
   int64_t page_bytes, row_bytes, head_bytes;
   int heads[3], first_cta[4];   // queries, keys and values have CTAs of their own
+  Divisor by_chunks[3];
 };
 
 template <typename T, typename CT, int G, bool HALVES>
@@ -402,7 +419,7 @@ __global__ void __launch_bounds__(THREADS, CTAS<T>) paged_append_kernel(const Ap
   const int gl = threadIdx.x % G, grp = threadIdx.x / G;
   const int half = p.r.D / 2;
   const bool in = gl * VEC < half;
-  const int heads = p.heads[kind], chunks = mca_ceil_div(heads, HEADS);
+  const int heads = p.heads[kind], chunks = mca_ceil_div(heads, HEADS<T>);
   const int64_t units = (int64_t)p.batch.n_tokens * chunks;
   Part<VEC> w;
 #pragma unroll
@@ -414,8 +431,8 @@ __global__ void __launch_bounds__(THREADS, CTAS<T>) paged_append_kernel(const Ap
     const int64_t unit = u0 + grp;
     const bool live = unit < units;
     const uint32_t un = live ? (uint32_t)unit : 0u;
-    const int token = (int)(un / (uint32_t)chunks);
-    const int h0 = (int)(un - (uint32_t)token * chunks) * HEADS;
+    const int token = (int)p.by_chunks[kind](un);
+    const int h0 = (int)(un - (uint32_t)token * chunks) * HEADS<T>;
     const int b = live ? paged::sequence_of(p.batch, token) : -1;
     const bool reporter = gl == 0 && h0 == 0;
     bool mine = b >= 0 && in, zero = false;
@@ -425,9 +442,9 @@ __global__ void __launch_bounds__(THREADS, CTAS<T>) paged_append_kernel(const Ap
       pos = s.length - s.count + (token - s.start);
       zero = !s.good;
     }
-    uint4 raw[HEADS][2];
+    uint4 raw[HEADS<T>][2];
 #pragma unroll
-    for (int i = 0; i < HEADS; ++i) {
+    for (int i = 0; i < HEADS<T>; ++i) {
       raw[i][0] = raw[i][1] = make_uint4(0, 0, 0, 0);
       if (mine && !zero && h0 + i < heads) {
         const char* row = at(p.in[kind], 0, token, h0 + i);
@@ -461,7 +478,7 @@ __global__ void __launch_bounds__(THREADS, CTAS<T>) paged_append_kernel(const Ap
       }
     }
 #pragma unroll
-    for (int i = 0; i < HEADS; ++i) {
+    for (int i = 0; i < HEADS<T>; ++i) {
       Part<VEC> x;
       Piece<T>::unpack(raw[i][0], x.v);
       Piece<T>::unpack(raw[i][1], x.v + VEC);
@@ -512,7 +529,7 @@ int check_norm(const McaQkRotation* rotation, const McaHeads* const (&views)[6],
   int e = check_rotation(rotation, D, &a->r);
   if (e) return e;
   if (B <= 0 || T <= 0 || n_heads <= 0 || n_kv_heads < 0) return ERROR_PARAM_OUT_OF_RANGE;
-  if ((int64_t)B * T * mca_ceil_div(std::max(n_heads, n_kv_heads), HEADS_BWD) >= (1ll << 31)) return ERROR_PARAM_OUT_OF_RANGE;
+  if ((int64_t)B * T * std::max(n_heads, n_kv_heads) >= (1ll << 31)) return ERROR_PARAM_OUT_OF_RANGE;
   if (rotation->cos_table && !positions && T > rotation->table_len) return ERROR_PARAM_OUT_OF_RANGE;
   if ((uintptr_t)positions & 3) return ERROR_PARAM_OUT_OF_RANGE;
   for (int i = 0; i < n_views; ++i) {
@@ -527,6 +544,7 @@ int check_norm(const McaQkRotation* rotation, const McaHeads* const (&views)[6],
     a->g[i] = n_views == 6 ? view(none ? nullptr : views[2 + i], size) : View{nullptr, 0, 0, 0};
   }
   a->positions = positions; a->B = B; a->T = T; a->heads[0] = n_heads; a->heads[1] = n_kv_heads; a->partial = nullptr;
+  a->by_t = divisor(T);
   return 0;
 }
 
@@ -534,8 +552,9 @@ template <typename T, int G>
 int launch_forward(NormArgs& a, bool halves, cudaStream_t st) {
   constexpr int GROUPS = THREADS / G, MOST = 148 * 16;
   const int64_t tokens = (int64_t)a.B * a.T;
-  a.ctas_q = ctas_for(tokens * mca_ceil_div(a.heads[0], HEADS), GROUPS, MOST);
-  const int ctas_k = a.heads[1] ? ctas_for(tokens * mca_ceil_div(a.heads[1], HEADS), GROUPS, MOST) : 0;
+  for (int i = 0; i < 2; ++i) a.by_chunks[i] = divisor(std::max(1, mca_ceil_div(a.heads[i], HEADS<T>)));
+  a.ctas_q = ctas_for(tokens * mca_ceil_div(a.heads[0], HEADS<T>), GROUPS, MOST);
+  const int ctas_k = a.heads[1] ? ctas_for(tokens * mca_ceil_div(a.heads[1], HEADS<T>), GROUPS, MOST) : 0;
   return mca_launch_pdl(halves ? qk_norm_rope_kernel<T, G, true> : qk_norm_rope_kernel<T, G, false>, dim3(a.ctas_q + ctas_k), dim3(THREADS), 0, st, a);
 }
 template <typename T, int G>
@@ -545,8 +564,9 @@ int launch_backward(NormArgs& a, bool halves, float* dwq, float* dwk, cudaStream
   const int all = a.heads[0] + a.heads[1];
   // the CTAs are shared between queries and keys by their heads
   const int most_q = a.heads[1] ? std::max(1, std::min(BWD_CTAS - 1, (int)((int64_t)BWD_CTAS * a.heads[0] / all))) : BWD_CTAS;
-  a.ctas_q = ctas_for(tokens * mca_ceil_div(a.heads[0], HEADS_BWD), GROUPS, most_q);
-  const int ctas_k = a.heads[1] ? ctas_for(tokens * mca_ceil_div(a.heads[1], HEADS_BWD), GROUPS, BWD_CTAS - most_q) : 0;
+  for (int i = 0; i < 2; ++i) a.by_chunks[i] = divisor(std::max(1, mca_ceil_div(a.heads[i], HEADS_BWD<T>)));
+  a.ctas_q = ctas_for(tokens * mca_ceil_div(a.heads[0], HEADS_BWD<T>), GROUPS, most_q);
+  const int ctas_k = a.heads[1] ? ctas_for(tokens * mca_ceil_div(a.heads[1], HEADS_BWD<T>), GROUPS, BWD_CTAS - most_q) : 0;
   int e = mca_launch_pdl(halves ? qk_norm_rope_bwd_kernel<T, G, true> : qk_norm_rope_bwd_kernel<T, G, false>, dim3(a.ctas_q + ctas_k), dim3(THREADS), 0, st, a);
   if (e || a.partial == nullptr) return e;
   return mca_launch_pdl(qk_norm_dw_kernel, dim3(2, mca_ceil_div(a.r.D, 32)), dim3(32, 32), 0, st, (const float*)a.partial, a.ctas_q + ctas_k, a.ctas_q,
@@ -556,8 +576,9 @@ template <typename T, typename CT, int G>
 int launch_append(AppendArgs& a, bool halves, cudaStream_t st) {
   constexpr int GROUPS = THREADS / G, MOST = 148 * 16;
   a.first_cta[0] = 0;
+  for (int i = 0; i < 3; ++i) a.by_chunks[i] = divisor(mca_ceil_div(a.heads[i], HEADS<T>));
   for (int i = 0; i < 3; ++i)
-    a.first_cta[i + 1] = a.first_cta[i] + ctas_for((int64_t)a.batch.n_tokens * mca_ceil_div(a.heads[i], HEADS), GROUPS, MOST);
+    a.first_cta[i + 1] = a.first_cta[i] + ctas_for((int64_t)a.batch.n_tokens * mca_ceil_div(a.heads[i], HEADS<T>), GROUPS, MOST);
   return mca_launch_pdl(halves ? paged_append_kernel<T, CT, G, true> : paged_append_kernel<T, CT, G, false>, dim3(a.first_cta[3] + 1), dim3(THREADS), 0, st, a);
 }
 
@@ -639,7 +660,7 @@ int mca_paged_append(const McaPagedCache* cache, const McaPagedBatch* batch, con
   if ((e = paged::check_heads(q, dtype, false)) || (e = paged::check_heads(k, dtype, false)) ||
       (e = paged::check_heads(v, dtype, false)) || (e = paged::check_heads(q_out, dtype, false)))
     return e;
-  if ((int64_t)batch->n_tokens * mca_ceil_div(cache->n_heads, HEADS) >= (1ll << 31)) return ERROR_PARAM_OUT_OF_RANGE;
+  if ((int64_t)batch->n_tokens * cache->n_heads >= (1ll << 31)) return ERROR_PARAM_OUT_OF_RANGE;
   const int size = dtype == MCA_DTYPE_BF16 ? 2 : 4, csize = cache->dtype == MCA_DTYPE_BF16 ? 2 : 4;
   a.in[0] = view(q, size); a.in[1] = view(k, size); a.in[2] = view(v, size); a.q_out = view(q_out, size);
   a.k_pages = static_cast<char*>(cache->k_pages); a.v_pages = static_cast<char*>(cache->v_pages);
