@@ -596,10 +596,13 @@ MCA_API int mca_paged_append(const McaPagedCache* cache, const McaPagedBatch* ba
                              const McaHeads* q, const McaHeads* k, const McaHeads* v, const McaHeads* q_out, void* stream);
 /* Attention of the new tokens over their sequences' pages, the new tokens' own keys among them (append first):
  * out_t = sum over j <= position(t) of softmax_j(scale q_t . k_j) v_j; scale 0: 1 / sqrt(head_size).  A token with no key left has a
- * zero row.  q, out (n_tokens, n_heads, D) in dtype: fp32 activations over an fp32 cache (exact fp32 products) or a bf16 one (exact fp32
- * where each key serves one query row of the call; else queries and probabilities as two bf16 halves, 3e-6 of the output in the 2-norm), or
- * bf16 over bf16 (probabilities rounded to bf16).  A value that is not finite reaches the tokens that see it and no others.  out must not overlap q or the pages.  workspace: mca_paged_attention_workspace_bytes bytes, 16-byte aligned (0: none is
- * needed; -1: arguments that mca_paged_attention refuses); two calls that may overlap, two captured graphs among them, need one each. */
+ * zero row; a value that is not finite reaches the tokens that see it and no others.  q, out (n_tokens, n_heads, D) in dtype:
+ *   fp32 over fp32 pages     exact fp32 products;
+ *   fp32 over bf16 pages     exact fp32 products where a key serves one query row of a sequence; else queries and probabilities as two
+ *                            bf16 halves each, 3e-6 of the output in the 2-norm;
+ *   bf16 over bf16 pages     probabilities rounded to bf16, sums in fp32.
+ * out must not overlap q or the pages.  workspace: mca_paged_attention_workspace_bytes bytes, 16-byte aligned (0: none is needed; -1:
+ * arguments that mca_paged_attention refuses); two calls that may overlap, two captured graphs among them, need one each. */
 MCA_API int64_t mca_paged_attention_workspace_bytes(const McaPagedCache* cache, const McaPagedBatch* batch, int dtype);
 MCA_API int mca_paged_attention(const McaPagedCache* cache, const McaPagedBatch* batch, int dtype, const McaHeads* q, float scale,
                                 const McaHeads* out, void* workspace, int64_t workspace_bytes, void* stream);
