@@ -336,3 +336,30 @@ def test_long_mixed_step_runs_alike(hs, page):
         assert torch.equal(first, s.out)
     s.check()
     assert s.cache.status() == (0, 0, 0, 0)
+
+
+@pytest.mark.parametrize("act,cache", TYPES)
+@pytest.mark.parametrize("new", [1, 40])
+def test_pages_beyond_32_bit_offsets(act, cache, new):
+    """The same pages at the end of a pool of more than 2^32 bytes give the same bits, through append and attention."""
+    from mycaffe_b200 import paged
+    s = setup([(new, 300), (1, 130)], 8, 4, 128, 256, act, cache, seed=20)
+    rot = paged.QkNormRope(None, None, norm=False)
+    k, v = (torch.randn(s.n_tokens, 4, 128, device="cuda").to(s.act) for _ in range(2))
+    n, size = s.k_pages.shape[0], s.k_pages.element_size() * s.k_pages[0].numel()
+    many = (1 << 32) // size + 64
+    big = [torch.empty((many,) + tuple(s.k_pages.shape[1:]), device="cuda", dtype=s.cache_t) for _ in range(2)]
+    for b, p in zip(big, (s.k_pages, s.v_pages)):
+        b[many - n:] = p
+    far = torch.where(s.table >= 0, s.table + (many - n), s.table).to(torch.int32).contiguous()
+    wide = paged.PagedCache(big[0], big[1], 8)
+    batch = wide.batch(s.starts, s.lengths, far, s.n_tokens, s.max_new, s.max_len)
+    q, out = torch.empty_like(s.q), torch.empty_like(s.out)
+    wide.append(batch, rot, s.q, k, v, q)
+    wide.attend(batch, q, out)
+    s.cache.append(s.batch, rot, s.q, k, v, q)
+    s.cache.attend(s.batch, q, s.out)
+    assert torch.equal(out, s.out) and torch.isfinite(out.float()).all()
+    assert wide.status() == (0, 0, 0, 0)
+    for b, p in zip(big, (s.k_pages, s.v_pages)):
+        assert torch.equal(b[many - n:].nan_to_num(9.0), p.nan_to_num(9.0))
