@@ -622,6 +622,11 @@ __device__ __forceinline__ int64_t key_tiles_of(int pos, int shift, int n) {
   return below(d + n) - below(d);
 }
 
+// a / b for a >= 0, b > 0: in 32 bits where both fit (a 64-bit division is some hundred instructions of one dependent chain).
+__device__ __forceinline__ int64_t quotient(int64_t a, int64_t b) {
+  return ((uint64_t)(a | b) >> 32) == 0 ? (int64_t)((uint32_t)a / (uint32_t)b) : a / b;
+}
+
 // The items in their order (sequences, their tiles of 2^tile_shift tokens, the heads of the CTA's span) and a CTA's share of their units;
 // all lanes of the walking warp hold the same.
 struct Walk {
@@ -651,12 +656,13 @@ struct Walk {
 
   __device__ __forceinline__ void begin(const AttnArgs& p, int cta) {
     const int lane = threadIdx.x & 31, n = p.batch.n_seqs;
-    int64_t total = 0;
-    for (int b = lane; b < n; b += 32) total += units_of(p, paged::sequence(p.batch, b));
+    const int64_t first = lane < n ? units_of(p, paged::sequence(p.batch, lane)) : 0;
+    int64_t total = first;
+    for (int b = lane + 32; b < n; b += 32) total += units_of(p, paged::sequence(p.batch, b));
 #pragma unroll
     for (int o = 16; o > 0; o >>= 1) total += __shfl_xor_sync(0xffffffffu, total, o);
     total *= p.inner;
-    share = max((total + p.span - 1) / p.span, (int64_t)p.least_units);
+    share = max(quotient(total + p.span - 1, p.span), (int64_t)p.least_units);
     head0 = p.inner == 1 ? cta / p.span : 0;
     first_cta = head0 * p.span;
     const int64_t lo = (int64_t)(cta - first_cta) * share;
@@ -665,7 +671,7 @@ struct Walk {
     if (left <= 0) return;
     int64_t before = 0;
     for (int s0 = 0; s0 < n; s0 += 32) {
-      const int64_t mine = s0 + lane < n ? units_of(p, paged::sequence(p.batch, s0 + lane)) * p.inner : 0;
+      const int64_t mine = (s0 == 0 ? first : (s0 + lane < n ? units_of(p, paged::sequence(p.batch, s0 + lane)) : 0)) * p.inner;
       int64_t incl = mine;
 #pragma unroll
       for (int o = 1; o < 32; o <<= 1) {
@@ -693,7 +699,7 @@ struct Walk {
     tile = a;
     const int64_t in = rel - units_of(p, pos0, tile) * p.inner;
     const int units = key_tiles(p) + ITEM_UNITS;
-    const int h = (int)(in / units);
+    const int h = (int)quotient(in, units);
     head = head0 + h;
     from = (int)(in - (int64_t)h * units);
     item_unit = lo - from;
@@ -877,7 +883,7 @@ __global__ void __launch_bounds__(TC_THREADS, (TcPlan<HDP, FEW>::CTAS)) paged_tc
         w.take(p, &kt0, &kt1);
         g = segment<R>(p, w, kt0, kt1);
         if (first && p.meta != nullptr && lane == 0 && g.n > 0 && kt0 > 0 && kt1 == w.key_tiles(p)) {   // what the join needs
-          p.meta[2 * blockIdx.x] = make_int4(w.first_cta + (int)((w.item_unit + ITEM_UNITS) / w.share), g.token0, g.head0, g.rows);
+          p.meta[2 * blockIdx.x] = make_int4(w.first_cta + (int)quotient(w.item_unit + ITEM_UNITS, w.share), g.token0, g.head0, g.rows);
           p.meta[2 * blockIdx.x + 1] = make_int4(g.heads, 0, 0, 0);
         }
         first = false;
