@@ -10,6 +10,7 @@
 //   paged_tile_kernel    fp32 pages, more rows: exact fp32 products on tiles in shared memory.
 //   paged_join_kernel, paged_simt_join_kernel   results of one row from several CTAs, each with some of the keys, joined by their maxima and sums.
 #include <algorithm>
+#include <cfloat>
 #include <cmath>
 #include <type_traits>
 
@@ -1142,8 +1143,7 @@ __global__ void __launch_bounds__(TC_THREADS, (TcPlan<HDP, FEW>::CTAS)) paged_tc
               for (int h = 0; h < 2; ++h) {
                 mx[h] = fmaxf(mx[h], __shfl_xor_sync(0xffffffffu, mx[h], 1));
                 mx[h] = fmaxf(mx[h], __shfl_xor_sync(0xffffffffu, mx[h], 2));
-                float m_new = mx[h] > m_used[h] + TC_RESCALE ? mx[h] : m_used[h];
-                if (m_new == -INFINITY) m_new = 0.f;   // no key seen yet
+                const float m_new = mx[h] > m_used[h] + TC_RESCALE ? mx[h] : m_used[h];   // minus infinity until the row sees a key
                 f[h] = m_new != m_used[h] ? fast_exp2(m_used[h] - m_new) : 1.0f;
                 l[h] *= f[h];
                 m_used[h] = m_new;
@@ -1166,8 +1166,10 @@ __global__ void __launch_bounds__(TC_THREADS, (TcPlan<HDP, FEW>::CTAS)) paged_tc
                 }
               }
             }
-            // p = 2^(s scale - m), handed over in three pieces (64, 32, 32 keys); the sum is of the unrounded ones
-            const float2 nm2[2] = {make_float2(-m_used[0], -m_used[0]), make_float2(-m_used[1], -m_used[1])};
+            // p = 2^(s scale - m), handed over in three pieces (64, 32, 32 keys); the sum is of the unrounded ones.  Of a row that has seen no
+            // key all s are minus infinity, and any finite m gives the zeros
+            const float nm[2] = {-fmaxf(m_used[0], -FLT_MAX), -fmaxf(m_used[1], -FLT_MAX)};
+            const float2 nm2[2] = {make_float2(nm[0], nm[0]), make_float2(nm[1], nm[1])};
             float2 rs[2] = {make_float2(0.f, 0.f), make_float2(0.f, 0.f)};
             auto quarter = [&](const int q) {
               uint32_t pk[8], pl[ACT32 ? 8 : 1];

@@ -363,3 +363,34 @@ def test_pages_beyond_32_bit_offsets(act, cache, new):
     assert wide.status() == (0, 0, 0, 0)
     for b, p in zip(big, (s.k_pages, s.v_pages)):
         assert torch.equal(b[many - n:].nan_to_num(9.0), p.nan_to_num(9.0))
+
+
+def far_below(s, level):
+    """Queries along one direction and keys against it: every scaled logit lies near `level`, far below zero."""
+    u = torch.randn(s.kv, s.hs, device="cuda").sign()
+    group = s.heads // s.kv
+    near = lambda *n: 1.0 + torch.randn(*n, 1, device="cuda") / 64
+    s.q.copy_((u.repeat_interleave(group, 0) * near(s.n_tokens, s.heads)).to(s.act))
+    for b, (_, n) in enumerate(s.seqs):
+        s.k[b] = (u * near(n, s.kv) * (level / math.sqrt(s.hs))).to(s.cache_t)
+        for i, page in enumerate(s.table[b].tolist()):
+            rows = s.k[b][i * s.page:(i + 1) * s.page]
+            if page >= 0 and len(rows):
+                s.k_pages[page, : len(rows)] = rows
+
+
+@pytest.mark.parametrize("act,cache", TYPES)
+@pytest.mark.parametrize("hs", [64, 128])
+@pytest.mark.parametrize("new,seqs,heads", [(1, 1, 4), (1, 400, 4), (40, 1, 2), (40, 40, 2), (300, 1, 4), (300, 12, 4)])
+@pytest.mark.parametrize("gone", [[0, 1, 2, 3, 6, 7, 8], [0, 1, 4, 5, 8, 9]])
+def test_logits_far_below_zero_behind_pages_that_are_gone(act, cache, hs, new, seqs, heads, gone):
+    """A window whose first key tiles are not held, and one in the middle; and every other tile: the softmax of what is left does not
+    depend on where the logits lie.  One sequence is shared out over the blocks of the launch, of many each is one block's."""
+    n, page = 700, 64
+    if seqs == 400:
+        n, gone = 330, [0, 1, 2, 3]
+    s = setup([(new, n - b % 7) for b in range(seqs)], heads, 1, hs, page, act, cache, seed=21, drop=[(b, i) for b in range(seqs) for i in gone])
+    far_below(s, -150.0)
+    s.cache.attend(s.batch, s.q, s.out)
+    s.check()
+    assert s.cache.status() == (0, 0, 0, 0)
