@@ -537,7 +537,10 @@ typedef struct McaPagedCache {
   int64_t page_stride;
   int n_pages, page_size, n_heads, n_kv_heads, head_size;
   int dtype;               /* of the pages: MCA_DTYPE_F32 or MCA_DTYPE_BF16 */
+  int* status;             /* MCA_PAGED_STATUS_WORDS device ints, 16-byte aligned and zero before the first call: where the calls over this
+                              cache record what they refuse (mca_paged_status_of); null: the device's own words (mca_paged_status) */
 } McaPagedCache;
+#define MCA_PAGED_STATUS_WORDS 8
 /* The new tokens of a step: those of sequence b are rows [starts[b], starts[b+1]) of the token tensors, the last of its
  * lengths[b] positions (so lengths counts them: token i of the sequence has position lengths[b] - (starts[b+1] - starts[b]) + i).
  * starts rises from 0 on; a sequence may have none (its length and pages are then not looked at).  Rows behind starts[n_seqs], up to n_tokens, are not read and not written.
@@ -606,11 +609,14 @@ MCA_API int mca_paged_append(const McaPagedCache* cache, const McaPagedBatch* ba
 MCA_API int64_t mca_paged_attention_workspace_bytes(const McaPagedCache* cache, const McaPagedBatch* batch, int dtype);
 MCA_API int mca_paged_attention(const McaPagedCache* cache, const McaPagedBatch* batch, int dtype, const McaHeads* q, float scale,
                                 const McaHeads* out, void* workspace, int64_t workspace_bytes, void* stream);
-/* Reads and clears the status words of the calls above on the current device (blocking; call after the stream has been
- * synchronised): status4[0] = 0, or what was refused first: 1 a sequence's lengths (status4[1] = the sequence, [2] = its length), 2 a
- * page id ([1] = the sequence, [2] = the id), 3 a position outside the tables ([1] = the token row, [2] = the position), 4 a bounded
- * wait of the attention kernel gave up ([1] = the stage, [2] = the block): its output is not complete; status4[3] = how many. */
+/* Takes what the calls above recorded out of the current device's own status words, which are those of all callers of the device whose
+ * caches have none, and of mca_qk_norm_rope_* (blocking; call after the stream has been synchronised): status4[0] = 0, or what was
+ * refused first: 1 a sequence's lengths (status4[1] = the sequence, [2] = its length), 2 a page id ([1] = the sequence, [2] = the id), 3 a
+ * position outside the tables ([1] = the token row, [2] = the position); status4[3] = how many.  4: a bounded wait of the attention kernel
+ * gave up ([1] = the stage, [2] = the block), and its output is not complete; what was refused besides is left for the next reading. */
 MCA_API int mca_paged_status(int* status4);
+/* The same from the words of a cache (McaPagedCache::status), on its device. */
+MCA_API int mca_paged_status_of(int* status, int* status4);
 
 /* TFT interpretable attention forward.  Replaces the attention block of
  * MultiHeadAttentionInterpLayer<T>.forward, MyCaffe.layers.tft/layers.tft/

@@ -98,6 +98,7 @@ SIGNATURES = {
     "mca_paged_append": (_i, [_vp, _vp, _vp, _i, _vp, _vp, _vp, _vp, _vp]),
     "mca_paged_attention_workspace_bytes": (_i64, [_vp, _vp, _i]),
     "mca_paged_attention": (_i, [_vp, _vp, _i, _vp, C.c_float, _vp, _vp, _i64, _vp]),
+    "mca_paged_status_of": (_i, [_vp, C.POINTER(_i)]),
     "mca_paged_status": (_i, [C.POINTER(_i)]),
     "mca_tft_attention_forward_f32": (_i, [_vp, _vp, _vp, _vp, _i, _i, _i, _i, _i, _vp, _vp, _vp]),
     "mca_tft_attention_backward_f32": (_i, [_vp, _vp, _vp, _vp, _vp, _vp, _i, _i, _i, _i, _i, _vp, _vp, _vp, _vp]),

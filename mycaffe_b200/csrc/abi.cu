@@ -91,15 +91,18 @@ struct DecodeHandle {
   int64_t scratch_floats = 0;
 };
 
-// A layer's paged cache as the dispatch ids see it: its geometry, the rotation's tables, and the attention's workspace (grow-only; the
-// calls of a kernel index follow one another on one stream).
+// A layer's paged cache as the dispatch ids see it: its geometry, the rotation's tables, its status words, and the attention's workspace
+// (grow-only; the calls of a kernel index follow one another on one stream).
 struct PagedHandle {
   McaPagedCache cache = {};
   McaQkRotation rotation = {};
   float *cos_t = nullptr, *sin_t = nullptr;
   void* work = nullptr;
   int64_t work_bytes = 0;
-  void release() { cudaFree(cos_t); cudaFree(sin_t); cudaFree(work); }
+  int* status = nullptr;       // the cache's status words
+  bool pending = false;        // a call was made in asynchronous mode and the words are unread
+  uint64_t looked = 0;         // the device's count of raised words (see paged_may_have_failed) up to which they are known
+  void release() { cudaFree(cos_t); cudaFree(sin_t); cudaFree(work); cudaFree(status); }
 };
 
 struct LayerNormHandle {
@@ -165,7 +168,8 @@ struct Kernel {
   // What a handle sees of it: no more than it asked for, so that its kernels, and its gradients' last bits, do not depend on which other
   // handles there are.
   int64_t ds_room(const AttnHandle& a) const { return std::min(a.ds_floats, ds_ws_floats); }
-  bool paged_pending = false;   // a paged call was made in asynchronous mode and its status words are unread
+  long paged_left = 0;          // what a paged handle that was freed before its status words were asked for had refused
+  std::string paged_left_detail;
   bool synced = false;     // the call being dispatched has already synchronised the stream behind its last launch
   bool by_word = false;    // the call being dispatched is waited for by the done word (see sync_call)
   bool fail_words = false; // this device's kernels raise its failure words (see g_fail)
@@ -211,8 +215,8 @@ Kernel* g_kernels[kMaxKernels];
 std::mutex g_table_lock;
 
 // The failure words (fail_words.h).  A raised MCA_FAIL_TC word stays raised (it stands for every attention handle's own status
-// words, and a bounded wait giving up is no ordinary event); the other two families have one status array per device and
-// their word is lowered before that array is read.
+// words, and a bounded wait giving up is no ordinary event); the decode and the projections have one status array per device and
+// their word is lowered before that array is read; for the paged caches see paged_may_have_failed.
 McaFailTable g_fail;
 uint64_t g_fail_armed = 0;   // devices whose kernels know their row
 
@@ -696,7 +700,7 @@ long tc_status(Kernel* k, AttnHandle& a) {
   if (k->async) { a.status_pending = true; return 0; }
   return read_status(k, a);
 }
-long paged_status(Kernel* k);
+long paged_status(Kernel* k, PagedHandle& p);
 long sync_and_collect_status(Kernel* k) {
   const long se = sync_call(k);
   if (se) return se;
@@ -707,9 +711,15 @@ long sync_and_collect_status(Kernel* k) {
     const long e = read_status(k, kv.second);
     if (e && !first) first = e;
   }
-  if (k->paged_pending) {
-    k->paged_pending = false;
-    const long e = paged_status(k);
+  if (k->paged_left != 0) {
+    if (!first) first = k->paged_left;
+    k->last_detail = k->paged_left_detail;
+    k->paged_left = 0;
+  }
+  for (auto& kv : k->paged) {
+    if (!kv.second.pending) continue;
+    kv.second.pending = false;
+    const long e = paged_status(k, kv.second);
     if (e && !first) first = e;
   }
   return first;
@@ -1357,15 +1367,20 @@ long paged_create(Kernel* k, long lInput, float* pf, long llInput, MCA_LONGLONG*
   if (!mca_decode_head_size_supported(c.head_size)) return ERROR_ATTN_UNSUPPORTED_SHAPE;
   if (c.n_heads % c.n_kv_heads || c.n_heads > 65535 || c.page_size < 16 || c.page_size > 65536 || (c.page_size & (c.page_size - 1))) return ERROR_PARAM_OUT_OF_RANGE;
   if (pl[7] & ~(MCA_QK_NORM | MCA_ROPE_HALVES)) return ERROR_PARAM_OUT_OF_RANGE;
+  const bool turn = pf[0] > 0.f;   // theta <= 0: no rotation, as DECODE_CREATE
+  if (turn && (pl[6] < 1 || pl[6] > (1 << 24))) return ERROR_PARAM_OUT_OF_RANGE;
   c.page_stride = (int64_t)c.page_size * c.n_kv_heads * c.head_size;
+  const size_t status_bytes = MCA_PAGED_STATUS_WORDS * sizeof(int);
+  if (cudaMalloc(&p.status, status_bytes) != cudaSuccess || cudaMemset(p.status, 0, status_bytes) != cudaSuccess) { cudaGetLastError(); p.release(); return ERROR_MEMORY_OUT; }
+  c.status = p.status;
   p.rotation.flags = (int)pl[7]; p.rotation.eps = pf[1];
-  if (pf[0] > 0.f) {   // theta <= 0: no rotation, as DECODE_CREATE
-    if (pl[6] < 1 || pl[6] > (1 << 24)) return ERROR_PARAM_OUT_OF_RANGE;
+  if (turn) {
     const size_t n = (size_t)pl[6] * (c.head_size / 2);
     std::vector<float> cs, sn;
     try {
       cs.resize(n); sn.resize(n);
     } catch (const std::bad_alloc&) {
+      p.release();
       return ERROR_MEMORY_OUT;
     }
     mca_rope_tables_host((int)pl[6], c.head_size, pf[0], cs.data(), sn.data());
@@ -1385,18 +1400,42 @@ long paged_free(Kernel* k, long lInput, float* pf) {
   auto it = k->paged.find((long)pf[0]);
   if (it == k->paged.end()) return ERROR_PARAM_OUT_OF_RANGE;
   cudaStreamSynchronize(0);
+  if (it->second.pending && k->paged_left == 0) {   // the next call that synchronises reports it
+    k->paged_left = paged_status(k, it->second);
+    k->paged_left_detail = k->last_detail;
+    k->last_detail.clear();
+  }
   it->second.release();
   k->paged.erase(it);
   return 0;
 }
 
+// Whether a cache's status words may say something.  The device's failure word stands for all its caches, those of other kernel indices and
+// of raw callers among them, and whoever finds it raised lowers it: that is counted, and each handle looks at its words once for each count
+// (a word raised while it is lowered falls under that count, whose handle has not looked yet).
+bool paged_may_have_failed(const Kernel* k, PagedHandle& p) {
+  if (!k->fail_words) return true;
+  static std::mutex lock;
+  static uint64_t raised[MCA_FAIL_DEVICES];
+  std::lock_guard<std::mutex> guard(lock);
+  if (g_fail.raised(k->device, MCA_FAIL_PAGED)) {
+    lower_fail_word(k, MCA_FAIL_PAGED);
+    ++raised[k->device];
+  }
+  if (p.looked == raised[k->device]) return false;
+  p.looked = raised[k->device];
+  return true;
+}
 // The status words after the stream has been waited for.
-long paged_status(Kernel* k) {
-  if (!may_have_failed(k, MCA_FAIL_PAGED)) return 0;
-  lower_fail_word(k, MCA_FAIL_PAGED);
+long paged_status(Kernel* k, PagedHandle& p) {
+  if (!paged_may_have_failed(k, p)) return 0;
   int st[4] = {0, 0, 0, 0};
-  const long e = mca_paged_status(st);
+  const long e = mca_paged_status_of(p.status, st);
   if (e || st[0] == 0) return e;
+  if (st[0] == 4) {   // what was refused besides is still there
+    int more[4];
+    if (mca_paged_status_of(p.status, more) == 0) st[3] = more[3];
+  }
   static const char* const what[5] = {"", "sequence with bad lengths", "page id outside the pool or page not held: sequence", "position outside the tables: token row",
                                       "bounded wait gave up at stage"};
   char buf[128];
@@ -1404,11 +1443,11 @@ long paged_status(Kernel* k) {
   k->last_detail = buf;
   return st[0] == 4 ? ERROR_ATTN_KERNEL_TIMEOUT : ERROR_PARAM_OUT_OF_RANGE;
 }
-long paged_result(Kernel* k, long e) {
+long paged_result(Kernel* k, PagedHandle& p, long e) {
   if (e) return e;
-  if (k->async) { k->paged_pending = true; return 0; }
+  if (k->async) { p.pending = true; return 0; }
   if ((e = sync_call(k))) return e;
-  return paged_status(k);
+  return paged_status(k, p);
 }
 
 // What APPEND and ATTN share: the handle, its pages, and the batch {hStarts,hLengths,hTable,tableStride,nSeqs,nTokens,maxNew,maxLen} at `b`.
@@ -1447,7 +1486,7 @@ long paged_append(Kernel* k, long llInput, MCA_LONGLONG* pl) {
   if ((e = check_activations(k, (long)pl[1], b.n_tokens * qn, &bf16, &q.data)) || (e = check_activations(k, (long)pl[2], b.n_tokens * kn, &bf16, &kk.data)) ||
       (e = check_activations(k, (long)pl[3], b.n_tokens * kn, &bf16, &v.data)) || (e = check_activations(k, (long)pl[16], b.n_tokens * qn, &bf16, &qo.data)))
     return e;
-  return paged_result(k, mca_paged_append(&c, &b, &r, bf16 ? MCA_DTYPE_BF16 : MCA_DTYPE_F32, &q, &kk, &v, &qo, 0));
+  return paged_result(k, *p, mca_paged_append(&c, &b, &r, bf16 ? MCA_DTYPE_BF16 : MCA_DTYPE_F32, &q, &kk, &v, &qo, 0));
 }
 
 long paged_attn(Kernel* k, long llInput, MCA_LONGLONG* pl) {
@@ -1469,7 +1508,7 @@ long paged_attn(Kernel* k, long llInput, MCA_LONGLONG* pl) {
     if (cudaMalloc(&p->work, (size_t)need) != cudaSuccess) { cudaGetLastError(); return ERROR_MEMORY_OUT; }
     p->work_bytes = need;
   }
-  return paged_result(k, mca_paged_attention(&c, &b, dtype, &q, 0.f, &out, p->work, p->work_bytes, 0));   // where need is -1 it says why
+  return paged_result(k, *p, mca_paged_attention(&c, &b, dtype, &q, 0.f, &out, p->work, p->work_bytes, 0));   // where need is -1 it says why
 }
 
 long tft_fwd(Kernel* k, long llInput, MCA_LONGLONG* pl) {

@@ -54,8 +54,8 @@ int mca_set_fail_words_proj(int* words);
 int mca_set_fail_words_qk_norm(int* words);
 int mca_set_fail_words_paged(int* words);
 
-// Internal: the status words (mca_paged_status) of the norm and append kernels; clears them.
-int mca_qk_norm_read_status(int* out);
+// Internal: the current device's own status words of the paged cache's kernels and the norm's (mca_paged_status).
+int mca_paged_device_status(int** words);
 
 // Internal: the decode attention inside a step of up to eight sequences.  Where step_rules says so its combine pass is left to
 // mca_decode_out_proj_partials (one sequence), which combines the partial results while it stages its activations: *partials

@@ -12,6 +12,7 @@
 #include <algorithm>
 #include <cfloat>
 #include <cmath>
+#include <mutex>
 #include <type_traits>
 
 #define MCA_TU_FAIL_FAMILY MCA_FAIL_PAGED
@@ -25,7 +26,7 @@ using paged::Sequence;
 
 constexpr float LOG2E = 1.4426950408889634f;
 
-__device__ int g_wait_status[4];   // what a bounded wait of the tensor-core kernel leaves (see tc_common.cuh)
+__device__ __align__(16) int g_status[8];   // the device's own status words (paged_common.cuh)
 
 struct AttnArgs {
   Batch batch;
@@ -84,7 +85,7 @@ template <typename T> __device__ void look_over(const AttnArgs& p) {
   for (int b0 = 0; b0 < p.batch.n_seqs; b0 += blockDim.x) {
     const int mine = b0 + threadIdx.x;
     const bool bad = mine < p.batch.n_seqs && !paged::sequence(p.batch, mine).good;
-    if (bad) paged::refuse(paged::REFUSED_LENGTHS, mine, p.batch.lengths[mine]);
+    if (bad) paged::refuse(p.batch.status, paged::REFUSED_LENGTHS, mine, p.batch.lengths[mine]);
     if (!__syncthreads_or(bad)) continue;
     for (int b = b0; b < min(b0 + (int)blockDim.x, p.batch.n_seqs); ++b) {
       if (paged::sequence(p.batch, b).good) continue;
@@ -102,7 +103,7 @@ template <typename T> __device__ void look_over(const AttnArgs& p) {
 __device__ __forceinline__ int page_of(const Batch& t, int seq, int pos, bool tell) {
   const int id = t.table[(int64_t)seq * t.table_stride + (pos >> t.page_shift)];
   if (id >= 0 && id < t.n_pages) return id;
-  if (tell && id != -1) paged::refuse(paged::REFUSED_PAGE, seq, id);
+  if (tell && id != -1) paged::refuse(t.status, paged::REFUSED_PAGE, seq, id);
   return -1;
 }
 
@@ -803,6 +804,16 @@ template <typename T> __device__ __noinline__ void add_odd(const AttnArgs& p, co
   }
 }
 
+// Bounded waits.  The words that one which gives up leaves are looked up where that happens: their address in the registers of the softmax
+// warps is spilled for others (2048 tokens over 16384, 32 / 8 heads of 128: 661 us for 609).
+__shared__ int* s_wait_words;
+__device__ __noinline__ bool wait_longer(uint32_t bar, uint32_t parity, int stage, int iter) {
+  return mbar_wait_limited(bar, parity, *const_cast<int* volatile*>(&s_wait_words), stage, iter, WAIT_LIMIT_NS);
+}
+__device__ __forceinline__ bool wait_for(uint32_t bar, uint32_t parity, int stage, int iter) {
+  return mbar_try_wait(bar, parity) || wait_longer(bar, parity, stage, iter);
+}
+
 template <int HDP, bool ACT32, bool FEW>
 __global__ void __launch_bounds__(TC_THREADS, (TcPlan<HDP, FEW>::CTAS)) paged_tc_kernel(const __grid_constant__ CUtensorMap map_k,
                                                                                        const __grid_constant__ CUtensorMap map_v, const __grid_constant__ AttnArgs p) {
@@ -815,7 +826,6 @@ __global__ void __launch_bounds__(TC_THREADS, (TcPlan<HDP, FEW>::CTAS)) paged_tc
   volatile uint32_t* tmem_slot = reinterpret_cast<volatile uint32_t*>(smem + PL::OFF_BAR + TB_COUNT * 8);
   auto bar = [&](int i) { return smem_base + PL::OFF_BAR + 8u * (uint32_t)i; };
   const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
-  int* const status = g_wait_status;
   __shared__ int s_abort;
 
   mca_pdl_launch_dependents();
@@ -842,7 +852,10 @@ __global__ void __launch_bounds__(TC_THREADS, (TcPlan<HDP, FEW>::CTAS)) paged_tc
     asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
   }
   mca_pdl_wait();   // from here on the results of the kernels before this one are complete and visible
-  if (tid == 32) s_abort = *reinterpret_cast<volatile int*>(status);
+  if (tid == 32) {
+    s_wait_words = p.batch.status + paged::WAIT_WORDS;
+    s_abort = *reinterpret_cast<volatile int*>(s_wait_words);
+  }
   tc_fence_before();
   __syncthreads();
   tc_fence_after();
@@ -857,7 +870,7 @@ __global__ void __launch_bounds__(TC_THREADS, (TcPlan<HDP, FEW>::CTAS)) paged_tc
   int item = 0;   // parts of items so far
   Segment* const ring = reinterpret_cast<Segment*>(smem + PL::OFF_SEG);
   auto next_segment = [&](int stage) -> const Segment* {   // for the roles but the producer; null: no more
-    ok = __all_sync(0xffffffffu, mbar_wait(bar(TB_GF + item % SEGMENTS), (uint32_t)((item / SEGMENTS) & 1), status, stage, item));
+    ok = __all_sync(0xffffffffu, wait_for(bar(TB_GF + item % SEGMENTS), (uint32_t)((item / SEGMENTS) & 1), stage, item));
     return ok && ring[item % SEGMENTS].n > 0 ? ring + item % SEGMENTS : nullptr;
   };
   auto release_segment = [&]() {
@@ -890,7 +903,7 @@ __global__ void __launch_bounds__(TC_THREADS, (TcPlan<HDP, FEW>::CTAS)) paged_tc
         first = false;
       }
       if (!more || g.n > 0) {
-        ok = __all_sync(0xffffffffu, mbar_wait(bar(TB_GE + item % SEGMENTS), (uint32_t)((item / SEGMENTS) & 1) ^ 1u, status, 9, item));
+        ok = __all_sync(0xffffffffu, wait_for(bar(TB_GE + item % SEGMENTS), (uint32_t)((item / SEGMENTS) & 1) ^ 1u, 9, item));
         if (!ok) break;
         if (lane == 0) {
           ring[item % SEGMENTS] = g;
@@ -911,7 +924,7 @@ __global__ void __launch_bounds__(TC_THREADS, (TcPlan<HDP, FEW>::CTAS)) paged_tc
         const uint32_t ph = (uint32_t)((c / STG) & 1);
         const int next = page_at(j + 1);
         const int slot = (g.k_begin + j * KEYS + lane * box_rows) & ((1 << shift) - 1);
-        ok = __all_sync(0xffffffffu, mbar_wait(bar(TB_KE + st), ph ^ 1u, status, 10, c));
+        ok = __all_sync(0xffffffffu, wait_for(bar(TB_KE + st), ph ^ 1u, 10, c));
         if (!ok) break;
         if (lane == 0) mbar_expect_tx(bar(TB_KF + st), PL::TILE_BYTES);
         __syncwarp();
@@ -920,7 +933,7 @@ __global__ void __launch_bounds__(TC_THREADS, (TcPlan<HDP, FEW>::CTAS)) paged_tc
           for (int s = 0; s < PL::SUB; ++s)
             tma_load_4d(smem_base + PL::OFF_K + st * PL::TILE_BYTES + s * PL::SUB_BYTES + lane * box_rows * 128, &map_k, bar(TB_KF + st), s * 64, g.kvh, slot, page);
         issued_k = c + 1;
-        ok = __all_sync(0xffffffffu, mbar_wait(bar(TB_VE + st), ph ^ 1u, status, 11, c));
+        ok = __all_sync(0xffffffffu, wait_for(bar(TB_VE + st), ph ^ 1u, 11, c));
         if (!ok) break;
         if (lane == 0) mbar_expect_tx(bar(TB_VF + st), PL::TILE_BYTES);
         __syncwarp();
@@ -935,8 +948,8 @@ __global__ void __launch_bounds__(TC_THREADS, (TcPlan<HDP, FEW>::CTAS)) paged_tc
       if (more) w.advance(p);
     }
     if (!ok) {   // copies in flight get a bounded time to land before the CTA's memory is released
-      for (int j = max(0, issued_k - STG); j < issued_k; ++j) mbar_wait(bar(TB_KF + (j % STG)), (uint32_t)((j / STG) & 1), status, 13, j);
-      for (int j = max(0, issued_v - STG); j < issued_v; ++j) mbar_wait(bar(TB_VF + (j % STG)), (uint32_t)((j / STG) & 1), status, 14, j);
+      for (int j = max(0, issued_k - STG); j < issued_k; ++j) wait_for(bar(TB_KF + (j % STG)), (uint32_t)((j / STG) & 1), 13, j);
+      for (int j = max(0, issued_v - STG); j < issued_v; ++j) wait_for(bar(TB_VF + (j % STG)), (uint32_t)((j / STG) & 1), 14, j);
     }
   } else if (warp == TC_WARP_MMA) {
     // ------------------------------------------------------------------ MMA issuer, in lock step; one elected lane issues
@@ -963,7 +976,7 @@ __global__ void __launch_bounds__(TC_THREADS, (TcPlan<HDP, FEW>::CTAS)) paged_tc
       for (int kk = lo; kk < hi; ++kk)
         umma_ts_if<false>(leader, tm + PL::O_COL, a + (uint32_t)(kk * 8), dv + (uint64_t)((uint32_t)kk * (2048u >> 4)), IDESC_PV, (first && kk == 0) ? 0u : 1u);
     };
-    auto wait = [&](int b, uint32_t ph, int stage) { return __all_sync(0xffffffffu, mbar_wait(bar(b), ph & 1u, status, stage, c)); };
+    auto wait = [&](int b, uint32_t ph, int stage) { return __all_sync(0xffffffffu, wait_for(bar(b), ph & 1u, stage, c)); };
     while (const Segment* g = next_segment(19)) {
       const int n = g->n;
       {
@@ -998,7 +1011,7 @@ __global__ void __launch_bounds__(TC_THREADS, (TcPlan<HDP, FEW>::CTAS)) paged_tc
       release_segment();
     }
     umma_commit_if(leader, bar(TB_DRAIN));   // the tensor pipe is idle (bounded) before TMEM is freed
-    mbar_wait(bar(TB_DRAIN), 0, status, 27, 0);
+    wait_for(bar(TB_DRAIN), 0, 27, 0);
     __syncwarp();
   } else {
     constexpr int CH = HDP / 8;   // 16-byte pieces of a row
@@ -1068,7 +1081,7 @@ __global__ void __launch_bounds__(TC_THREADS, (TcPlan<HDP, FEW>::CTAS)) paged_tc
             const int id = p.batch.table[(int64_t)g.seq * p.batch.table_stride + i];
             if (id < 0 || id >= p.batch.n_pages) {
               hole = true;
-              if (id != -1 && rank == 0 && g.head0 == 0) paged::refuse(paged::REFUSED_PAGE, g.seq, id);
+              if (id != -1 && rank == 0 && g.head0 == 0) paged::refuse(p.batch.status, paged::REFUSED_PAGE, g.seq, id);
             }
           }
           const bool holes = __any_sync(0xffffffffu, hole);
@@ -1080,13 +1093,13 @@ __global__ void __launch_bounds__(TC_THREADS, (TcPlan<HDP, FEW>::CTAS)) paged_tc
           float m_used[2] = {-INFINITY, -INFINITY}, l[2] = {0.f, 0.f};
           for (int j = 0; j < g.n; ++j, ++c) {
             const uint32_t t_s = t_row + (FEW ? (uint32_t)(c & 1) * 128u : 0u);
-            ok = __all_sync(0xffffffffu, mbar_wait(bar(TB_S + (FEW ? c & 1 : 0)), (uint32_t)((FEW ? c >> 1 : c) & 1), status, 30, c));
+            ok = __all_sync(0xffffffffu, wait_for(bar(TB_S + (FEW ? c & 1 : 0)), (uint32_t)((FEW ? c >> 1 : c) & 1), 30, c));
             if (!ok) break;
             const int key0 = g.k_begin + j * KEYS;
             // g.pos: the last key the tile's first row sees.  Here, while there are registers for it, and not before S is there: with one stage,
             // S says that the values before these have arrived and been used, so that the parity waited for is these values' own
             if (key0 + KEYS - 1 > g.pos) {
-              ok = __all_sync(0xffffffffu, mbar_wait(bar(TB_VF + c % STG), (uint32_t)((c / STG) & 1), status, 31, c));
+              ok = __all_sync(0xffffffffu, wait_for(bar(TB_VF + c % STG), (uint32_t)((c / STG) & 1), 31, c));
               if (!ok) break;
               if (clear_odd<HDP>(smem_base + PL::OFF_V + (c % STG) * PL::TILE_BYTES, max(g.pos + 1 - key0, 0), g.last + 1 - key0, rank * 32 + lane, p.warps * 32)) *s_odd = item + 1;
             }
@@ -1150,7 +1163,7 @@ __global__ void __launch_bounds__(TC_THREADS, (TcPlan<HDP, FEW>::CTAS)) paged_tc
               }
               if (j > 0) {
                 if constexpr (FEW) {   // P V(c - 1) may still be running; with one S tile it finished before S(c) did
-                  ok = __all_sync(0xffffffffu, mbar_wait(bar(TB_O), (uint32_t)((c - 1) & 1), status, 32, c));
+                  ok = __all_sync(0xffffffffu, wait_for(bar(TB_O), (uint32_t)((c - 1) & 1), 32, c));
                   if (!ok) break;
                   tc_fence_after();
                 }
@@ -1228,8 +1241,8 @@ __global__ void __launch_bounds__(TC_THREADS, (TcPlan<HDP, FEW>::CTAS)) paged_tc
           if (FEW && gn != nullptr) load_query(*gn);
           item = at;
         }
-        if (ok) ok = __all_sync(0xffffffffu, mbar_wait(bar(TB_DONE), (uint32_t)(item & 1), status, 34, c));
-        if (ok) ok = __all_sync(0xffffffffu, mbar_wait(bar(TB_RED), (uint32_t)(item & 1), status, 36, c));
+        if (ok) ok = __all_sync(0xffffffffu, wait_for(bar(TB_DONE), (uint32_t)(item & 1), 34, c));
+        if (ok) ok = __all_sync(0xffffffffu, wait_for(bar(TB_RED), (uint32_t)(item & 1), 36, c));
         const int first_row = ACT32 ? (warp & 3) * 16 : (warp & 3) * 32;
         if (ok && first_row < g.rows) {
           tc_fence_after();
@@ -1349,6 +1362,32 @@ __global__ void __launch_bounds__(256) paged_join_kernel(const AttnArgs p) {
     if constexpr (sizeof(T) == 4) reinterpret_cast<float4*>(dst)[q] = make_float4(a[i].x * inv, a[i].y * inv, a[i].z * inv, a[i].w * inv);
     else reinterpret_cast<uint2*>(dst)[q] = make_uint2(pack_bf16(a[i].x * inv, a[i].y * inv), pack_bf16(a[i].z * inv, a[i].w * inv));
   }
+}
+
+// ---------------------------------------------------------------------------------------------------------------------
+// Takes what the status words say out of them.  A wait that gave up goes first and leaves the refusals for the next reading, as does a
+// refusal whose details are still being written.
+// ---------------------------------------------------------------------------------------------------------------------
+__device__ int g_taken[4];
+__global__ void __launch_bounds__(1) take_status_kernel(int* words) {
+  volatile int* const w = words;
+  int kind = 0, a = 0, b = 0, n = 0;
+  if (w[paged::WAIT_WORDS] != 0) {
+    __threadfence();
+    kind = paged::REFUSED_WAIT; a = w[paged::WAIT_WORDS + 1]; b = w[paged::WAIT_WORDS + 2]; n = 1;
+    for (int i = 3; i > 0; --i) w[paged::WAIT_WORDS + i] = 0;
+    __threadfence();
+    w[paged::WAIT_WORDS] = 0;
+  } else if (w[0] > 0) {
+    kind = w[0];
+    __threadfence();
+    a = w[1]; b = w[2];
+    __threadfence();
+    atomicExch(words, 0);
+    __threadfence();
+    n = max(atomicExch(words + 3, 0), 1);   // 0: counted by the reading before, which came between its count and its details
+  }
+  g_taken[0] = kind; g_taken[1] = a; g_taken[2] = b; g_taken[3] = n;
 }
 
 // ---------------------------------------------------------------------------------------------------------------------
@@ -1502,6 +1541,7 @@ int mca_paged_attention(const McaPagedCache* cache, const McaPagedBatch* batch, 
     if (!workspace || workspace_bytes < plan.bytes) return ERROR_ATTN_SCRATCH_TOO_SMALL;
     if ((uintptr_t)workspace & 15) return ERROR_PARAM_OUT_OF_RANGE;
   }
+  if ((e = paged::find_status(&a.batch.status))) return e;
   const int D = cache->head_size, size = dtype == MCA_DTYPE_BF16 ? 2 : 4, csize = cache->dtype == MCA_DTYPE_BF16 ? 2 : 4;
   a.q = static_cast<const char*>(q->data); a.out = static_cast<char*>(out->data);
   a.q_st = q->stride_t * size; a.q_sh = q->stride_h * size; a.out_st = out->stride_t * size; a.out_sh = out->stride_h * size;
@@ -1538,21 +1578,34 @@ int mca_paged_attention(const McaPagedCache* cache, const McaPagedBatch* batch, 
   return mca_launch_pdl(paged_simt_join_kernel, dim3((unsigned)((rows + 3) / 4)), dim3(128), 0, st, a);
 }
 
+int mca_paged_device_status(int** words) {
+  static std::atomic<int*> known[MCA_FAIL_DEVICES];
+  int dev = 0;
+  MCA_CUDA_TRY(cudaGetDevice(&dev));
+  int* at = dev < MCA_FAIL_DEVICES ? known[dev].load(std::memory_order_relaxed) : nullptr;
+  if (at == nullptr) {
+    MCA_CUDA_TRY(cudaGetSymbolAddress((void**)&at, g_status));
+    if (dev < MCA_FAIL_DEVICES) known[dev].store(at, std::memory_order_relaxed);
+  }
+  *words = at;
+  return 0;
+}
+
+int mca_paged_status_of(int* status, int* status4) {
+  if (!status || !status4) return ERROR_PARAM_NULL;
+  if ((uintptr_t)status & 15) return ERROR_PARAM_OUT_OF_RANGE;
+  static std::mutex one_reader;   // of g_taken
+  std::lock_guard<std::mutex> lock(one_reader);
+  take_status_kernel<<<1, 1>>>(status);
+  const int e = mca_launch_status();
+  if (e) return e;
+  return (int)cudaMemcpyFromSymbol(status4, g_taken, sizeof(int) * 4);
+}
 int mca_paged_status(int* status4) {
   if (!status4) return ERROR_PARAM_NULL;
-  int own[4] = {0, 0, 0, 0}, norm[4] = {0, 0, 0, 0}, wait[4] = {0, 0, 0, 0};
-  int e = paged::read_status(own);
-  if (e || (e = mca_qk_norm_read_status(norm))) return e;
-  MCA_CUDA_TRY(cudaMemcpyFromSymbol(wait, g_wait_status, sizeof(wait)));
-  if (wait[0] != 0) {
-    const int zero[4] = {0, 0, 0, 0};
-    MCA_CUDA_TRY(cudaMemcpyToSymbol(g_wait_status, zero, sizeof(zero)));
-    status4[0] = paged::REFUSED_WAIT; status4[1] = wait[1]; status4[2] = wait[2]; status4[3] = 1;
-    return 0;
-  }
-  const int* s = norm[3] != 0 ? norm : own;
-  status4[0] = s[0]; status4[1] = s[1]; status4[2] = s[2]; status4[3] = own[3] + norm[3];
-  return 0;
+  int* words = nullptr;
+  const int e = mca_paged_device_status(&words);
+  return e ? e : mca_paged_status_of(words, status4);
 }
 
 int mca_set_fail_words_paged(int* words) {

@@ -5,35 +5,33 @@
 
 namespace paged {
 
-// Status words (see mca_paged_status): kind and two details of what was refused first, and how many were.
+// Status words, a cache's own or the device's (see mca_paged_status): {kind and two details of what was refused first, how many were} and
+// the four words of a bounded wait (tc_common.cuh).
 enum Refusal : int { REFUSED_LENGTHS = 1, REFUSED_PAGE = 2, REFUSED_POSITION = 3, REFUSED_WAIT = 4 };
-static __device__ int g_status[4];
+constexpr int BEING_WRITTEN = -1;      // kind, while the details are
+constexpr int WAIT_WORDS = 4;          // where a wait's words begin
 static __device__ int* g_fail_words;   // this device's failure words (McaFailWord), or null
 
-static __device__ __noinline__ void refuse(int kind, int a, int b) {
-  if (atomicAdd(&g_status[3], 1) == 0) {
-    g_status[1] = a;
-    g_status[2] = b;
-    g_status[0] = kind;
+// Counted before the first one's place is tried for, and the place is given up before the count is taken (paged_attn.cu): what another
+// stream refuses while the words are read is found by this reading or the next.
+static __device__ __noinline__ void refuse(int* status, int kind, int a, int b) {
+  atomicAdd(status + 3, 1);
+  __threadfence();
+  if (atomicCAS(status, 0, BEING_WRITTEN) == 0) {
+    status[1] = a;
+    status[2] = b;
     __threadfence();
+    atomicExch(status, kind);
   }
+  __threadfence();
   mca_raise_fail_word(g_fail_words, MCA_FAIL_PAGED);
-}
-
-// Words of this translation unit; those that say something are cleared.
-static inline int read_status(int* out) {
-  MCA_CUDA_TRY(cudaMemcpyFromSymbol(out, g_status, sizeof(int) * 4));
-  if (out[3] != 0 || out[0] != 0) {
-    const int zero[4] = {0, 0, 0, 0};
-    MCA_CUDA_TRY(cudaMemcpyToSymbol(g_status, zero, sizeof(zero)));
-  }
-  return 0;
 }
 
 struct Batch {
   const int* starts;
   const int* lengths;
   const int* table;
+  int* status;
   int table_stride, n_seqs, n_tokens, max_new, max_len, n_pages, page_shift;
 };
 
@@ -74,16 +72,19 @@ static inline int check(const McaPagedCache* c, const McaPagedBatch* b, Batch* o
   const int vec = c->dtype == MCA_DTYPE_BF16 ? 8 : 4;
   if (c->page_stride % vec != 0 || c->page_stride < (int64_t)c->page_size * c->n_kv_heads * c->head_size) return ERROR_PARAM_OUT_OF_RANGE;
   if ((((uintptr_t)c->k_pages | (uintptr_t)c->v_pages) & 15) != 0) return ERROR_PARAM_OUT_OF_RANGE;
+  if (((uintptr_t)c->status & 15) != 0) return ERROR_PARAM_OUT_OF_RANGE;
   if ((((uintptr_t)b->starts | (uintptr_t)b->lengths | (uintptr_t)b->page_table) & 3) != 0) return ERROR_PARAM_OUT_OF_RANGE;
   if (b->n_seqs <= 0 || b->n_seqs > 65535 || b->n_tokens < 0 || b->max_new <= 0 || b->max_len <= 0 || b->table_stride <= 0) return ERROR_PARAM_OUT_OF_RANGE;
   if (b->max_len > (int64_t)b->table_stride * c->page_size || b->max_len > (1 << 30) || b->n_tokens > (1 << 30)) return ERROR_PARAM_OUT_OF_RANGE;
-  out->starts = b->starts; out->lengths = b->lengths; out->table = b->page_table;
+  out->starts = b->starts; out->lengths = b->lengths; out->table = b->page_table; out->status = c->status;
   out->table_stride = b->table_stride; out->n_seqs = b->n_seqs; out->n_tokens = b->n_tokens;
   out->max_new = b->max_new; out->max_len = b->max_len; out->n_pages = c->n_pages;
   out->page_shift = 0;
   while ((1 << out->page_shift) < c->page_size) ++out->page_shift;
   return 0;
 }
+// Host: the words that a call records in: those of its cache, or the current device's.
+static inline int find_status(int** status) { return *status != nullptr ? 0 : mca_paged_device_status(status); }
 // Host: a view whose rows are read and written as 16-byte vectors.
 static inline int check_heads(const McaHeads* h, int dtype, bool batched) {
   if (!h || !h->data) return ERROR_PARAM_NULL;

@@ -197,6 +197,7 @@ struct NormArgs {
   View x[2], out[2];        // queries, keys.  Backward: x and dx
   View g[2];                // backward: gradients of the outputs
   const int* positions;
+  int* status;
   int B, T, heads[2], ctas_q;
   Divisor by_chunks[2], by_t;
   float* partial;           // backward: (CTAs, D), or null
@@ -254,7 +255,7 @@ __global__ void __launch_bounds__(THREADS, CTAS<T>) qk_norm_rope_kernel(const No
     } else {
 #pragma unroll
       for (int i = 0; i < VEC; ++i) { c[i] = 1.f; s[i] = 0.f; }
-      if (bad && live && gl == 0 && h0 == 0 && kind == 0) paged::refuse(paged::REFUSED_POSITION, (int)token, pos);
+      if (bad && live && gl == 0 && h0 == 0 && kind == 0) paged::refuse(p.status, paged::REFUSED_POSITION, (int)token, pos);
     }
 #pragma unroll
     for (int i = 0; i < HEADS<T>; ++i) {
@@ -326,7 +327,7 @@ __global__ void __launch_bounds__(THREADS, CTAS<T>) qk_norm_rope_bwd_kernel(cons
     } else {
 #pragma unroll
       for (int i = 0; i < VEC; ++i) { c[i] = 1.f; s[i] = 0.f; }
-      if (bad && live && gl == 0 && h0 == 0 && kind == 0) paged::refuse(paged::REFUSED_POSITION, (int)token, pos);
+      if (bad && live && gl == 0 && h0 == 0 && kind == 0) paged::refuse(p.status, paged::REFUSED_POSITION, (int)token, pos);
     }
 #pragma unroll
     for (int i = 0; i < HEADS_BWD<T>; ++i) {
@@ -410,7 +411,7 @@ __global__ void __launch_bounds__(THREADS, CTAS<T>) paged_append_kernel(const Ap
   if ((int)blockIdx.x == p.first_cta[3]) {   // one more CTA looks the sequences over
     for (int b = threadIdx.x; b < p.batch.n_seqs; b += THREADS) {
       const paged::Sequence s = paged::sequence(p.batch, b);
-      if (!s.good) paged::refuse(paged::REFUSED_LENGTHS, b, s.length);
+      if (!s.good) paged::refuse(p.batch.status, paged::REFUSED_LENGTHS, b, s.length);
     }
     return;
   }
@@ -463,7 +464,7 @@ __global__ void __launch_bounds__(THREADS, CTAS<T>) paged_append_kernel(const Ap
         load_angles<VEC, HALVES>(p.r.sin_table + ar, gl, half, s);
       } else {
         zero = true;
-        if (reporter && kind == 0) paged::refuse(paged::REFUSED_POSITION, token, pos);
+        if (reporter && kind == 0) paged::refuse(p.batch.status, paged::REFUSED_POSITION, token, pos);
       }
     }
     char* dst = nullptr;     // the page row of a key or value
@@ -472,7 +473,7 @@ __global__ void __launch_bounds__(THREADS, CTAS<T>) paged_append_kernel(const Ap
       if (p.r.cos_table != nullptr && pos >= p.r.table_len) mine = false;   // its key is refused: neither is stored
       else if (page < 0 || page >= p.batch.n_pages) {
         mine = false;
-        if (reporter && kind == 1) paged::refuse(paged::REFUSED_PAGE, b, page);
+        if (reporter && kind == 1) paged::refuse(p.batch.status, paged::REFUSED_PAGE, b, page);
       } else {
         dst = (kind == 1 ? p.k_pages : p.v_pages) + page * p.page_bytes + (int64_t)(pos & ((1 << p.batch.page_shift) - 1)) * p.row_bytes;
       }
@@ -545,6 +546,7 @@ int check_norm(const McaQkRotation* rotation, const McaHeads* const (&views)[6],
   }
   a->positions = positions; a->B = B; a->T = T; a->heads[0] = n_heads; a->heads[1] = n_kv_heads; a->partial = nullptr;
   a->by_t = divisor(T);
+  a->status = nullptr;
   return 0;
 }
 
@@ -590,6 +592,7 @@ int mca_qk_norm_rope_forward(const McaQkRotation* rotation, const McaHeads* q, c
   const McaHeads* const views[6] = {q, k, q_out, k_out, nullptr, nullptr};
   int e = check_norm(rotation, views, 4, positions, dtype, B, T, n_heads, n_kv_heads, D, &a);
   if (e) return e;
+  if ((e = paged::find_status(&a.status))) return e;
   const bool halves = (rotation->flags & MCA_ROPE_HALVES) != 0;
   cudaStream_t st = (cudaStream_t)stream;
   if (dtype == MCA_DTYPE_BF16) {
@@ -627,6 +630,7 @@ int mca_qk_norm_rope_backward(const McaQkRotation* rotation, const McaHeads* q, 
     if (((uintptr_t)scratch | (uintptr_t)dq_weight | (uintptr_t)dk_weight) & 3) return ERROR_PARAM_OUT_OF_RANGE;
     a.partial = scratch;
   }
+  if ((e = paged::find_status(&a.status))) return e;
   const bool halves = (rotation->flags & MCA_ROPE_HALVES) != 0;
   cudaStream_t st = (cudaStream_t)stream;
   if (dtype == MCA_DTYPE_BF16) {
@@ -661,6 +665,7 @@ int mca_paged_append(const McaPagedCache* cache, const McaPagedBatch* batch, con
       (e = paged::check_heads(v, dtype, false)) || (e = paged::check_heads(q_out, dtype, false)))
     return e;
   if ((int64_t)batch->n_tokens * cache->n_heads >= (1ll << 31)) return ERROR_PARAM_OUT_OF_RANGE;
+  if ((e = paged::find_status(&a.batch.status))) return e;
   const int size = dtype == MCA_DTYPE_BF16 ? 2 : 4, csize = cache->dtype == MCA_DTYPE_BF16 ? 2 : 4;
   a.in[0] = view(q, size); a.in[1] = view(k, size); a.in[2] = view(v, size); a.q_out = view(q_out, size);
   a.k_pages = static_cast<char*>(cache->k_pages); a.v_pages = static_cast<char*>(cache->v_pages);
@@ -686,5 +691,4 @@ int mca_paged_append(const McaPagedCache* cache, const McaPagedBatch* batch, con
   return launch_append<float, float, 16>(a, halves, st);
 }
 
-int mca_qk_norm_read_status(int* out) { return paged::read_status(out); }
 int mca_set_fail_words_qk_norm(int* words) { return (int)cudaMemcpyToSymbol(paged::g_fail_words, &words, sizeof(words)); }

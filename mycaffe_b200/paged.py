@@ -30,13 +30,15 @@ class McaQkRotation(C.Structure):
 
 class McaPagedCache(C.Structure):
     _fields_ = [("k_pages", C.c_void_p), ("v_pages", C.c_void_p), ("page_stride", C.c_int64)] + [
-        (n, C.c_int) for n in ("n_pages", "page_size", "n_heads", "n_kv_heads", "head_size", "dtype")]
+        (n, C.c_int) for n in ("n_pages", "page_size", "n_heads", "n_kv_heads", "head_size", "dtype")] + [("status", C.c_void_p)]
 
 
 class McaPagedBatch(C.Structure):
     _fields_ = [("starts", C.c_void_p), ("lengths", C.c_void_p), ("page_table", C.c_void_p)] + [
         (n, C.c_int) for n in ("table_stride", "n_seqs", "n_tokens", "max_new", "max_len")]
 
+
+STATUS_WORDS = 8
 
 _DTYPES = {torch.float32: ids.MCA_DTYPE_F32, torch.bfloat16: ids.MCA_DTYPE_BF16}
 
@@ -175,18 +177,22 @@ class PagedBatch:
 
 class PagedCache:
     """The pages of one layer: k_pages, v_pages (n_pages, page_size, kv_heads, head_size), float32 or bfloat16; pages may lie apart
-    (a slice of a larger pool)."""
+    (a slice of a larger pool).  status: STATUS_WORDS int32 zeros on the device, 16-byte aligned, where the calls over this cache record what
+    they refuse; None: the device's own words, which all such caches and ``QkNormRope`` share."""
 
-    def __init__(self, k_pages, v_pages, n_heads):
+    def __init__(self, k_pages, v_pages, n_heads, status=None):
         self._lib = _lib.load()
         if k_pages.dim() != 4 or k_pages.shape != v_pages.shape or k_pages.dtype != v_pages.dtype or k_pages.device != v_pages.device:
             raise ValueError("k_pages and v_pages: two alike tensors (n_pages, page_size, kv_heads, head_size) are wanted")
         n_pages, page, kv, hs = k_pages.shape
         if k_pages.stride() != v_pages.stride() or k_pages.stride()[1:] != (kv * hs, hs, 1):
             raise ValueError("k_pages and v_pages: contiguous within a page, with the same distance between pages")
-        self._keep = (k_pages, v_pages)
+        if status is not None:
+            _indices(status, "status", (STATUS_WORDS,), k_pages.device)
+        self._keep = (k_pages, v_pages, status)
         self.device, self.n_heads, self.kv_heads, self.head_size, self.page_size = k_pages.device, int(n_heads), kv, hs, page
-        self.c = McaPagedCache(k_pages.data_ptr(), v_pages.data_ptr(), k_pages.stride(0), n_pages, page, self.n_heads, kv, hs, _dtype(k_pages, "k_pages"))
+        self.c = McaPagedCache(k_pages.data_ptr(), v_pages.data_ptr(), k_pages.stride(0), n_pages, page, self.n_heads, kv, hs, _dtype(k_pages, "k_pages"),
+                              None if status is None else status.data_ptr())
         self._ref = C.byref(self.c)
 
     def batch(self, starts, lengths, page_table, n_tokens, max_new, max_len):
@@ -223,12 +229,12 @@ class PagedCache:
               None if work is None else work.data_ptr(), max(need, 0))
 
     def status(self):
-        """What the calls on this device refused since the last time this was asked: (kind, detail, detail, how many), all zero if
-        nothing.  Waits for the device."""
+        """What the calls over this cache refused since the last time this was asked -- of a cache without status words of its own, what those
+        of all such callers on the device did: (kind, detail, detail, how many), all zero if nothing.  Waits for the device."""
         torch.cuda.synchronize(self.device)
         st = (C.c_int * 4)()
         with torch.cuda.device(self.device):
-            rc = self._lib.mca_paged_status(st)
+            rc = self._lib.mca_paged_status_of(self.c.status, st) if self.c.status else self._lib.mca_paged_status(st)
         if rc:
             raise PagedError(rc, "mca_paged_status")
         return tuple(st)

@@ -394,3 +394,106 @@ def test_logits_far_below_zero_behind_pages_that_are_gone(act, cache, hs, new, s
     s.cache.attend(s.batch, s.q, s.out)
     s.check()
     assert s.cache.status() == (0, 0, 0, 0)
+
+
+def with_words(s):
+    """The setup's cache with status words of its own, and a batch of it."""
+    from mycaffe_b200 import paged
+    words = torch.zeros(paged.STATUS_WORDS, dtype=torch.int32, device="cuda")
+    c = paged.PagedCache(s.k_pages, s.v_pages, s.heads, status=words)
+    return c, lambda lengths=s.lengths: c.batch(s.starts, lengths, s.table, s.n_tokens, s.max_new, s.max_len), words
+
+
+@pytest.mark.parametrize("act,cache", TYPES)
+def test_status_words_of_a_cache(act, cache):
+    """What a cache with words of its own refuses is told to those who ask it, and to no one else."""
+    from mycaffe_b200 import paged
+    a, b = (setup([(2, 40), (3, 50)], 4, 2, 64, 16, act, cache, seed=22 + i) for i in range(2))
+    (ca, ba, _), (cb, bb, _) = with_words(a), with_words(b)
+    bad = torch.tensor([40, 2], device="cuda", dtype=torch.int32)
+    rot = paged.QkNormRope(None, None, norm=False)
+    k, v = (torch.randn(a.n_tokens, 2, 64, device="cuda").to(a.act) for _ in range(2))
+    ca.attend(ba(bad), a.q, a.out)
+    cb.attend(bb(), b.q, b.out)
+    assert cb.status() == (0, 0, 0, 0) and a.cache.status() == (0, 0, 0, 0)
+    assert ca.status() == (1, 1, 2, 1) and ca.status() == (0, 0, 0, 0)
+    b.check()
+    cb.append(bb(bad), rot, b.q, k, v, torch.empty_like(b.q))
+    a.cache.attend(a.cache.batch(a.starts, bad, a.table, a.n_tokens, a.max_new, a.max_len), a.q, a.out)
+    assert ca.status() == (0, 0, 0, 0)
+    assert cb.status() == (1, 1, 2, 1) and a.cache.status() == (1, 1, 2, 1)
+
+
+@pytest.mark.parametrize("own", [False, True])
+def test_status_says_what_was_refused_first(own):
+    """The attention's refusal before the append's, and the other way round; all are counted."""
+    from mycaffe_b200 import paged
+    s = setup([(2, 40), (3, 50)], 4, 2, 64, 16, "bf16", "bf16", seed=24, drop=[(0, 1)])
+    c, batch, _ = with_words(s)
+    if not own:
+        c, batch = s.cache, lambda n=s.lengths: s.cache.batch(s.starts, n, s.table, s.n_tokens, s.max_new, s.max_len)
+    s.table[0, 1] = -7
+    bad = torch.tensor([40, 2], device="cuda", dtype=torch.int32)
+    rot = paged.QkNormRope(None, None, norm=False)
+    k, v = (torch.randn(s.n_tokens, 2, 64, device="cuda").to(s.act) for _ in range(2))
+    attend = lambda: c.attend(batch(), s.q, s.out)
+    append = lambda: c.append(batch(bad), rot, s.q, k, v, torch.empty_like(s.q))
+    attend()
+    torch.cuda.synchronize()
+    append()
+    st = c.status()
+    assert st[:3] == (2, 0, -7) and st[3] >= 2
+    append()
+    torch.cuda.synchronize()
+    attend()
+    st = c.status()
+    assert st[:3] == (1, 1, 2) and st[3] >= 2
+    assert c.status() == (0, 0, 0, 0)
+
+
+def test_function_ids_tell_each_handle_its_own_refusals():
+    """Two kernel indices of one device, and two handles of one: a refusal comes back to the caller that made it."""
+    import numpy as np
+    from mycaffe_b200 import CudaDnn, function_ids as ids
+    from mycaffe_b200.cudadnn import CudaDnnError
+    rng = np.random.default_rng(0)
+
+    def caller(cuda):
+        H, D, page, n = 2, 64, 16, 40
+        hP = cuda.CreatePaged(3, page, H, H, D)
+        x = [cuda.AllocMemory(rng.standard_normal(m).astype(np.float32)) for m in (n * H * D, 3 * page * H * D, 3 * page * H * D, n * H * D)]
+        ints = []
+        for a in ([0, n], [n], [0, 1, 2]):
+            ints.append(cuda.AllocMemory(len(a)))
+            cuda.SetMemoryInt32(ints[-1], np.array(a, np.int32))
+        return hP, ints[1], lambda: cuda.PagedAttention(hP, x[0], x[1], x[2], *ints, 3, 1, n, n, n, x[3])
+
+    one, two = CudaDnn(0), CudaDnn(0)
+    (hA, lenA, callA), (hB, _, callB), (hC, lenC, callC) = caller(one), caller(two), caller(one)
+    one.SetMemoryInt32(lenA, np.array([5], np.int32))
+    one.SetAsync(True)
+    callA()
+    two.SynchronizeDevice()
+    callB()                                       # another kernel index: none of its calls was refused
+    callC()                                       # another handle of the same one
+    with pytest.raises(CudaDnnError) as err:
+        one.SynchronizeDevice()
+    assert err.value.code == ids.ERROR_PARAM_OUT_OF_RANGE and "0 (5)" in err.value.native_message
+    one.SetAsync(False)
+    callB(), callC()
+    with pytest.raises(CudaDnnError):
+        callA()
+    one.SetMemoryInt32(lenA, np.array([40], np.int32))
+    callA()
+    one.SetMemoryInt32(lenC, np.array([3], np.int32))
+    one.SetAsync(True)
+    callC()
+    one.FreePaged(hC)                             # freed before anyone asked
+    callA()
+    with pytest.raises(CudaDnnError) as err:
+        one.SynchronizeDevice()
+    assert "0 (3)" in err.value.native_message
+    one.SynchronizeDevice()
+    two.FreePaged(hB)
+    one.Dispose()
+    two.Dispose()

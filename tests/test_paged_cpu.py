@@ -166,3 +166,27 @@ def test_python_checks():
     r = paged.QkNormRope(torch.zeros(8, 32), torch.zeros(8, 32))
     with pytest.raises(ValueError):
         r.check(128, k.device)
+
+
+def test_status_words(lib):
+    """A cache's own status words: 16-byte aligned, and asked for by their address."""
+    st = (C.c_int * 4)()
+    assert lib.mca_paged_status_of(None, st) == NULL and lib.mca_paged_status_of(A, None) == NULL
+    assert lib.mca_paged_status_of(A + 4, st) == OUT_OF_RANGE
+    c, b = cache(status=A + 4), batch()
+    assert attend(lib, c=c) == OUT_OF_RANGE
+    assert lib.mca_paged_attention_workspace_bytes(C.byref(c), C.byref(b), 2) == -1
+    assert lib.mca_paged_attention_workspace_bytes(C.byref(cache(status=A)), C.byref(b), 2) == lib.mca_paged_attention_workspace_bytes(
+        C.byref(cache()), C.byref(b), 2)
+
+
+def test_status_words_of_a_tensor():
+    torch = pytest.importorskip("torch")
+    from mycaffe_b200 import paged
+    k = torch.zeros(4, 16, 2, 64)
+    words = torch.zeros(paged.STATUS_WORDS, dtype=torch.int32)
+    assert paged.PagedCache(k, k.clone(), 4, status=words).c.status == words.data_ptr()
+    assert paged.PagedCache(k, k.clone(), 4).c.status is None
+    for bad in (words[:4], words.long(), torch.zeros(16, dtype=torch.int32)[::2]):
+        with pytest.raises(ValueError):
+            paged.PagedCache(k, k.clone(), 4, status=bad)
