@@ -613,7 +613,9 @@ MCA_API int mca_paged_attention(const McaPagedCache* cache, const McaPagedBatch*
  * caches have none, and of mca_qk_norm_rope_* (blocking; call after the stream has been synchronised): status4[0] = 0, or what was
  * refused first: 1 a sequence's lengths (status4[1] = the sequence, [2] = its length), 2 a page id ([1] = the sequence, [2] = the id), 3 a
  * position outside the tables ([1] = the token row, [2] = the position); status4[3] = how many.  4: a bounded wait of the attention kernel
- * gave up ([1] = the stage, [2] = the block), and its output is not complete; what was refused besides is left for the next reading. */
+ * gave up ([1] = the stage, [2] = the block), and its output is not complete; what was refused besides is left for the next reading.
+ * Until it has been read, the attention calls on the tensor cores (bf16 pages) that record in the same words compute nothing: their output
+ * stays as it was. */
 MCA_API int mca_paged_status(int* status4);
 /* The same from the words of a cache (McaPagedCache::status), on its device. */
 MCA_API int mca_paged_status_of(int* status, int* status4);

@@ -855,12 +855,13 @@ __global__ void __launch_bounds__(TC_THREADS, (TcPlan<HDP, FEW>::CTAS)) paged_tc
   if (tid == 32) {
     s_wait_words = p.batch.status + paged::WAIT_WORDS;
     s_abort = *reinterpret_cast<volatile int*>(s_wait_words);
+    if (p.meta != nullptr) p.meta[2 * blockIdx.x].x = -1;   // no item ends here that another CTA began, unless the producer finds one
   }
   tc_fence_before();
   __syncthreads();
   tc_fence_after();
   const uint32_t tmem_base = *tmem_slot;
-  if (s_abort != 0) {   // an earlier CTA gave up (a uniform decision, before any copy or product)
+  if (s_abort != 0) {   // a CTA of this call or, until its words are read, an earlier one gave up (a uniform decision, before any copy or product)
     if (warp == TC_WARP_MMA) tmem_dealloc(tmem_base, PL::TMEM);
     return;
   }
@@ -887,7 +888,6 @@ __global__ void __launch_bounds__(TC_THREADS, (TcPlan<HDP, FEW>::CTAS)) paged_tc
     int issued_k = 0, issued_v = 0;
     Walk w;
     w.begin(p, blockIdx.x);
-    if (p.meta != nullptr && lane == 0) p.meta[2 * blockIdx.x].x = -1;   // no item ends here that another CTA began, unless found below
     bool more = w.left > 0, first = true;
     while (ok) {
       int kt0 = 0, kt1 = 0;
@@ -1319,11 +1319,12 @@ template <typename T>
 __global__ void __launch_bounds__(256) paged_join_kernel(const AttnArgs p) {
   mca_pdl_launch_dependents();
   mca_pdl_wait();
+  const int gave_up = __ldcg(p.batch.status + paged::WAIT_WORDS);   // then there are parts that nobody wrote
   const int4 m0 = __ldcg(p.meta + 2 * blockIdx.x);
   const int heads = __ldcg(p.meta + 2 * blockIdx.x + 1).x;
   const int r = threadIdx.x & ((1 << p.row_shift) - 1), lanes = 256 >> p.row_shift, quads = p.hs / 4;
   const int q0 = blockIdx.y * lanes * JOIN_QUADS + (threadIdx.x >> p.row_shift);
-  if (m0.x < 0 || r >= m0.w || q0 >= quads) return;
+  if (gave_up != 0 || m0.x < 0 || r >= m0.w || q0 >= quads) return;
   const int first = m0.x, n = (int)blockIdx.x - first + 1;
   auto slot = [&](int k) { return 2ll * (first + k) + (k == 0 ? 1 : 0); };   // the first CTA's last part, then the others' first ones
   const float2* ml = reinterpret_cast<const float2*>(p.part_ml) + r;

@@ -497,3 +497,48 @@ def test_function_ids_tell_each_handle_its_own_refusals():
     two.FreePaged(hB)
     one.Dispose()
     two.Dispose()
+
+
+@pytest.mark.parametrize("act", ["bf16", "f32"])
+@pytest.mark.parametrize("seqs", [[(2, 5003), (1, 129), (2, 2500)], [(300, 2000), (5, 700), (2, 40)]])
+def test_calls_after_a_wait_that_gave_up(act, seqs):
+    """With the wait words set (by the self-check's wait, which nothing arrives for) a call touches neither the output nor anything
+    else, whatever its workspace holds; once they are read it is right again, and what was refused meanwhile is told after them."""
+    import ctypes as C
+    from mycaffe_b200 import paged
+    s = setup(seqs, 8, 2, 64, 16, act, "bf16", seed=25, pad=3)
+    c, batch, words = with_words(s)
+    wide = torch.full((s.n_tokens + 8, 10, 64), 7.0, device="cuda", dtype=s.act)
+    out = wide[4:-4, 1:9]
+    lib, dt = c._lib, paged._DTYPES[s.act]
+    shape = tuple(s.q.shape)
+    q, o = (paged._heads(t, "t", shape, s.act, t.device) for t in (s.q, out))
+
+    def attend(b, work):
+        stream = torch.cuda.current_stream().cuda_stream
+        return lib.mca_paged_attention(c._ref, b.ref, dt, C.byref(q), 0.0, C.byref(o), work.data_ptr(), work.numel(), stream)
+
+    b = batch()
+    need = lib.mca_paged_attention_workspace_bytes(c._ref, b.ref, dt)
+    assert need > 0
+    work = torch.ones(need // 4, dtype=torch.int32, device="cuda").view(torch.uint8)   # block 1's row 1 of one row, wherever it is read as such
+    assert lib.mca_wait_probe(words.data_ptr() + 16, 1000, torch.cuda.current_stream().cuda_stream) == 0
+    torch.cuda.synchronize()
+    assert words.tolist() == [0, 0, 0, 0, 1, 99, 0, 0]
+    assert attend(b, work) == 0
+    torch.cuda.synchronize()
+    assert (wide == 7.0).all()
+    bad = s.lengths.clone()
+    bad[1] = seqs[1][1] + s.max_len
+    assert attend(batch(bad), work) == 0
+    assert c.status() == (4, 99, 0, 1)
+    rows = slice(4 + seqs[0][0], 4 + seqs[0][0] + seqs[1][0])
+    assert not wide[rows, 1:9].any()                   # a refused sequence's rows are zeros as ever
+    wide[rows, 1:9] = 7.0
+    assert (wide == 7.0).all()
+    assert c.status() == (1, 1, seqs[1][1] + s.max_len, 1) and c.status() == (0, 0, 0, 0)
+    assert attend(b, work) == 0
+    s.out = out.contiguous()
+    s.check()
+    wide[4:-4, 1:9] = 7.0
+    assert (wide == 7.0).all() and c.status() == (0, 0, 0, 0)
