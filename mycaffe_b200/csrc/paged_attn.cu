@@ -233,7 +233,7 @@ __global__ void __launch_bounds__(SIMT_THREADS, R <= 2 ? 2 : 1) paged_simt_kerne
       float s = s2.x + s2.y;
 #pragma unroll
       for (int o = G / 2; o > 0; o >>= 1) s += __shfl_xor_sync(0xffffffffu, s, o);
-      if (valid && row <= lim[x]) {
+      if (valid && row <= lim[x] && s != -INFINITY) {   // a logit of minus infinity weighs nothing, also before the first of another kind
         if (s > m[x]) {   // the running maximum moves (rare once it has settled): rescale what was accumulated
           const float f = tc::fast_exp2(m[x] - s);
           l[x] *= f;

@@ -542,3 +542,19 @@ def test_calls_after_a_wait_that_gave_up(act, seqs):
     s.check()
     wide[4:-4, 1:9] = 7.0
     assert (wide == 7.0).all() and c.status() == (0, 0, 0, 0)
+
+
+@pytest.mark.parametrize("act,cache,heads,new", [("f32", "f32", 2, 1), ("f32", "f32", 4, 1), ("f32", "f32", 8, 1), ("f32", "f32", 4, 40),
+                                                 ("f32", "bf16", 2, 1), ("bf16", "bf16", 4, 1), ("bf16", "bf16", 4, 40)])
+@pytest.mark.parametrize("n", [100, 1500])
+def test_logits_of_minus_infinity_weigh_nothing(act, cache, heads, new, n):
+    """Keys whose logits are minus infinity, met first, in between and alone, through each of the kernels."""
+    s = setup([(new, n), (new, n), (new, new)], heads, 2, 64, 16, act, cache, seed=26)
+    s.q[..., 3] = s.q[..., 3].abs() + 0.125
+    for b, at in enumerate([list(range(21)) + [40, 41, 57, 90], list(range(0, n, 2)), range(new)]):
+        for pos in at:
+            s.k_pages[int(s.table[b, pos // 16]), pos % 16, :, 3] = -math.inf
+            s.held[b][pos] = False
+    s.cache.attend(s.batch, s.q, s.out)
+    s.check()
+    assert not s.out[2 * new:].any()
