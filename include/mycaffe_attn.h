@@ -598,8 +598,9 @@ MCA_API int mca_qk_norm_rope_backward(const McaQkRotation* rotation, const McaHe
 MCA_API int mca_paged_append(const McaPagedCache* cache, const McaPagedBatch* batch, const McaQkRotation* rotation, int dtype,
                              const McaHeads* q, const McaHeads* k, const McaHeads* v, const McaHeads* q_out, void* stream);
 /* Attention of the new tokens over their sequences' pages, the new tokens' own keys among them (append first):
- * out_t = sum over j <= position(t) of softmax_j(scale q_t . k_j) v_j; scale 0: 1 / sqrt(head_size).  A token with no key left has a
- * zero row; a value that is not finite reaches the tokens that see it and no others.  q, out (n_tokens, n_heads, D) in dtype:
+ * out_t = sum over j <= position(t) of softmax_j(scale q_t . k_j) v_j; scale 0: 1 / sqrt(head_size), else positive, and scale x log2(e) a
+ * normal float.  A token with no key left, or with none but such whose logits are minus infinity, has a zero row; a value that is not
+ * finite reaches the tokens that see it and no others.  q, out (n_tokens, n_heads, D) in dtype:
  *   fp32 over fp32 pages     exact fp32 products;
  *   fp32 over bf16 pages     exact fp32 products where a key serves one query row of a sequence; else queries and probabilities as two
  *                            bf16 halves each, 3e-6 of the output in the 2-norm;

@@ -1533,7 +1533,8 @@ int mca_paged_attention(const McaPagedCache* cache, const McaPagedBatch* batch, 
   AttnArgs a;
   int e = paged::check(cache, batch, &a.batch);
   if (e || (e = check_types(cache, dtype))) return e;
-  if (!(scale >= 0.f) || scale > 3.0e38f) return ERROR_PARAM_OUT_OF_RANGE;
+  // as a power of two's factor it has to be a normal number too: minus infinity times a zero is no mask, nor is infinity a factor
+  if (scale != 0.f && !(scale * LOG2E >= FLT_MIN && scale * LOG2E <= FLT_MAX)) return ERROR_PARAM_OUT_OF_RANGE;
   if (batch->n_tokens == 0) return 0;
   if ((e = paged::check_heads(q, dtype, false)) || (e = paged::check_heads(out, dtype, false))) return e;
   Plan plan;

@@ -218,7 +218,9 @@ class PagedCache:
 
     def attend(self, batch, q, out, scale=None):
         """out = attention of the new tokens' q over their sequences' pages (their own keys among them); both (n_tokens, heads,
-        head_size).  scale None: 1 / sqrt(head_size)."""
+        head_size).  scale: positive; None: 1 / sqrt(head_size)."""
+        if scale is not None and not scale > 0.0:   # the C side's zero is its default
+            raise ValueError(f"scale: a positive number or None is wanted, got {scale}")
         dev, shape = self.device, (batch.n_tokens, self.n_heads, self.head_size)
         dt = _dtype(q, "q")
         a, o = _heads(q, "q", shape, q.dtype, dev), _heads(out, "out", shape, q.dtype, dev)

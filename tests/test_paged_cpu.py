@@ -190,3 +190,21 @@ def test_status_words_of_a_tensor():
     for bad in (words[:4], words.long(), torch.zeros(16, dtype=torch.int32)[::2]):
         with pytest.raises(ValueError):
             paged.PagedCache(k, k.clone(), 4, status=bad)
+
+
+def test_scales(lib):
+    """Zero is the C side's default; what is not a positive factor in powers of two is refused, and by the tensors' call zero too."""
+    for bad in (-0.125, -1e-45, 1e-45, 1e-38 / 2, 2.5e38, 3.4e38, float("inf"), float("nan")):
+        assert attend(lib, scale=bad) == OUT_OF_RANGE, bad
+    b = batch(n_tokens=0)
+    for good in (0.0, -0.0, 1e-37, 2.3e38):
+        assert attend(lib, b=b, scale=good) == 0, good
+    torch = pytest.importorskip("torch")
+    from mycaffe_b200 import paged
+    k = torch.zeros(4, 16, 2, 64)
+    c = paged.PagedCache(k, k.clone(), 4)
+    i = lambda *n: torch.zeros(*n, dtype=torch.int32)
+    b, q = c.batch(i(3), i(2), i(2, 4), 3, 2, 64), torch.zeros(3, 4, 64)
+    for bad in (0.0, -0.125, float("nan")):
+        with pytest.raises(ValueError):
+            c.attend(b, q, q.clone(), scale=bad)
