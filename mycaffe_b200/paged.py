@@ -172,7 +172,7 @@ class PagedBatch:
     """A step's new tokens (see ``PagedCache.batch``)."""
 
     def __init__(self, c, n_tokens, keep):
-        self.c, self.ref, self.n_tokens, self._keep = c, C.byref(c), n_tokens, keep
+        self.c, self.ref, self.n_tokens, self.device, self._keep = c, C.byref(c), n_tokens, keep[0].device, keep
 
 
 class PagedCache:
@@ -205,10 +205,15 @@ class PagedCache:
                           _indices(page_table, "page_table", (n, stride), dev), stride, n, n_tokens, max_new, max_len)
         return PagedBatch(c, n_tokens, (starts, lengths, page_table))
 
+    def _device_of(self, batch):
+        if batch.device != self.device:
+            raise ValueError(f"batch: its arrays are on {batch.device}, the pages on {self.device}")
+        return self.device
+
     def append(self, batch, rotation, q, k, v, q_out):
         """Norm and rotation of the new tokens' q into q_out and of k into the pages; v into its pages.  q, q_out (n_tokens, heads,
         head_size), k, v (n_tokens, kv_heads, head_size)."""
-        n, dev = batch.n_tokens, self.device
+        n, dev = batch.n_tokens, self._device_of(batch)
         rotation.check(self.head_size, dev)
         dt, qs, ks = _dtype(q, "q"), (n, self.n_heads, self.head_size), (n, self.kv_heads, self.head_size)
         a = (_heads(q, "q", qs, q.dtype, dev), _heads(k, "k", ks, q.dtype, dev), _heads(v, "v", ks, q.dtype, dev),
@@ -221,7 +226,7 @@ class PagedCache:
         head_size).  scale: positive; None: 1 / sqrt(head_size)."""
         if scale is not None and not scale > 0.0:   # the C side's zero is its default
             raise ValueError(f"scale: a positive number or None is wanted, got {scale}")
-        dev, shape = self.device, (batch.n_tokens, self.n_heads, self.head_size)
+        dev, shape = self._device_of(batch), (batch.n_tokens, self.n_heads, self.head_size)
         dt = _dtype(q, "q")
         a, o = _heads(q, "q", shape, q.dtype, dev), _heads(out, "out", shape, q.dtype, dev)
         need = self._lib.mca_paged_attention_workspace_bytes(self._ref, batch.ref, dt)

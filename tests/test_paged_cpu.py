@@ -208,3 +208,17 @@ def test_scales(lib):
     for bad in (0.0, -0.125, float("nan")):
         with pytest.raises(ValueError):
             c.attend(b, q, q.clone(), scale=bad)
+
+
+def test_a_batch_of_another_device_is_refused():
+    torch = pytest.importorskip("torch")
+    from mycaffe_b200 import paged
+    k, far = torch.zeros(4, 16, 2, 64), torch.zeros(4, 16, 2, 64, device="meta")
+    c, other = paged.PagedCache(k, k.clone(), 4), paged.PagedCache(far, far.clone(), 4)
+    i = lambda *n: torch.zeros(*n, dtype=torch.int32)
+    b = c.batch(i(3), i(2), i(2, 4), 3, 2, 64)
+    q, kv = torch.zeros(3, 4, 64, device="meta"), torch.zeros(3, 2, 64, device="meta")
+    with pytest.raises(ValueError, match="batch"):
+        other.attend(b, q, q.clone())
+    with pytest.raises(ValueError, match="batch"):
+        other.append(b, paged.QkNormRope(None, None), q, kv, kv, q.clone())
