@@ -558,3 +558,22 @@ def test_logits_of_minus_infinity_weigh_nothing(act, cache, heads, new, n):
     s.cache.attend(s.batch, s.q, s.out)
     s.check()
     assert not s.out[2 * new:].any()
+
+
+@pytest.mark.parametrize("act,cache", TYPES)
+@pytest.mark.parametrize("heads,kv", [(65, 1), (71, 1), (129, 1), (142, 1), (300, 2)])
+@pytest.mark.parametrize("seqs", [[(1, 700), (1, 1), (1, 130)], [(1, 2), (5, 300), (20, 20)]])
+def test_more_heads_to_a_key_than_a_tile_has_rows(act, cache, heads, kv, seqs):
+    """The query heads that share a key fill more than one tile: parts of the group, whole and ragged."""
+    s = setup(seqs, heads, kv, 32, 16, act, cache, seed=27, pad=2, drop=[(0, 0)] if seqs[0][1] > 16 else ())
+    s.cache.attend(s.batch, s.q, s.out)
+    s.check()
+    assert s.cache.status() == (0, 0, 0, 0)
+
+
+@pytest.mark.parametrize("act,cache", TYPES)
+@pytest.mark.parametrize("heads,kv", [(5, 1), (14, 2), (21, 3), (24, 2)])
+def test_groups_that_do_not_divide_a_tile(act, cache, heads, kv):
+    s = setup([(1, 900), (150, 400), (33, 33), (2, 129)], heads, kv, 128, 32, act, cache, seed=28)
+    s.cache.attend(s.batch, s.q, s.out)
+    s.check()

@@ -286,3 +286,39 @@ def test_prompt_in_chunks_and_token_by_token(act, cache):
     tol = {"f32f32": 1e-5, "f32bf16": 2e-4, "bf16bf16": 4 * 2.0 ** -8}[act + cache] * whole.abs().amax()
     assert (whole - parts).abs().amax() <= tol
     assert s.cache.status() == (0, 0, 0, 0)
+
+
+@pytest.mark.parametrize("dtype", ["f32", "bf16"])
+@pytest.mark.parametrize("halves", [False, True])
+def test_positions_with_norm_and_weights(dtype, halves):
+    """Explicit positions, some twice, some outside the tables: the norm, both inputs' gradients and both weights' follow them."""
+    from mycaffe_b200 import paged
+    gen = torch.Generator("cuda").manual_seed(7)
+    B, T, H, KV, D, dt = 3, 37, 5, 2, 96, DT[dtype]
+    cos, sin = tables(50, D, gen)
+    wq, wk = (1 + 0.3 * torch.randn(D, device="cuda", generator=gen) for _ in range(2))
+    rot = paged.QkNormRope(cos, sin, wq, wk, eps=EPS, halves=halves)
+    pos = torch.randint(0, 50, (B, T), device="cuda", generator=gen, dtype=torch.int32)
+    pos[0, 3], pos[2, 36] = 50, -1
+    good = ((pos >= 0) & (pos < 50))[:, :, None, None]
+    at = pos.clamp(0, 49).long()
+    c64, s64 = cos.double()[at][:, :, None], sin.double()[at][:, :, None]
+    x = [torch.randn(B, T, h, D, device="cuda", generator=gen).to(dt) for h in (H, KV)]
+    g = [torch.randn(B, T, h, D, device="cuda", generator=gen).to(dt) for h in (H, KV)]
+    y, dx = [torch.full_like(t, 7.0) for t in x], [torch.full_like(t, 7.0) for t in x]
+    rot.forward(*x, *y, positions=pos)
+    dw = rot.backward(*x, *g, *dx, positions=pos)
+    for i, w in enumerate((wq, wk)):
+        x64, w64 = x[i].double().requires_grad_(), w.double().requires_grad_()
+        ref = torch.where(good, formula(x64, w64, c64, s64, True, halves), 0.0)
+        grads = torch.autograd.grad(ref, [x64, w64], g[i].double())
+        # the bounds of test_forward_and_backward
+        close(y[i], ref.detach(), dt, pair_size(ref.detach(), halves), D / 2 + 12)
+        inv = 1 / torch.sqrt((x64 * x64).mean(-1, keepdim=True) + EPS).detach()
+        size, unit = pair_size(g[i].double(), halves), (x64 * inv).detach()
+        big = size * w64.detach().abs()
+        close(dx[i], grads[0], dt, inv * (big + unit.abs() * (big * unit.abs()).mean(-1, keepdim=True)), 2 * D + 20)
+        total = (size * unit.abs()).sum((0, 1, 2))
+        over = ((dw[i].double() - grads[1]).abs() / (total * (D / 2 + 16 + B * T * x[i].shape[2]) * 2.0 ** -24)).amax().item()
+        assert over <= 1.0, over
+    paged.PagedCache(torch.zeros(1, 16, 1, 64, device="cuda"), torch.zeros(1, 16, 1, 64, device="cuda"), 1).status()
