@@ -1370,6 +1370,7 @@ long paged_create(Kernel* k, long lInput, float* pf, long llInput, MCA_LONGLONG*
   const bool turn = pf[0] > 0.f;   // theta <= 0: no rotation, as DECODE_CREATE
   if (turn && (pl[6] < 1 || pl[6] > (1 << 24))) return ERROR_PARAM_OUT_OF_RANGE;
   c.page_stride = (int64_t)c.page_size * c.n_kv_heads * c.head_size;
+  if (c.n_pages > INT64_MAX / c.page_stride) return ERROR_PARAM_OUT_OF_RANGE;   // what the pages' handles are checked against
   const size_t status_bytes = MCA_PAGED_STATUS_WORDS * sizeof(int);
   if (cudaMalloc(&p.status, status_bytes) != cudaSuccess || cudaMemset(p.status, 0, status_bytes) != cudaSuccess) { cudaGetLastError(); p.release(); return ERROR_MEMORY_OUT; }
   c.status = p.status;

@@ -577,3 +577,15 @@ def test_groups_that_do_not_divide_a_tile(act, cache, heads, kv):
     s = setup([(1, 900), (150, 400), (33, 33), (2, 129)], heads, kv, 128, 32, act, cache, seed=28)
     s.cache.attend(s.batch, s.q, s.out)
     s.check()
+
+
+def test_a_pool_of_more_elements_than_64_bits_count_is_refused():
+    """Its size would wrap, and handles that are far too small would pass for its pages."""
+    from mycaffe_b200 import CudaDnn, function_ids as ids
+    from mycaffe_b200.cudadnn import CudaDnnError
+    cuda = CudaDnn(0)
+    with pytest.raises(CudaDnnError) as err:
+        cuda.CreatePaged(1 << 26, 1 << 16, 1 << 15, 1 << 15, 128)      # 2^64 elements
+    assert err.value.code == ids.ERROR_PARAM_OUT_OF_RANGE
+    cuda.FreePaged(cuda.CreatePaged(1 << 24, 1 << 16, 1 << 15, 1 << 15, 128))   # 2^62
+    cuda.Dispose()
