@@ -602,9 +602,13 @@ MCA_API int mca_paged_append(const McaPagedCache* cache, const McaPagedBatch* ba
  * normal float.  A token with no key left, or with none but such whose logits are minus infinity, has a zero row; a value that is not
  * finite reaches the tokens that see it and no others.  q, out (n_tokens, n_heads, D) in dtype:
  *   fp32 over fp32 pages     exact fp32 products;
- *   fp32 over bf16 pages     exact fp32 products where a key serves one query row of a sequence; else queries and probabilities as two
- *                            bf16 halves each, 3e-6 of the output in the 2-norm;
- *   bf16 over bf16 pages     probabilities rounded to bf16, sums in fp32.
+ *   fp32 over bf16 pages     exact fp32 products where no key serves more than one query row of a sequence (max_new x n_heads / n_kv_heads
+ *                            is 1); else queries and probabilities as two bf16 halves each: a logit is off by up to 2^-16 of the sum of
+ *                            the magnitudes of its terms, and an output by up to twice that relative to the mean magnitude of its values
+ *                            (3e-6 in the 2-norm for queries, keys and values of unit variance); max_new thus chooses between the two.  An
+ *                            infinite key may make NaN of the rows that see it, where the others' products give it the weight 0;
+ *   bf16 over bf16 pages     probabilities rounded to bf16, sums in fp32.  (bf16 activations over fp32 pages are refused: what append would
+ *                            put there are bf16 numbers.)
  * out must not overlap q or the pages.  workspace: mca_paged_attention_workspace_bytes bytes, 16-byte aligned (0: none is needed; -1:
  * arguments that mca_paged_attention refuses); two calls that may overlap, two captured graphs among them, need one each. */
 MCA_API int64_t mca_paged_attention_workspace_bytes(const McaPagedCache* cache, const McaPagedBatch* batch, int dtype);

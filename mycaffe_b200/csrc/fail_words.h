@@ -3,8 +3,8 @@
 // load behind its one stream synchronisation that nothing failed.  (Copying the status words back after every call cost a
 // 3 us transfer and its launch on each.)  A device's kernels know their row's address by a symbol of each translation
 // unit, set when a kernel index is initialised; null (raw callers) means no word is raised.
-// The rows are per device because the status words are: a call lowers a word before it reads the status array behind it, and
-// the array it reads is its own device's.
+// The rows are per device: a call lowers a word before it reads the status words behind it, and those it reads are its own
+// device's.  Where the words are a handle's, as those of attention handles and paged caches, see g_fail and paged_may_have_failed.
 #pragma once
 
 enum McaFailWord : int { MCA_FAIL_TC = 0, MCA_FAIL_DECODE = 1, MCA_FAIL_PROJ = 2, MCA_FAIL_PAGED = 3, MCA_FAIL_WORDS = 4 };

@@ -6,7 +6,8 @@
 // tile (row = token x group + head), so that a page is read once for all of them.  The kernels:
 //
 //   paged_tc_kernel      bf16 pages: S = Q K^T and O += P V on the tensor cores (tcgen05, TMEM), pages by TMA.
-//   paged_simt_kernel    fp32 activations, up to four rows: exact fp32 products, a lane group per cache row.
+//   paged_simt_kernel    fp32 activations over fp32 pages up to eight rows, four at a time, and over bf16 pages one row: exact fp32 products,
+//                        a lane group per cache row.
 //   paged_tile_kernel    fp32 pages, more rows: exact fp32 products on tiles in shared memory.
 //   paged_join_kernel, paged_simt_join_kernel   results of one row from several CTAs, each with some of the keys, joined by their maxima and sums.
 #include <algorithm>
@@ -565,9 +566,10 @@ __global__ void __launch_bounds__(128) paged_simt_join_kernel(const AttnArgs p) 
 //   warp 9      MMA issuer (an elected lane), owner of the TMEM allocation.
 // FEW: no sequence has more rows than a tile, so pages are read once: bound by memory.  One CTA per SM with all its shared
 //   memory in K and V stages (192 KB on their way), two S tiles, so that the next product runs under this one's softmax.  64 sequences of
-//   up to 4096 keys, 32 / 8 heads of 128: 114 us for 700 MB, 6.1 TB/s (two CTAs of one stage each: 145).
+//   up to 4096 keys, 32 / 8 heads of 128: 112 us for 700 MB, 6.2 TB/s (two CTAs of one stage each: 145).
 // else: tiles share their keys through L2, and the products bound: two CTAs per SM, one's softmax under the other's products.  2048 tokens
-//   over 16384, 32 / 8 heads of 128: 534 us, 1.09 PFLOP/s in short runs; 613 under the power cap.
+//   over 16384, 32 / 8 heads of 128: 605 us call after call, 0.97 PFLOP/s at 1485 MHz; the tensor pipe is 62 % active, between a tile's S and
+//   its P V it waits for the softmax.
 // fp32 activations (ACT32) over bf16 pages: a query row q is two bf16 rows of the tile, hi = bf16(q) and lo = bf16(q - hi), 16
 // lanes apart, so that one product S = [hi; lo] K^T forms both and the softmax warp adds them (the pages are bf16 as they are: q
 // to 2^-16 is all that is rounded); the probabilities go back the same way, [p_hi; p_lo], and the two halves of O are added at the
@@ -575,7 +577,9 @@ __global__ void __launch_bounds__(128) paged_simt_join_kernel(const AttnArgs p) 
 using namespace tc;
 
 constexpr int KEYS = 128;   // of a key tile
-constexpr int ITEM_UNITS = 2;   // queries in, sums out: 4500 cycles where a key tile takes 3200 (prompts of up to 1000 tokens: 48.4 us with 1, 46.6 with 2, 45.7 with 3)
+// Queries in, sums out: 4500 cycles where a key tile takes 3200.  Eight prompts of 400 to 1000 tokens, with 1, 2, 3 and 4: 16 heads of 64 46.1, 45.0, 45.3,
+// 45.7 us, 32 / 8 of 128 112, 98.6, 93.3, 92.5; 32 prompts of 33 to 160, 16 of 64: 26.2, 24.7, 26.1, 25.7; steps of single tokens the same within 3 %.
+constexpr int ITEM_UNITS = 2;
 
 template <int HDP, bool FEW> struct TcPlan {   // HDP: 64 or 128, the head size padded
   static constexpr int SUB = HDP / 64;
@@ -1179,8 +1183,9 @@ __global__ void __launch_bounds__(TC_THREADS, (TcPlan<HDP, FEW>::CTAS)) paged_tc
                 }
               }
             }
-            // p = 2^(s scale - m), handed over in three pieces (64, 32, 32 keys); the sum is of the unrounded ones.  Of a row that has seen no
-            // key all s are minus infinity, and any finite m gives the zeros
+            // p = 2^(s scale - m), handed over in three pieces (64, 32, 32 keys); the sum is of the unrounded ones.  They are rounded to bf16, the type of the
+            // values they multiply (fp32 activations: to two halves, 2^-16): with the output's own rounding 2.3e-3 off in the 2-norm, that alone
+            // 1.7e-3.  Of a row that has seen no key all s are minus infinity, and any finite m gives the zeros
             const float nm[2] = {-fmaxf(m_used[0], -FLT_MAX), -fmaxf(m_used[1], -FLT_MAX)};
             const float2 nm2[2] = {make_float2(nm[0], nm[0]), make_float2(nm[1], nm[1])};
             float2 rs[2] = {make_float2(0.f, 0.f), make_float2(0.f, 0.f)};
@@ -1428,7 +1433,10 @@ int make_plan(const McaPagedCache* c, const McaPagedBatch* b, int dtype, Plan* o
     out->ctas = (int)std::min((double)(out->few ? 148 : 296), std::max(1.0, std::ceil(units / out->least_units)));
     const int items = out->parts * c->n_kv_heads;
     out->span = out->ctas; out->inner = items;
-    if (out->ctas / items * items * 8 >= out->ctas * 7) {   // at most an eighth of the CTAs is left out
+    // each head CTAs of its own where that leaves out at most an eighth of them.  64 sequences of 1200 to 4000 keys, heads of 64, with / without: 12 heads
+    // (144 of 148 CTAs) 110 / 126 us, 20 (140) 178 / 202, 32 (128: a seventh, and so without) 302 / 316, 40 (120) 398 / 391; four prompts of 400 to
+    // 1000, 128-wide: 12 heads (288 of 296) 37.0 / 36.5, 20 (280) 48.1 / 49.4
+    if (out->ctas / items * items * 8 >= out->ctas * 7) {
       out->span = out->ctas / items; out->inner = 1;
       out->ctas = out->span * items;
     }
@@ -1436,7 +1444,10 @@ int make_plan(const McaPagedCache* c, const McaPagedBatch* b, int dtype, Plan* o
     out->bytes = out->join ? (int64_t)out->ctas * (2ll * out->rows_max * (c->head_size + 2) * 4 + 32) : 0;
     return 0;
   }
-  // fp32 pages: more than eight rows on tiles, fewer a lane group a key, four rows a CTA
+  // fp32 pages: more than eight rows on tiles, fewer a lane group a key, four rows a CTA, which read a sequence's keys once for each four.  16 tokens over 500 to
+  // 1500 keys, rows x 4 heads of 64 over 4, tiles / lane groups: 5 rows 36.0 / 26.2 us, 8 36.0 / 34.0, 9 36.4 / 41.6, 16 37.1 / 55.7; 128-wide 5 62 / 46,
+  // 8 62 / 49, 9 62 / 65, 16 63 / 83.  In steps that leave most of the machine empty the lane groups are ahead for longer (three chunks over 100 to 500 keys,
+  // 8 heads of 64: 9 rows 19.5 / 10.8, 24 23.6 / 11.4): the rule is that of full ones.
   out->rows = most_rows > 8 ? TILE_ROWS : (most_rows > 2 ? 4 : (int)most_rows);
   const int64_t tiles = most_rows <= out->rows ? b->n_seqs : (int64_t)b->n_tokens * group / out->rows + b->n_seqs;
   if (tiles >= (1ll << 30)) return ERROR_PARAM_OUT_OF_RANGE;
@@ -1445,7 +1456,8 @@ int make_plan(const McaPagedCache* c, const McaPagedBatch* b, int dtype, Plan* o
   const int tile_bytes = (TILE_ROWS + TILE_KEYS) * (c->head_size + 4) * 4 + TILE_KEYS * (c->head_size + TILE_ROWS + 4) * 4 + 2048;
   const int slots = out->rows == TILE_ROWS ? 148 * (227 * 1024 / tile_bytes) : (out->rows == 4 ? 148 : 296);
   // time in keys of one CTA: whole waves of (set-up + the keys of a split); more than one split also writes partial results (at some 5 TB/s)
-  // and joins them in some 4 us.  128 keys take a lane group's CTA about a microsecond, a tile's eight.
+  // and joins them in some 4 us.  128 keys take a lane group's CTA about a microsecond, a tile's eight (of 48-wide heads; with 5, 14 and 24 for them the splits, and the
+  // times of 19 of 20 steps of 32- to 128-wide heads, are the same: only four prompts of up to 200 over 512, 16 heads of 64, take 53 us from 14 on for 69).
   const double key_us = (out->rows == TILE_ROWS ? 8.0 : 1.0) / 128.0;
   const double part_keys = (double)b->n_tokens * c->n_heads * c->head_size * 8.0 / 5e6 / key_us, join_keys = 4.0 / key_us;
   double best = 1e300;

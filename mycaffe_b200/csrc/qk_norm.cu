@@ -20,7 +20,7 @@ using paged::Batch;
 constexpr int THREADS = 256;
 // Heads of one token that a group takes at once, forward and backward, and the CTAs per SM that registers are left for.  fp32 rows are four
 // elements a piece and gain from more warps (8 x 1024 x 24 heads of 64, forward and backward: 48.1 us with four and two heads and three CTAs,
-// 45.8 so); bf16 ones are eight, are bound by the instructions of a piece and spill in fewer registers (2 x 4095 x 40 heads of 128: 91 us,
+// 45.6 so); bf16 ones are eight, are bound by the instructions of a piece and spill in fewer registers (2 x 4095 x 40 heads of 128: 91 us,
 // with three CTAs 160, with pieces of four 112).
 template <typename T> constexpr int HEADS = sizeof(T) == 4 ? 2 : 4;
 template <typename T> constexpr int HEADS_BWD = sizeof(T) == 4 ? 1 : 2;

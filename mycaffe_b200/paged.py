@@ -223,7 +223,7 @@ class PagedCache:
 
     def attend(self, batch, q, out, scale=None):
         """out = attention of the new tokens' q over their sequences' pages (their own keys among them); both (n_tokens, heads,
-        head_size).  scale: positive; None: 1 / sqrt(head_size)."""
+        head_size), and out not overlapping q or the pages.  scale: positive; None: 1 / sqrt(head_size)."""
         if scale is not None and not scale > 0.0:   # the C side's zero is its default
             raise ValueError(f"scale: a positive number or None is wanted, got {scale}")
         dev, shape = self._device_of(batch), (batch.n_tokens, self.n_heads, self.head_size)
