@@ -543,7 +543,8 @@ typedef struct McaPagedCache {
 #define MCA_PAGED_STATUS_WORDS 8
 /* The new tokens of a step: those of sequence b are rows [starts[b], starts[b+1]) of the token tensors, the last of its
  * lengths[b] positions (so lengths counts them: token i of the sequence has position lengths[b] - (starts[b+1] - starts[b]) + i).
- * starts rises from 0 on; a sequence may have none (its length and pages are then not looked at).  Rows behind starts[n_seqs], up to n_tokens, are not read and not written.
+ * starts rises from 0 on; a sequence may have none (its length and pages are then not looked at).  Rows behind starts[n_seqs], up to
+ * n_tokens, are not read and not written.  Up to 65535 sequences and heads, 2^30 tokens and positions; append: n_tokens x n_heads below 2^31.
  * starts, lengths and page_table are device memory; what the host knows of them is an upper bound: no sequence has more than max_new
  * new tokens or max_len positions (max_len <= table_stride * page_size).  A sequence outside these bounds, or with fewer positions
  * than new tokens, is refused on the device: nothing of it is read or stored, those of its rows that lie below n_tokens are zero, and
@@ -579,7 +580,7 @@ typedef struct McaHeads {
 /* The norm and rotation for training.  q (B,T,n_heads,D) and k (B,T,n_kv_heads,D) -> q_out, k_out, fp32 or bf16 (dtype), arithmetic
  * in fp32 with one rounding at the end.  positions: (B,T) device ints, or null: 0 .. T-1 of every batch item (then T <= table_len); a
  * position outside the tables gives a zero row, which mca_paged_status reports.  An output may be its own input (same data and
- * strides); other overlaps are not allowed.  D: a multiple of 16 up to 256.  k (and k_out, dk_out, dk) may be null with n_kv_heads 0. */
+ * strides); other overlaps are not allowed.  D: a multiple of 16 up to 256; B x T x heads below 2^31.  k (and k_out, dk_out, dk) may be null with n_kv_heads 0. */
 MCA_API int mca_qk_norm_rope_forward(const McaQkRotation* rotation, const McaHeads* q, const McaHeads* k, const int* positions, int dtype,
                                      int B, int T, int n_heads, int n_kv_heads, int D, const McaHeads* q_out, const McaHeads* k_out,
                                      void* stream);
