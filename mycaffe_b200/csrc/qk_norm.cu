@@ -530,7 +530,7 @@ int check_norm(const McaQkRotation* rotation, const McaHeads* const (&views)[6],
   int e = check_rotation(rotation, D, &a->r);
   if (e) return e;
   if (B <= 0 || T <= 0 || n_heads <= 0 || n_kv_heads < 0) return ERROR_PARAM_OUT_OF_RANGE;
-  if ((int64_t)B * T * std::max(n_heads, n_kv_heads) >= (1ll << 31)) return ERROR_PARAM_OUT_OF_RANGE;
+  if ((int64_t)B * T >= (1ll << 31) || (int64_t)B * T * std::max(n_heads, n_kv_heads) >= (1ll << 31)) return ERROR_PARAM_OUT_OF_RANGE;
   if (rotation->cos_table && !positions && T > rotation->table_len) return ERROR_PARAM_OUT_OF_RANGE;
   if ((uintptr_t)positions & 3) return ERROR_PARAM_OUT_OF_RANGE;
   for (int i = 0; i < n_views; ++i) {

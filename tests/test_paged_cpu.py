@@ -222,3 +222,12 @@ def test_a_batch_of_another_device_is_refused():
         other.attend(b, q, q.clone())
     with pytest.raises(ValueError, match="batch"):
         other.append(b, paged.QkNormRope(None, None), q, kv, kv, q.clone())
+
+
+def test_norm_rows_beyond_31_bits(lib):
+    """B x T x heads is bounded where it does not wrap, too: (2^31 - 1)^2 x 4 is negative in 64 bits."""
+    r, q, k = rotation(), heads(4), heads(2)
+    call = lambda B, T, H, KV: lib.mca_qk_norm_rope_forward(C.byref(r), C.byref(q), C.byref(k), A, 2, B, T, H, KV, 64, C.byref(q), C.byref(k), None)
+    most = (1 << 31) - 1
+    for B, T, H, KV in [(most, most, 4, 2), (most, most, 2, 4), (1 << 16, 1 << 15, 1, 1), (1 << 16, 1 << 14, 2, 1), (1 << 16, 1 << 14, 1, 2), (1, most, 3, 0)]:
+        assert call(B, T, H, KV) == OUT_OF_RANGE, (B, T, H, KV)
