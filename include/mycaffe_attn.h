@@ -557,7 +557,8 @@ typedef struct McaPagedBatch {
 } McaPagedBatch;
 /* Norm of each head and rotation by position, y = R(position) (w o x / sqrt(mean(x^2) + eps)).  MCA_QK_NORM: with the norm; the
  * weights are (head_size) floats shared by the heads, or null: ones.  Tables (table_len, head_size / 2) as mca_rope_tables_host
- * builds them, or both null: no rotation.  MCA_ROPE_HALVES: pair p is (x[p], x[p + head_size / 2]); else the reference's (x[2p],
+ * builds them (the reference's angles, products in fp32: at position 10^5 up to 0.007 off; for far positions hand over tables formed
+ * in 64 bits), or both null: no rotation.  MCA_ROPE_HALVES: pair p is (x[p], x[p + head_size / 2]); else the reference's (x[2p],
  * x[2p+1]) (rope.cu:724-864). */
 #define MCA_QK_NORM 1
 #define MCA_ROPE_HALVES 2
@@ -571,7 +572,8 @@ typedef struct McaQkRotation {
   float eps;
 } McaQkRotation;
 /* A (B, T, heads, head_size) view: head_size contiguous, the other strides in elements.  Base 16-byte aligned, strides multiples of
- * 16 bytes.  Where there are token rows instead of (B, T), stride_b is not used. */
+ * 16 bytes.  Where there are token rows instead of (B, T), stride_b is not used.  The rows of an input may lie on one another (a stride of
+ * 0), those of an output must not. */
 typedef struct McaHeads {
   void* data;
   int64_t stride_b, stride_t, stride_h;

@@ -55,13 +55,15 @@ def _dtype(t, what):
     return _DTYPES[t.dtype]
 
 
-def _heads(t, what, shape, dtype, device):
-    """A (..., heads, head_size) tensor as the C side sees it; rows of heads are read where they lie."""
+def _heads(t, what, shape, dtype, device, written=False):
+    """A (..., heads, head_size) tensor as the C side sees it; rows of heads are read, or written, where they lie."""
     s = t.stride()
     if t.shape != shape or t.dtype is not dtype or t.device != device:
         raise ValueError(f"{what}: {tuple(shape)} of {dtype} on {device} is wanted, got {tuple(t.shape)} of {t.dtype} on {t.device}")
     if s[-1] != 1:
         raise ValueError(f"{what}: a head's elements have to be contiguous")
+    if written and 0 in s and any(step == 0 and n > 1 for step, n in zip(s, t.shape)):
+        raise ValueError(f"{what}: an expanded tensor's rows lie on one another and cannot be written")
     return McaHeads(t.data_ptr(), s[0] if len(s) == 4 else 0, s[-3], s[-2])
 
 
@@ -146,8 +148,8 @@ class QkNormRope:
         (B,heads,T,D) tensors, parts of a packed projection).  k and k_out may be None."""
         B, T, H, KV, D, dt, pos = self._common(q, k, positions)
         dev, qs, ks = q.device, (B, T, H, D), (B, T, KV, D)
-        a = [_heads(q, "q", qs, q.dtype, dev), _heads(q_out, "q_out", qs, q.dtype, dev)]
-        b = [None, None] if k is None else [C.byref(_heads(k, "k", ks, q.dtype, dev)), C.byref(_heads(k_out, "k_out", ks, q.dtype, dev))]
+        a = [_heads(q, "q", qs, q.dtype, dev), _heads(q_out, "q_out", qs, q.dtype, dev, True)]
+        b = [None, None] if k is None else [C.byref(_heads(k, "k", ks, q.dtype, dev)), C.byref(_heads(k_out, "k_out", ks, q.dtype, dev, True))]
         _call(dev, "mca_qk_norm_rope_forward", self._lib.mca_qk_norm_rope_forward, C.byref(self.c), C.byref(a[0]), b[0], pos, dt, B, T, H, KV, D,
               C.byref(a[1]), b[1])
 
@@ -156,8 +158,8 @@ class QkNormRope:
         None for a weight that there is not (or with ``weight_grads`` False)."""
         B, T, H, KV, D, dt, pos = self._common(q, k, positions)
         dev, qs, ks = q.device, (B, T, H, D), (B, T, KV, D)
-        a = [C.byref(_heads(t, n, qs, q.dtype, dev)) for t, n in ((q, "q"), (dq_out, "dq_out"), (dq, "dq"))]
-        b = [None] * 3 if k is None else [C.byref(_heads(t, n, ks, q.dtype, dev)) for t, n in ((k, "k"), (dk_out, "dk_out"), (dk, "dk"))]
+        a = [C.byref(_heads(t, n, qs, q.dtype, dev, t is dq)) for t, n in ((q, "q"), (dq_out, "dq_out"), (dq, "dq"))]
+        b = [None] * 3 if k is None else [C.byref(_heads(t, n, ks, q.dtype, dev, t is dk)) for t, n in ((k, "k"), (dk_out, "dk_out"), (dk, "dk"))]
         want = (weight_grads and self.weights[0], weight_grads and self.weights[1] and k is not None)
         dw = [torch.empty(D, device=dev) if w else None for w in want]
         need = self._lib.mca_qk_norm_rope_backward_scratch_floats(D) if any(want) else 0
@@ -171,8 +173,8 @@ class QkNormRope:
 class PagedBatch:
     """A step's new tokens (see ``PagedCache.batch``)."""
 
-    def __init__(self, c, n_tokens, keep):
-        self.c, self.ref, self.n_tokens, self.device, self._keep = c, C.byref(c), n_tokens, keep[0].device, keep
+    def __init__(self, c, n_tokens, device, keep):
+        self.c, self.ref, self.n_tokens, self.device, self._keep = c, C.byref(c), n_tokens, device, keep
 
 
 class PagedCache:
@@ -203,10 +205,10 @@ class PagedCache:
         n, stride, dev = lengths.shape[0], page_table.shape[-1], self.device
         c = McaPagedBatch(_indices(starts, "starts", (n + 1,), dev), _indices(lengths, "lengths", (n,), dev),
                           _indices(page_table, "page_table", (n, stride), dev), stride, n, n_tokens, max_new, max_len)
-        return PagedBatch(c, n_tokens, (starts, lengths, page_table))
+        return PagedBatch(c, n_tokens, dev, (starts, lengths, page_table))
 
     def _device_of(self, batch):
-        if batch.device != self.device:
+        if batch.device is not self.device and batch.device != self.device:   # a batch of this cache has this cache's own object
             raise ValueError(f"batch: its arrays are on {batch.device}, the pages on {self.device}")
         return self.device
 
@@ -217,7 +219,7 @@ class PagedCache:
         rotation.check(self.head_size, dev)
         dt, qs, ks = _dtype(q, "q"), (n, self.n_heads, self.head_size), (n, self.kv_heads, self.head_size)
         a = (_heads(q, "q", qs, q.dtype, dev), _heads(k, "k", ks, q.dtype, dev), _heads(v, "v", ks, q.dtype, dev),
-             _heads(q_out, "q_out", qs, q.dtype, dev))
+             _heads(q_out, "q_out", qs, q.dtype, dev, True))
         _call(dev, "mca_paged_append", self._lib.mca_paged_append, self._ref, batch.ref, C.byref(rotation.c), dt, C.byref(a[0]), C.byref(a[1]),
               C.byref(a[2]), C.byref(a[3]))
 
@@ -228,7 +230,7 @@ class PagedCache:
             raise ValueError(f"scale: a positive number or None is wanted, got {scale}")
         dev, shape = self._device_of(batch), (batch.n_tokens, self.n_heads, self.head_size)
         dt = _dtype(q, "q")
-        a, o = _heads(q, "q", shape, q.dtype, dev), _heads(out, "out", shape, q.dtype, dev)
+        a, o = _heads(q, "q", shape, q.dtype, dev), _heads(out, "out", shape, q.dtype, dev, True)
         need = self._lib.mca_paged_attention_workspace_bytes(self._ref, batch.ref, dt)
         # of the current stream's allocator (or a captured graph's own pool): no two calls that overlap share it
         work = torch.empty(need, dtype=torch.uint8, device=dev) if need > 0 else None

@@ -231,3 +231,29 @@ def test_norm_rows_beyond_31_bits(lib):
     most = (1 << 31) - 1
     for B, T, H, KV in [(most, most, 4, 2), (most, most, 2, 4), (1 << 16, 1 << 15, 1, 1), (1 << 16, 1 << 14, 2, 1), (1 << 16, 1 << 14, 1, 2), (1, most, 3, 0)]:
         assert call(B, T, H, KV) == OUT_OF_RANGE, (B, T, H, KV)
+
+
+def test_outputs_whose_rows_lie_on_one_another_are_refused():
+    """An expanded tensor is an input like any other; as an output its rows would race for the same memory."""
+    torch = pytest.importorskip("torch")
+    from mycaffe_b200 import paged
+    k = torch.zeros(4, 16, 2, 64)
+    c = paged.PagedCache(k, k.clone(), 4)
+    i = lambda *n: torch.zeros(*n, dtype=torch.int32)
+    b, q, kv = c.batch(i(3), i(2), i(2, 4), 3, 2, 64), torch.zeros(3, 4, 64), torch.zeros(3, 2, 64)
+    rot = paged.QkNormRope(None, None)
+    refused = lambda what: pytest.raises(ValueError, match=f"{what}: an expanded")
+    for out in (torch.zeros(1, 4, 64).expand(3, 4, 64), torch.zeros(3, 1, 64).expand(3, 4, 64)):
+        with refused("out"):
+            c.attend(b, q, out)
+        with refused("q_out"):
+            c.append(b, rot, q, kv, kv, out)
+        x, y, wide = q[None], kv[None], out[None]
+        with refused("q_out"):
+            rot.forward(x, y, wide, y.clone())
+        with refused("k_out"):
+            rot.forward(x, y, x.clone(), torch.zeros(1, 3, 1, 64).expand(1, 3, 2, 64))
+        with refused("dq"):
+            rot.backward(x, y, out[None], y, wide, y.clone())
+        with refused("dk"):
+            rot.backward(x, y, wide, y, x.clone(), torch.zeros(1, 1, 2, 64).expand(1, 3, 2, 64))
