@@ -705,23 +705,26 @@ long sync_and_collect_status(Kernel* k) {
   const long se = sync_call(k);
   if (se) return se;
   long first = 0;
+  std::string detail;   // of the same failure as the code
+  auto note = [&](long e) {
+    if (e && !first) { first = e; detail = k->last_detail; }
+  };
   for (auto& kv : k->attn) {
     if (!kv.second.status_pending) continue;
     kv.second.status_pending = false;
-    const long e = read_status(k, kv.second);
-    if (e && !first) first = e;
+    note(read_status(k, kv.second));
   }
   if (k->paged_left != 0) {
-    if (!first) first = k->paged_left;
     k->last_detail = k->paged_left_detail;
+    note(k->paged_left);
     k->paged_left = 0;
   }
   for (auto& kv : k->paged) {
     if (!kv.second.pending) continue;
     kv.second.pending = false;
-    const long e = paged_status(k, kv.second);
-    if (e && !first) first = e;
+    note(paged_status(k, kv.second));
   }
+  k->last_detail = detail;
   return first;
 }
 

@@ -589,3 +589,30 @@ def test_a_pool_of_more_elements_than_64_bits_count_is_refused():
     assert err.value.code == ids.ERROR_PARAM_OUT_OF_RANGE
     cuda.FreePaged(cuda.CreatePaged(1 << 24, 1 << 16, 1 << 15, 1 << 15, 128))   # 2^62
     cuda.Dispose()
+
+
+def test_the_message_belongs_to_the_error_that_is_returned():
+    """A wait that gave up and a refused sequence, both in asynchronous mode: the code is the first's, and so is the text."""
+    import numpy as np
+    from mycaffe_b200 import CudaDnn, function_ids as ids
+    from mycaffe_b200.cudadnn import CudaDnnError
+    cuda = CudaDnn(0)
+    H, D, page, n = 2, 64, 16, 40
+    hCudnn = cuda.CreateCuDNN()
+    hAttn = cuda.CreateAttn()
+    cuda.SetAttn(hCudnn, hAttn, 0, True, 1, 256, 2, 64, 0.0, 0, ids.MCA_DTYPE_BF16, ids.MCA_FLAG_CAUSAL_IMPLICIT)
+    hP = cuda.CreatePaged(3, page, H, H, D)
+    x = [cuda.AllocMemory(np.ones(m, np.float32)) for m in (n * H * D, 3 * page * H * D, 3 * page * H * D, n * H * D)]
+    ints = []
+    for a in ([0, n], [5], [0, 1, 2]):
+        ints.append(cuda.AllocMemory(len(a)))
+        cuda.SetMemoryInt32(ints[-1], np.array(a, np.int32))
+    cuda.SetAsync(True)
+    cuda._invoke(ids.MCA_FN_WAIT_PROBE, None, [hAttn, 1000])
+    cuda.PagedAttention(hP, x[0], x[1], x[2], *ints, 3, 1, n, n, n, x[3])
+    with pytest.raises(CudaDnnError) as err:
+        cuda.SynchronizeDevice()
+    assert err.value.code == ids.ERROR_ATTN_KERNEL_TIMEOUT
+    assert "stage 99" in err.value.native_message and "lengths" not in err.value.native_message
+    cuda.SynchronizeDevice()
+    cuda.Dispose()
